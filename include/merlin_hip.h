@@ -17,7 +17,8 @@
  *   - every launch is asynchronous on `stream` (a hipStream_t passed as void*; NULL = the
  *     default stream) and ordered with respect to that stream only.
  *   - no exceptions cross the ABI, no torch / C++ types appear in signatures.
- *   - all floating point data is IEEE fp32; ids are int32 or int64 (MH_I32 / MH_I64).
+ *   - all floating point data is IEEE fp32 unless an entry point takes a type code (MH_F32 / MH_BF16 / MH_F16);
+ *     ids are int32 or int64 (MH_I32 / MH_I64).
  */
 #ifndef MERLIN_HIP_H
 #define MERLIN_HIP_H
@@ -37,6 +38,11 @@ extern "C" {
 /* id dtypes */
 #define MH_I32 0
 #define MH_I64 1
+
+/* element types of the entry points that take one */
+#define MH_F32 0
+#define MH_BF16 1
+#define MH_F16 2
 
 /* activations, keras names: linear / relu / sigmoid (blocks/mlp.py:35-139) */
 #define MH_ACT_NONE 0
@@ -693,6 +699,30 @@ int32_t mh_sharded_lookup_bwd(mh_comm_t comm, int32_t F, int64_t B, int64_t capa
                               float* local_shards, float* state, float* state2, int64_t local_rows_total,
                               int32_t optimizer, float lr, float eps, float beta1, float beta2, const float* lr_device,
                               void* workspace, int64_t workspace_bytes, mh_stream_t stream);
+
+/* ---- 8-bit products with a scale for each block of 128 --------------------------------------------------------------------
+ * The Dense layer (tf/blocks/mlp.py:275-280) with e4m3 operands.  An 8-bit matrix of R rows and K columns is
+ *   q       [R, ldq] e4m3, ldq >= ceil(K / 128) * 128, a multiple of 16; the columns past K up to the whole block are zero;
+ *   scales  [R, lds] bytes, lds >= ceil(K / 128) rounded up to 4, a multiple of 4; byte b of a row is e + 127 for its block b of 128
+ *           columns, which stands for q * 2^e.  Bytes past the last block are not used (the quantiser writes 127).
+ * mh_fp8_quantize: x [R, K] (type code dtype, leading dimension ldx) to that form, e the least integer with max |x| <= 448 * 2^e over the
+ * block (at least -126; 0 for a block of zeros), values rounded to nearest, ties to even; an infinity or NaN becomes NaN and does not
+ * enter the scale.  transpose != 0: the matrix stored is x^T -- K rows of R columns, blocks along the rows of x; colsum (optional, then
+ * only, [K] floats) receives the column sums of x in a fixed order, from a workspace of ceil(R / 128) * K floats.
+ * mh_fp8_matmul: out[M, N] = a b^T + bias, a [M, K] and b [N, K] in that form, bias [N] floats or NULL, out of type out_dtype with leading
+ * dimension ldo.  An MH_F32 or MH_F16 output is summed in 32 bits throughout; an MH_BF16 one by the 8-bit matrix instruction, at twice the
+ * rate, whose sums are off by at most 7 * 2^-13 of sum |a b| (under half a step of bf16; 1.5e-5 of the norm on random values).  mh_fp8_linear: x [M, K] quantised into the workspace, then the product with w [N, K].
+ * No atomics: results do not change from call to call.  Rows past M and columns past N of out are left as they were. */
+int32_t mh_fp8_quantize(const void* x, int32_t dtype, int64_t ldx, int64_t R, int64_t K, int32_t transpose, void* q, int64_t ldq,
+                        void* scales, int64_t lds, float* colsum, void* workspace, int64_t workspace_bytes, mh_stream_t stream);
+int64_t mh_fp8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int32_t mh_fp8_matmul(const void* a, int64_t lda, const void* a_scales, int64_t ldas, const void* b, int64_t ldb, const void* b_scales,
+                      int64_t ldbs, int64_t M, int64_t N, int64_t K, const float* bias, int32_t out_dtype, void* out, int64_t ldo,
+                      void* workspace, int64_t workspace_bytes, mh_stream_t stream);
+int64_t mh_fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int32_t mh_fp8_linear(const void* x, int32_t x_dtype, int64_t ldx, const void* w, int64_t ldw, const void* w_scales, int64_t ldws,
+                      int64_t M, int64_t N, int64_t K, const float* bias, int32_t out_dtype, void* out, int64_t ldo, void* workspace,
+                      int64_t workspace_bytes, mh_stream_t stream);
 
 /* ---- launch recorder: a train step traced once, replayed without re-entering the host language ----------------------------
  * Replaces the role of Keras' traced `train_function` (BaseModel.fit -> make_train_function, models/base.py:1361-1421): between

@@ -15,6 +15,7 @@ from . import build as _build
 
 MH_OK = 0
 MH_I32, MH_I64 = 0, 1
+MH_F32, MH_BF16, MH_F16 = 0, 1, 2
 ACT = {"linear": 0, None: 0, "none": 0, "relu": 1, "sigmoid": 2}
 COMBINER = {"sum": 0, "mean": 1, "sqrtn": 2, "max": 3}
 OPT = {"sgd": 0, "adagrad": 1, "adam": 2, "lazy_adam": 2}
@@ -113,6 +114,11 @@ SIGNATURES = {
     "mh_bce_fwd_bwd": (_i32, [_p, _p, _i64, _f32, _p, _p, _p]),
     "mh_bce_mean_fwd_bwd": (_i32, [_p, _p, _i64, _f32, _p, _p, _p, _p]),
     "mh_mean": (_i32, [_p, _i64, _p, _p, _p]),
+    "mh_fp8_quantize": (_i32, [_p, _i32, _i64, _i64, _i64, _i32, _p, _i64, _p, _i64, _p, _p, _i64, _p]),
+    "mh_fp8_matmul_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "mh_fp8_matmul": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _i32, _p, _i64, _p, _i64, _p]),
+    "mh_fp8_linear_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "mh_fp8_linear": (_i32, [_p, _i32, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _i32, _p, _i64, _p, _i64, _p]),
     "mh_record_begin": (_i32, []),
     "mh_record_end": (_i32, [C.POINTER(_p)]),
     "mh_record_abort": (_i32, []),

@@ -1,0 +1,597 @@
+// Products of e4m3 matrices with a power-of-two scale for every row and every 128 entries of the summed axis, and the quantiser that makes
+// such matrices: the Dense layer of ``mh_linear_bias_act_fwd`` (tf/blocks/mlp.py:275-280) with 8-bit operands.
+//
+//   quantise  e = the least integer with max |x| <= 448 2^e over a block; stored: e4m3(x 2^-e), ties to even, and the byte e + 127
+//   product   C[m, n] = sum_b 2^(ea[m, b] + eb[n, b]) sum_{k in b} a[m, k] b[n, k]  (+ bias[n])
+//
+// A power of two as the scale makes x 2^-e exact, so a matrix is quantised to the same bits wherever it is done, and it is the form that the
+// scaled matrix instruction takes beside its operands: the scales cost no vector instruction in the loop.  Both operands are stored with the
+// summed axis contiguous and padded with zeros to whole blocks, so the loop has no tail in k.
+#include "mh_lowp.h"
+
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+// ---- quantiser -----------------------------------------------------------------------------------------------------------------------
+// The scale's exponent from the block's largest magnitude: amax = 1.f 2^(E - 127) <= 448 2^e = 1.75 2^(8 + e) for e = E - 135, one more where
+// 1.f > 1.75.  -126 below keeps 2^e and 2^-e normal numbers.
+__device__ __forceinline__ int q_exponent(float amax) {
+    const uint32_t b = __float_as_uint(amax);
+    if (b == 0) return 0;
+    const int e = (int)(b >> 23) - 135 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return e < -126 ? -126 : e;
+}
+__device__ __forceinline__ float q_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+// |v| where v is finite, else 0: an infinity or NaN becomes NaN in e4m3 and leaves its block's scale to the others
+__device__ __forceinline__ float q_mag(float v) {
+    const float a = fabsf(v);
+    return a <= 3.402823466e38f ? a : 0.f;
+}
+__device__ __forceinline__ float q_in(float v) { return fabsf(v) <= 3.402823466e38f ? v : __uint_as_float(0x7fc00000u); }
+__device__ __forceinline__ uint32_t q_pack4(float a, float b, float c, float d) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(q_in(a), q_in(b), 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q_in(c), q_in(d), w, true);
+}
+
+// Blocks along the rows of x.  A wavefront takes four blocks (512 entries, 8 a lane: 16 lanes share a block) of one row and writes one word of
+// scales; one pass, bound by its reads.
+template <typename T>
+__global__ __launch_bounds__(256) void fp8_quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t R, int K, int quads, uint8_t* __restrict__ q,
+                                                               int64_t ldq, uint8_t* __restrict__ s, int64_t lds) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)(blockIdx.x / (uint32_t)quads) * 4 + (threadIdx.x >> 6);
+    const int quad = (int)(blockIdx.x % (uint32_t)quads);
+    if (row >= R) return;
+    const int k = quad * 512 + lane * 8;
+    float v[8];
+    const T* p = x + row * ldx + k;
+    if (k + 8 <= K) {
+        lp_load8(p, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = k + i < K ? lp_float(p[i]) : 0.f;
+    }
+    float a = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a = fmaxf(a, q_mag(v[i]));
+#pragma unroll
+    for (int m = 8; m; m >>= 1) a = fmaxf(a, __shfl_xor(a, m));
+    const int e = q_exponent(a);
+    const float inv = q_pow2(-e);
+    const int kp = (K + 127) / 128 * 128;
+    if (k < kp) {
+        uint2 w;
+        w.x = q_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+        w.y = q_pack4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+        *reinterpret_cast<uint2*>(q + row * ldq + k) = w;
+    }
+    uint32_t sw = 0;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) sw |= (uint32_t)(__shfl(e, 16 * b) + 127) << (8 * b);
+    if (lane == 0) *reinterpret_cast<uint32_t*>(s + row * lds + quad * 4) = sw;
+}
+
+// Blocks along the columns of x: q[c, r] = x[r, c].  A workgroup takes 128 rows x 64 columns; a wavefront reads 16 rows, whole lines, and the
+// tile turns round in LDS so that eight lanes write one 128-byte line of q.  colsum, if given, receives the tile's column sums ([blocks, C]).
+template <typename T>
+__global__ __launch_bounds__(512) void fp8_quantize_cols_kernel(const T* __restrict__ x, int64_t ldx, int64_t R, int64_t C, int rblocks, int sbytes,
+                                                               uint8_t* __restrict__ q, int64_t ldq, uint8_t* __restrict__ s, int64_t lds,
+                                                               float* __restrict__ colsum) {
+    __shared__ float red[8][64], red2[8][64];
+    __shared__ __attribute__((aligned(16))) uint8_t tile[64][144];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int rb = (int)(blockIdx.x % (uint32_t)rblocks);
+    const int64_t c0 = (int64_t)(blockIdx.x / (uint32_t)rblocks) * 64, c = c0 + lane;
+    const int64_t r0 = (int64_t)rb * 128 + w * 16;
+    float v[16], a = 0.f, t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = (c < C && r0 + i < R) ? lp_float(x[(r0 + i) * ldx + c]) : 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        a = fmaxf(a, q_mag(v[i]));
+        t += v[i];
+    }
+    red[w][lane] = a;
+    red2[w][lane] = t;
+    __syncthreads();
+    t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        a = fmaxf(a, red[i][lane]);
+        t += red2[i][lane];
+    }
+    const int e = q_exponent(a);
+    const float inv = q_pow2(-e);
+    uint4 o;
+    o.x = q_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+    o.y = q_pack4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+    o.z = q_pack4(v[8] * inv, v[9] * inv, v[10] * inv, v[11] * inv);
+    o.w = q_pack4(v[12] * inv, v[13] * inv, v[14] * inv, v[15] * inv);
+    *reinterpret_cast<uint4*>(&tile[lane][w * 16]) = o;
+    if (w == 0 && c < C) {
+        s[c * lds + rb] = (uint8_t)(e + 127);
+        if (rb == rblocks - 1)
+            for (int b = rblocks; b < sbytes; ++b) s[c * lds + b] = 127;
+        if (colsum) colsum[(int64_t)rb * C + c] = t;
+    }
+    __syncthreads();
+    const int64_t cc = c0 + threadIdx.x / 8;
+    if (cc < C) *reinterpret_cast<uint4*>(q + cc * ldq + rb * 128 + (threadIdx.x % 8) * 16) = *reinterpret_cast<const uint4*>(&tile[threadIdx.x / 8][(threadIdx.x % 8) * 16]);
+}
+
+// out[c] = sum_b part[b, c], in order
+__global__ __launch_bounds__(256) void fp8_colsum_kernel(const float* __restrict__ part, int blocks, int64_t C, float* __restrict__ out) {
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (c >= C) return;
+    float t = 0.f;
+    for (int b = 0; b < blocks; ++b) t += part[(int64_t)b * C + c];
+    out[c] = t;
+}
+
+// ---- product -------------------------------------------------------------------------------------------------------------------------
+struct F8Args {
+    const uint8_t *a, *as, *b, *bs;
+    int64_t lda, ldas, ldb, ldbs;
+    int64_t M, N;
+    int kblocks, kb_split;  // blocks of 128 in all, and in each slice of blockIdx.y (a multiple of 4)
+    int mt, nt, per_xcd;    // output tiles, and how many of them an XCD takes
+    const float* bias;
+    int kind;  // MH_F32 / MH_BF16 / MH_F16
+    void* out;
+    int64_t ldo, slab;  // slab: entries between the slices' partial outputs
+    int vec;            // four entries of an output row can be stored together
+};
+
+__device__ __forceinline__ void f8_dma16(const void* g, void* l) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g, (__attribute__((address_space(3))) void*)l, 16, 0, 0);
+}
+__device__ __forceinline__ void f8_dma4(const void* g, void* l) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g, (__attribute__((address_space(3))) void*)l, 4, 0, 0);
+}
+
+// 32 e4m3 of one row, scaled, as four operands of the bf16 matrix instruction: e4m3 has 4 significant bits and bf16 8, so nothing is lost
+__device__ __forceinline__ void f8_widen(const i32x8& v, float scale, bf16x8 (&o)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const bf16x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * j], scale, false), p1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * j], scale, true);
+        const bf16x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * j + 1], scale, false), p3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * j + 1], scale, true);
+        o[j] = bf16x8{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
+    }
+}
+
+__device__ __forceinline__ void f8_store4(const F8Args& g, int64_t m, int64_t n, float v0, float v1, float v2, float v3, int64_t slab) {
+    const int64_t at = slab + m * g.ldo + n;
+    const float v[4] = {v0, v1, v2, v3};
+    if (g.vec && n + 4 <= g.N) {
+        if (g.kind == MH_F32) {
+            *reinterpret_cast<f32x4*>(static_cast<float*>(g.out) + at) = f32x4{v0, v1, v2, v3};
+        } else {
+            uint2 w;
+            w.x = g.kind == MH_BF16 ? lp_pack_bf16(v0, v1) : lp_pack_f16(v0, v1);
+            w.y = g.kind == MH_BF16 ? lp_pack_bf16(v2, v3) : lp_pack_f16(v2, v3);
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(g.out) + at) = w;
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (n + i < g.N) {
+            if (g.kind == MH_F32) static_cast<float*>(g.out)[at + i] = v[i];
+            else static_cast<uint16_t*>(g.out)[at + i] = (uint16_t)(g.kind == MH_BF16 ? lp_pack_bf16(v[i], 0.f) : lp_pack_f16(v[i], 0.f));
+        }
+}
+
+// Tiled product.  WIDE: operands widened to bf16 on the way from LDS, for outputs of fp32 and fp16.  The 8-bit matrix instruction takes its
+// products in groups of eight and cuts each at 2^-13 of the group's largest (measured with single products on both shapes; the groups' sums
+// are then added in fp32): at most 7 2^-13 = 2^-10.2 of sum |a b|, 1.5e-5 of the norm on random values.  Half a step of a bf16 output is 2^-8 of
+// the result and hides that; the finer types take the bf16 instruction, which adds in fp32, at half the rate.
+// Each wavefront holds (BM / WM) x (BN / WN) of the output as 32 x 32 accumulators, rows of b as the instruction's rows: a lane then owns four
+// neighbouring columns of C.  Tiles of one block of k (128 bytes a row) come by direct-to-LDS loads, two stages, one barrier a block; 16-byte
+// chunk c of row r lies at c ^ ((r >> 1) & 7), which spreads the 16 rows of a read phase over all 64 banks.
+template <int BM, int BN, int WM, int WN, bool WIDE>
+__global__ __launch_bounds__(WM * WN * 64, 2) void fp8_gemm_kernel(const F8Args g) {
+    constexpr int NT = WM * WN * 64, TM = BM / WM / 32, TN = BN / WN / 32;
+    constexpr int STAGE = (BM + BN) * 128, DMA = STAGE / 16 / NT, SCALES = (BM + BN) * 4, SDMA = SCALES / 4 / NT;
+    static_assert(SDMA * NT * 4 == SCALES && DMA * NT * 16 == STAGE, "every thread issues the same number of loads");
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;
+    const int wm = wave / WN, wn = wave % WN;
+    // tile of this workgroup: consecutive workgroups go to the eight XCDs in turn, so each XCD takes a run of tiles of its own, in groups of
+    // eight tile rows: the tiles in flight on one L2 share their operands' panels
+    const int tile = (int)(blockIdx.x & 7) * g.per_xcd + (int)(blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= g.per_xcd || tile >= g.mt * g.nt) return;
+    const int group = tile / (8 * g.nt), in = tile - group * 8 * g.nt, rows = g.mt - group * 8 < 8 ? g.mt - group * 8 : 8;
+    const int64_t m0 = (int64_t)(group * 8 + in % rows) * BM, n0 = (int64_t)(in / rows) * BN;
+    const int kb0 = blockIdx.y * g.kb_split, kb1 = kb0 + g.kb_split < g.kblocks ? kb0 + g.kb_split : g.kblocks;
+
+    const uint8_t* src[DMA];
+#pragma unroll
+    for (int j = 0; j < DMA; ++j) {
+        const int L = j * NT + threadIdx.x, r = L >> 3, c = (L & 7) ^ ((r >> 1) & 7);
+        if (r < BM) {
+            const int64_t row = m0 + r < g.M ? m0 + r : g.M - 1;  // rows past the end repeat the last: never stored
+            src[j] = g.a + row * g.lda + c * 16;
+        } else {
+            const int64_t row = n0 + r - BM < g.N ? n0 + r - BM : g.N - 1;
+            src[j] = g.b + row * g.ldb + c * 16;
+        }
+    }
+    const uint8_t* ssrc[SDMA];
+#pragma unroll
+    for (int j = 0; j < SDMA; ++j) {
+        const int r = j * NT + threadIdx.x;
+        if (r < BM) ssrc[j] = g.as + (m0 + r < g.M ? m0 + r : g.M - 1) * g.ldas;
+        else ssrc[j] = g.bs + (n0 + r - BM < g.N ? n0 + r - BM : g.N - 1) * g.ldbs;
+    }
+    uint8_t* const sbase = smem + 2 * STAGE;
+    auto issue = [&](int kb) {
+        uint8_t* st = smem + (kb & 1) * STAGE;
+#pragma unroll
+        for (int j = 0; j < DMA; ++j) f8_dma16(src[j] + (int64_t)kb * 128, st + (j * NT + wave * 64) * 16);
+        if ((kb & 3) == 0) {  // four blocks' scales, one word a row
+#pragma unroll
+            for (int j = 0; j < SDMA; ++j) f8_dma4(ssrc[j] + kb, sbase + ((kb >> 2) & 1) * SCALES + (j * NT + wave * 64) * 4);
+        }
+    };
+    f32x16 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    int ar[TM], br[TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) ar[i] = wm * (BM / WM) + i * 32 + l31;
+#pragma unroll
+    for (int j = 0; j < TN; ++j) br[j] = BM + wn * (BN / WN) + j * 32 + l31;
+    uint32_t sa[TM], sb[TN];
+    issue(kb0);
+    for (int kb = kb0; kb < kb1; ++kb) {
+        // block kb has arrived, and every wavefront is done with the stage that block kb + 1 takes
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (kb + 1 < kb1) issue(kb + 1);
+        const uint8_t* st = smem + (kb & 1) * STAGE;
+        if ((kb & 3) == 0) {
+            const uint32_t* sp = reinterpret_cast<const uint32_t*>(sbase + ((kb >> 2) & 1) * SCALES);
+#pragma unroll
+            for (int i = 0; i < TM; ++i) sa[i] = sp[ar[i]];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) sb[j] = sp[br[j]];
+        }
+        const int sh = (kb & 3) * 8;
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+            const int c = 4 * hh + 2 * h;
+            auto frag = [&](int r) {
+                const i32x4 lo = *reinterpret_cast<const i32x4*>(st + r * 128 + ((c ^ ((r >> 1) & 7)) << 4));
+                const i32x4 hi = *reinterpret_cast<const i32x4*>(st + r * 128 + (((c + 1) ^ ((r >> 1) & 7)) << 4));
+                return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            };
+            if (!WIDE) {
+                i32x8 fa[TM], fb[TN];
+#pragma unroll
+                for (int j = 0; j < TN; ++j) fb[j] = frag(br[j]);
+#pragma unroll
+                for (int i = 0; i < TM; ++i) fa[i] = frag(ar[i]);
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[j], fa[i], acc[i][j], 0, 0, 0, (int)(sb[j] >> sh), 0, (int)(sa[i] >> sh));
+            } else {
+                bf16x8 wb[TN][4];
+#pragma unroll
+                for (int j = 0; j < TN; ++j) f8_widen(frag(br[j]), __uint_as_float(((sb[j] >> sh) & 255u) << 23), wb[j]);
+#pragma unroll
+                for (int i = 0; i < TM; ++i) {
+                    bf16x8 wa[4];
+                    f8_widen(frag(ar[i]), __uint_as_float(((sa[i] >> sh) & 255u) << 23), wa);
+#pragma unroll
+                    for (int s = 0; s < 4; ++s)
+#pragma unroll
+                        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wb[j][s], wa[s], acc[i][j], 0, 0, 0);
+                }
+            }
+        }
+    }
+    // acc[i][j][4 q + e] = C[m0 + .. + l31][n0 + .. + 8 q + 4 h + e]
+    const int64_t slab = (int64_t)blockIdx.y * g.slab;
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int qd = 0; qd < 4; ++qd) {
+            const int64_t n = n0 + wn * (BN / WN) + j * 32 + 8 * qd + 4 * h;
+            float b[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) b[e] = g.bias && n + e < g.N ? g.bias[n + e] : 0.f;
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                const int64_t m = m0 + wm * (BM / WM) + i * 32 + l31;
+                if (m < g.M) f8_store4(g, m, n, acc[i][j][4 * qd] + b[0], acc[i][j][4 * qd + 1] + b[1], acc[i][j][4 * qd + 2] + b[2], acc[i][j][4 * qd + 3] + b[3], slab);
+            }
+        }
+}
+
+// Few rows of a (at most 16 MT): bound by reading b once.  A workgroup takes 16 rows of b; its wavefronts take the blocks of k in turn, each
+// lane 32 bytes of a row straight into the registers that the 16 x 16 x 128 instruction reads, and the partial sums meet in LDS in a fixed order.
+template <int MT, bool WIDE>
+__global__ __launch_bounds__(1024) void fp8_rows_kernel(const F8Args g) {
+    extern __shared__ __attribute__((aligned(16))) float part[];  // [waves][MT][256]
+    const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6, lane = threadIdx.x & 63, l15 = lane & 15, h = lane >> 4;
+    const int64_t n0 = (int64_t)blockIdx.x * 16;
+    const int64_t n = n0 + l15 < g.N ? n0 + l15 : g.N - 1;
+    const uint8_t *pb = g.b + n * g.ldb + h * 32, *psb = g.bs + n * g.ldbs;
+    const uint8_t *pa[MT], *psa[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int64_t m = 16 * i + l15 < g.M ? 16 * i + l15 : g.M - 1;
+        pa[i] = g.a + m * g.lda + h * 32;
+        psa[i] = g.as + m * g.ldas;
+    }
+    f32x4 acc[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int kb = wave; kb < g.kblocks; kb += waves) {
+        const i32x8 vb = *reinterpret_cast<const i32x8*>(pb + (int64_t)kb * 128);
+        const uint32_t sb = psb[kb];
+        bf16x8 wb[4];
+        if (WIDE) f8_widen(vb, __uint_as_float(sb << 23), wb);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const i32x8 va = *reinterpret_cast<const i32x8*>(pa[i] + (int64_t)kb * 128);
+            const uint32_t sa = psa[i][kb];
+            if (!WIDE) {
+                acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vb, va, acc[i], 0, 0, 0, (int)sb, 0, (int)sa);
+            } else {
+                bf16x8 wa[4];
+                f8_widen(va, __uint_as_float(sa << 23), wa);
+#pragma unroll
+                for (int s = 0; s < 4; ++s) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[s], wa[s], acc[i], 0, 0, 0);
+            }
+        }
+    }
+    // acc[i][e] = C[16 i + l15][n0 + 4 h + e]
+#pragma unroll
+    for (int i = 0; i < MT; ++i) *reinterpret_cast<f32x4*>(&part[(wave * MT + i) * 256 + l15 * 16 + h * 4]) = acc[i];
+    __syncthreads();
+    for (int t = threadIdx.x; t < MT * 64; t += blockDim.x) {
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        for (int w = 0; w < waves; ++w) v += *reinterpret_cast<const f32x4*>(&part[w * MT * 256 + t * 4]);
+        const int64_t m = t / 4, nn = n0 + (t & 3) * 4;
+        if (m >= g.M) continue;
+        if (g.bias)
+            for (int e = 0; e < 4; ++e)
+                if (nn + e < g.N) v[e] += g.bias[nn + e];
+        f8_store4(g, m, nn, v[0], v[1], v[2], v[3], 0);
+    }
+}
+
+// out = sum of the slices' partial outputs, in order, + bias
+__global__ __launch_bounds__(256) void fp8_join_kernel(const float* __restrict__ part, int slices, const F8Args g) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, quads = (g.N + 3) / 4;
+    if (i >= g.M * quads) return;
+    const int64_t m = i / quads, n = (i % quads) * 4;
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        v[e] = 0.f;
+        if (n + e < g.N) {
+            for (int s = 0; s < slices; ++s) v[e] += part[(int64_t)s * g.slab + m * g.N + n + e];
+            if (g.bias) v[e] += g.bias[n + e];
+        }
+    }
+    f8_store4(g, m, n, v[0], v[1], v[2], v[3], 0);
+}
+
+constexpr int ROWS_MOST = 64;  // rows of a that the streaming kernel takes
+
+struct F8Plan {
+    bool rows, big;
+    int slices, kb_split;
+};
+// How a product is laid out, from its sizes alone.
+F8Plan f8_plan(int64_t M, int64_t N, int64_t K) {
+    F8Plan p = {};
+    const int kb = (int)mh_ceil_div(K, 128);
+    p.slices = 1;
+    p.kb_split = (kb + 3) / 4 * 4;
+    if (M <= ROWS_MOST) {
+        p.rows = true;
+        return p;
+    }
+    p.big = mh_ceil_div(M, 256) * mh_ceil_div(N, 256) >= 256;
+    if (!p.big) {
+        // too few tiles for the chip: slices of the summed axis, each long enough to be worth its partial output
+        const int64_t tiles = mh_ceil_div(M, 128) * mh_ceil_div(N, 128);
+        int64_t s = 512 / tiles;
+        if (s > kb / 8) s = kb / 8;
+        if (s > 1) {
+            p.kb_split = (int)mh_ceil_div(mh_ceil_div(kb, s), 4) * 4;
+            p.slices = (int)mh_ceil_div(kb, p.kb_split);
+        }
+    }
+    return p;
+}
+
+int64_t f8_part_bytes(int64_t M, int64_t N, int64_t K) {
+    const F8Plan p = f8_plan(M, N, K);
+    return p.slices > 1 ? (int64_t)p.slices * M * N * 4 : 0;
+}
+
+template <int BM, int BN, int WM, int WN>
+int32_t f8_launch_tiles(F8Args g, int slices, bool wide, hipStream_t s) {
+    g.mt = (int)mh_ceil_div(g.M, BM);
+    g.nt = (int)mh_ceil_div(g.N, BN);
+    g.per_xcd = (int)mh_ceil_div((int64_t)g.mt * g.nt, 8);
+    const dim3 grid(8 * g.per_xcd, slices), block(WM * WN * 64);
+    constexpr int lds = 2 * ((BM + BN) * 128 + (BM + BN) * 4);
+    const auto kern = wide ? fp8_gemm_kernel<BM, BN, WM, WN, true> : fp8_gemm_kernel<BM, BN, WM, WN, false>;
+    if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
+        mh_set_error("mh_fp8_matmul: %d bytes of LDS refused", lds);
+        return MH_ERR_LAUNCH;
+    }
+    MH_LAUNCH(kern, grid, block, lds, s, g);
+    return MH_OK;
+}
+
+template <bool WIDE>
+void f8_launch_rows(const F8Args& g, hipStream_t s) {
+    const int mt = (int)mh_ceil_div(g.M, 16);
+    const int waves = g.kblocks >= 32 ? 16 : g.kblocks >= 8 ? 8 : 4;
+    const dim3 grid((unsigned)mh_ceil_div(g.N, 16)), block(waves * 64);
+    if (mt == 1) MH_LAUNCH((fp8_rows_kernel<1, WIDE>), grid, block, (size_t)waves * 1024, s, g);
+    else if (mt == 2) MH_LAUNCH((fp8_rows_kernel<2, WIDE>), grid, block, (size_t)waves * 2048, s, g);
+    else MH_LAUNCH((fp8_rows_kernel<4, WIDE>), grid, block, (size_t)waves * 4096, s, g);
+}
+
+int32_t f8_check_matrix(const char* who, const char* name, const void* q, int64_t ld, const void* s, int64_t lds, int64_t rows, int64_t K) {
+    const int64_t kp = mh_ceil_div(K, 128) * 128;
+    MH_REQUIRE(rows == 0 || (q && s), "%s: %s is NULL", who, name);
+    MH_REQUIRE(ld >= kp && ld % 16 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0,
+               "%s: rows of %s must be 16-byte aligned and hold %lld entries (whole blocks of 128)", who, name, (long long)kp);
+    MH_REQUIRE(lds >= mh_ceil_div(kp / 128, 4) * 4 && lds % 4 == 0 && (reinterpret_cast<uintptr_t>(s) & 3) == 0,
+               "%s: rows of the scales of %s must be 4-byte aligned and hold a multiple of four blocks", who, name);
+    return MH_OK;
+}
+
+int32_t f8_matmul(const char* who, const uint8_t* a, int64_t lda, const uint8_t* as, int64_t ldas, const uint8_t* b, int64_t ldb, const uint8_t* bs,
+                  int64_t ldbs, int64_t M, int64_t N, int64_t K, const float* bias, int32_t kind, void* out, int64_t ldo, void* ws, int64_t ws_bytes,
+                  hipStream_t s) {
+    F8Args g = {};
+    g.a = a, g.as = as, g.b = b, g.bs = bs, g.lda = lda, g.ldas = ldas, g.ldb = ldb, g.ldbs = ldbs, g.M = M, g.N = N;
+    g.kblocks = (int)mh_ceil_div(K, 128);
+    g.bias = bias, g.kind = kind, g.out = out, g.ldo = ldo;
+    const int64_t es = kind == MH_F32 ? 4 : 2;
+    g.vec = ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) % (4 * es)) == 0;
+    const F8Plan p = f8_plan(M, N, K);
+    const bool wide = kind != MH_BF16;
+    g.kb_split = p.kb_split;
+    if (p.rows) {
+        if (wide) f8_launch_rows<true>(g, s);
+        else f8_launch_rows<false>(g, s);
+        MH_CHECK_LAUNCH(who);
+        return MH_OK;
+    }
+    F8Args t = g;
+    if (p.slices > 1) {
+        if (ws_bytes < f8_part_bytes(M, N, K) || !ws) {
+            mh_set_error("%s: workspace too small (%lld bytes)", who, (long long)ws_bytes);
+            return MH_ERR_WORKSPACE;
+        }
+        g.slab = t.slab = M * N;
+        t.out = ws, t.ldo = N, t.kind = MH_F32, t.bias = nullptr, t.vec = N % 4 == 0;
+    }
+    const int32_t rc = p.big ? f8_launch_tiles<256, 256, 2, 4>(t, p.slices, wide, s) : f8_launch_tiles<128, 128, 2, 2>(t, p.slices, wide, s);
+    if (rc) return rc;
+    MH_CHECK_LAUNCH(who);
+    if (p.slices > 1) {
+        MH_LAUNCH(fp8_join_kernel, dim3((unsigned)mh_ceil_div(M * mh_ceil_div(N, 4), 256)), dim3(256), 0, s, (const float*)ws, p.slices, g);
+        MH_CHECK_LAUNCH(who);
+    }
+    return MH_OK;
+}
+
+template <typename T>
+int32_t f8_quantize(const T* x, int64_t ldx, int64_t R, int64_t K, bool transpose, uint8_t* q, int64_t ldq, uint8_t* sc, int64_t lds, float* colsum,
+                    hipStream_t s) {
+    if (!transpose) {
+        const int64_t quads = mh_ceil_div(mh_ceil_div(K, 128), 4), blocks = mh_ceil_div(R, 4) * quads;
+        MH_REQUIRE(blocks < (int64_t)1 << 31, "mh_fp8_quantize: matrix too large");
+        MH_LAUNCH(fp8_quantize_rows_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, x, ldx, R, (int)K, (int)quads, q, ldq, sc, lds);
+    } else {
+        const int64_t rb = mh_ceil_div(R, 128), blocks = rb * mh_ceil_div(K, 64);
+        MH_REQUIRE(blocks < (int64_t)1 << 31, "mh_fp8_quantize: matrix too large");
+        MH_LAUNCH(fp8_quantize_cols_kernel<T>, dim3((unsigned)blocks), dim3(512), 0, s, x, ldx, R, K, (int)rb, (int)(mh_ceil_div(rb, 4) * 4), q, ldq, sc, lds,
+                  colsum);
+    }
+    MH_CHECK_LAUNCH("mh_fp8_quantize");
+    return MH_OK;
+}
+
+int64_t f8_q_bytes(int64_t rows, int64_t K) { return mh_ceil_div(rows * mh_ceil_div(K, 128) * 128, 256) * 256; }
+int64_t f8_s_bytes(int64_t rows, int64_t K) { return mh_ceil_div(rows * mh_ceil_div(mh_ceil_div(K, 128), 4) * 4, 256) * 256; }
+
+int32_t f8_check_out(const char* who, int64_t M, int64_t N, int64_t K, int32_t kind, const void* out, int64_t ldo) {
+    MH_REQUIRE(M >= 0 && N >= 0 && K >= 1 && K < (int64_t)1 << 31 && M < (int64_t)1 << 31 && N < (int64_t)1 << 31, "%s: sizes M=%lld N=%lld K=%lld", who,
+               (long long)M, (long long)N, (long long)K);
+    MH_REQUIRE(kind == MH_F32 || kind == MH_BF16 || kind == MH_F16, "%s: unknown output type %d", who, (int)kind);
+    MH_REQUIRE(ldo >= N && (out || M * N == 0), "%s: output rows of %lld entries cannot hold %lld", who, (long long)ldo, (long long)N);
+    MH_REQUIRE(mh_ceil_div(M, 128) * mh_ceil_div(N, 128) < (int64_t)1 << 28 && M * mh_ceil_div(N, 4) < (int64_t)1 << 38, "%s: output too large", who);
+    return MH_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t mh_fp8_quantize(const void* x, int32_t dtype, int64_t ldx, int64_t R, int64_t K, int32_t transpose, void* q, int64_t ldq, void* scales,
+                        int64_t lds, float* colsum, void* workspace, int64_t workspace_bytes, mh_stream_t stream) {
+    const int64_t rows = transpose ? K : R, len = transpose ? R : K;
+    MH_REQUIRE(R >= 0 && K >= 0 && R < (int64_t)1 << 31 && K < (int64_t)1 << 31 && ldx >= K, "mh_fp8_quantize: sizes R=%lld K=%lld ldx=%lld", (long long)R,
+               (long long)K, (long long)ldx);
+    MH_REQUIRE(dtype == MH_F32 || dtype == MH_BF16 || dtype == MH_F16, "mh_fp8_quantize: unknown type %d", (int)dtype);
+    MH_REQUIRE(!colsum || transpose, "mh_fp8_quantize: column sums come with transpose only");
+    if (rows == 0 || len == 0) return MH_OK;
+    MH_REQUIRE(x, "mh_fp8_quantize: x is NULL");
+    if (int32_t rc = f8_check_matrix("mh_fp8_quantize", "q", q, ldq, scales, lds, rows, len)) return rc;
+    const int64_t rb = mh_ceil_div(R, 128);
+    if (colsum && (!workspace || workspace_bytes < rb * K * 4)) {
+        mh_set_error("mh_fp8_quantize: workspace too small (%lld bytes)", (long long)workspace_bytes);
+        return MH_ERR_WORKSPACE;
+    }
+    hipStream_t s = mh_stream(stream);
+    uint8_t *qq = static_cast<uint8_t*>(q), *ss = static_cast<uint8_t*>(scales);
+    float* part = colsum ? static_cast<float*>(workspace) : nullptr;
+    int32_t rc;
+    if (dtype == MH_F32) rc = f8_quantize(static_cast<const float*>(x), ldx, R, K, transpose != 0, qq, ldq, ss, lds, part, s);
+    else if (dtype == MH_BF16) rc = f8_quantize(static_cast<const lp_bf16*>(x), ldx, R, K, transpose != 0, qq, ldq, ss, lds, part, s);
+    else rc = f8_quantize(static_cast<const lp_f16*>(x), ldx, R, K, transpose != 0, qq, ldq, ss, lds, part, s);
+    if (rc == MH_OK && colsum) {
+        MH_LAUNCH(fp8_colsum_kernel, dim3((unsigned)mh_ceil_div(K, 256)), dim3(256), 0, s, (const float*)part, (int)rb, K, colsum);
+        MH_CHECK_LAUNCH("mh_fp8_quantize");
+    }
+    return rc;
+}
+
+int64_t mh_fp8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K) { return M > 0 && N > 0 && K > 0 ? f8_part_bytes(M, N, K) : 0; }
+
+int32_t mh_fp8_matmul(const void* a, int64_t lda, const void* a_scales, int64_t ldas, const void* b, int64_t ldb, const void* b_scales, int64_t ldbs,
+                      int64_t M, int64_t N, int64_t K, const float* bias, int32_t out_dtype, void* out, int64_t ldo, void* workspace,
+                      int64_t workspace_bytes, mh_stream_t stream) {
+    if (int32_t rc = f8_check_out("mh_fp8_matmul", M, N, K, out_dtype, out, ldo)) return rc;
+    if (M == 0 || N == 0) return MH_OK;
+    if (int32_t rc = f8_check_matrix("mh_fp8_matmul", "a", a, lda, a_scales, ldas, M, K)) return rc;
+    if (int32_t rc = f8_check_matrix("mh_fp8_matmul", "b", b, ldb, b_scales, ldbs, N, K)) return rc;
+    return f8_matmul("mh_fp8_matmul", static_cast<const uint8_t*>(a), lda, static_cast<const uint8_t*>(a_scales), ldas, static_cast<const uint8_t*>(b), ldb,
+                     static_cast<const uint8_t*>(b_scales), ldbs, M, N, K, bias, out_dtype, out, ldo, workspace, workspace_bytes, mh_stream(stream));
+}
+
+int64_t mh_fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    return M > 0 && N > 0 && K > 0 ? f8_q_bytes(M, K) + f8_s_bytes(M, K) + f8_part_bytes(M, N, K) : 0;
+}
+
+int32_t mh_fp8_linear(const void* x, int32_t x_dtype, int64_t ldx, const void* w, int64_t ldw, const void* w_scales, int64_t ldws, int64_t M, int64_t N,
+                      int64_t K, const float* bias, int32_t out_dtype, void* out, int64_t ldo, void* workspace, int64_t workspace_bytes,
+                      mh_stream_t stream) {
+    if (int32_t rc = f8_check_out("mh_fp8_linear", M, N, K, out_dtype, out, ldo)) return rc;
+    if (M == 0 || N == 0) return MH_OK;
+    if (int32_t rc = f8_check_matrix("mh_fp8_linear", "w", w, ldw, w_scales, ldws, N, K)) return rc;
+    if (!workspace || workspace_bytes < mh_fp8_linear_workspace_bytes(M, N, K)) {
+        mh_set_error("mh_fp8_linear: workspace too small (%lld bytes)", (long long)workspace_bytes);
+        return MH_ERR_WORKSPACE;
+    }
+    uint8_t* q = static_cast<uint8_t*>(workspace);
+    uint8_t* sc = q + f8_q_bytes(M, K);
+    uint8_t* part = sc + f8_s_bytes(M, K);
+    const int64_t ldq = mh_ceil_div(K, 128) * 128, lds = mh_ceil_div(ldq / 128, 4) * 4;
+    if (int32_t rc = mh_fp8_quantize(x, x_dtype, ldx, M, K, 0, q, ldq, sc, lds, nullptr, nullptr, 0, stream)) return rc;
+    return f8_matmul("mh_fp8_linear", q, ldq, sc, lds, static_cast<const uint8_t*>(w), ldw, static_cast<const uint8_t*>(w_scales), ldws, M, N, K, bias,
+                     out_dtype, out, ldo, part, workspace_bytes - (part - q), mh_stream(stream));
+}
+
+}  // extern "C"

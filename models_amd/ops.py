@@ -22,6 +22,11 @@ __all__ = [
     "embedding_dense_list",
     "linear",
     "dot_interaction",
+    "Fp8Matrix",
+    "fp8_quantize",
+    "fp8_matmul",
+    "fp8_linear",
+    "fp8_linear_backward",
 ]
 
 
@@ -2113,3 +2118,193 @@ def route_local_rows(recv_keys: torch.Tensor, base: torch.Tensor, shard_rows: Op
         check(lib.mh_route_local_rows(_ptr(recv_keys), recv_keys.numel(), _ptr(base), _ptr(shard_rows), base.numel(),
                                       _ptr(rows), _stream()), "mh_route_local_rows")
     return rows
+
+
+# --------------------------------------------------------------------------------------------
+# products of 8-bit matrices with a scale for each block of 128
+# --------------------------------------------------------------------------------------------
+_FLOATS = {torch.float32: _lib.MH_F32, torch.bfloat16: _lib.MH_BF16, torch.float16: _lib.MH_F16}
+_FP8_BLOCK = 128
+
+
+class _NoSwitch:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NO_SWITCH = _NoSwitch()
+
+
+def _device_of(first: torch.Tensor, *others: Optional[torch.Tensor]):
+    """The context in which a call on ``first`` launches: its own device is made the current one where it is not (the stream is that device's
+    current stream), and every other tensor has to be on it."""
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"all tensors of a call must be on one device, got {first.device} and {t.device}")
+    return _NO_SWITCH if first.device.index == torch.cuda.current_device() else torch.cuda.device(first.device)
+
+
+def _float_2d(t: torch.Tensor, name: str) -> int:
+    """The type code of a 2-D fp32 / bf16 / fp16 tensor whose rows are contiguous (any distance between rows)."""
+    _dev(t, name)
+    if t.dtype not in _FLOATS:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        raise ValueError(f"{name} must be 2-D with contiguous rows that do not overlap, got shape {tuple(t.shape)}, strides {t.stride()}")
+    return _FLOATS[t.dtype]
+
+
+def _ld(t: torch.Tensor) -> int:
+    """Distance between the rows of a 2-D tensor; a single row's may be anything."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+
+def _scratch(nbytes: int, like: torch.Tensor) -> torch.Tensor:
+    """Scratch of one call, from the caching allocator on the current stream: calls on two streams, and two captured graphs, never share it."""
+    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=like.device)
+
+
+class Fp8Matrix(NamedTuple):
+    """An ``[R, cols]`` matrix in 8 bits (``fp8_quantize``): block b of 128 columns of row r stands for ``values * 2 ** (scales[r, b] - 127)``."""
+
+    values: torch.Tensor  # [R, cols rounded up to 128] float8_e4m3fn, zero past cols
+    scales: torch.Tensor  # [R, blocks rounded up to 4] uint8
+    cols: int
+
+
+def _fp8_check(m: Fp8Matrix, name: str) -> Tuple[int, int]:
+    v, s, K = m
+    _dev(v, f"{name}.values", torch.float8_e4m3fn)
+    _dev(s, f"{name}.scales", torch.uint8)
+    kp = -(-int(K) // _FP8_BLOCK) * _FP8_BLOCK
+    if K < 1 or v.dim() != 2 or s.dim() != 2 or v.shape[1] != kp or s.shape != (v.shape[0], -(-(kp // _FP8_BLOCK) // 4) * 4):
+        raise ValueError(f"{name}: values {tuple(v.shape)} and scales {tuple(s.shape)} are not the 8-bit form of a matrix of {K} columns")
+    if not (v.is_contiguous() and s.is_contiguous()):
+        raise ValueError(f"{name}: values and scales must be contiguous")
+    if s.device != v.device:
+        raise ValueError(f"{name}: values and scales must be on one device")
+    return v.shape[0], int(K)
+
+
+def fp8_quantize(x: torch.Tensor, transpose: bool = False, column_sums: bool = False):
+    """``x`` [R, K] (float32 / bfloat16 / float16) as an ``Fp8Matrix``: e4m3 values with one power-of-two scale for each row and each block
+    of 128 columns.  ``transpose=True``: the 8-bit form of ``x`` transposed (blocks of 128 along the rows of x), which is how the Keras kernel
+    ``[K, N]`` of a Dense layer becomes the ``[N, K]`` operand of ``fp8_linear``; with ``column_sums=True`` also returns the column sums of
+    x in float32 (a bias gradient, from the same read).  An infinity or NaN becomes NaN and leaves the scale to the other entries."""
+    lib = _lib.load()
+    dt = _float_2d(x, "x")
+    if column_sums and not transpose:
+        raise ValueError("column_sums comes with transpose=True")
+    R, K = x.shape
+    rows, cols = (K, R) if transpose else (R, K)
+    if cols < 1:
+        raise ValueError(f"fp8_quantize needs at least one entry along the blocks, got shape {tuple(x.shape)}")
+    kb = -(-cols // _FP8_BLOCK)
+    with _device_of(x):
+        q = torch.empty((rows, kb * _FP8_BLOCK), dtype=torch.float8_e4m3fn, device=x.device)
+        s = torch.empty((rows, -(-kb // 4) * 4), dtype=torch.uint8, device=x.device)
+        sums = torch.empty((K,), dtype=torch.float32, device=x.device) if column_sums else None
+        if rows:
+            ws = _scratch(4 * kb * K, x) if column_sums else None
+            with _timed("fp8_quantize", nbytes=R * K * (x.element_size() + 1)):
+                check(lib.mh_fp8_quantize(_ptr(x), dt, _ld(x), R, K, int(transpose), _ptr(q), q.shape[1], _ptr(s), s.shape[1], _ptr(sums),
+                                          _ptr(ws), 0 if ws is None else ws.numel(), _stream()), "mh_fp8_quantize")
+    m = Fp8Matrix(q, s, cols)
+    return (m, sums) if column_sums else m
+
+
+def _fp8_out(M: int, N: int, out: Optional[torch.Tensor], out_dtype, device) -> torch.Tensor:
+    if out_dtype not in _FLOATS:
+        raise TypeError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
+    if out is None:
+        return torch.empty((M, N), dtype=out_dtype, device=device)
+    _float_2d(out, "out")
+    if tuple(out.shape) != (M, N) or out.dtype != out_dtype:
+        raise ValueError(f"out must be [{M}, {N}] of {out_dtype}, got {tuple(out.shape)} of {out.dtype}")
+    return out
+
+
+def _fp8_bias(bias: Optional[torch.Tensor], N: int) -> Optional[torch.Tensor]:
+    if bias is not None:
+        _dev(bias, "bias", torch.float32)
+        if bias.numel() != N or not bias.is_contiguous():
+            raise ValueError(f"bias must be contiguous with {N} entries")
+    return bias
+
+
+def fp8_matmul(a: Fp8Matrix, b: Fp8Matrix, bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``a @ b.T + bias`` of two 8-bit matrices ``[M, K]`` and ``[N, K]`` -> ``[M, N]``.  A float32 or
+    float16 output is summed in 32 bits throughout; a bfloat16 one by the scaled 8-bit matrix instruction, at twice the rate: its sums are
+    off by at most 2^-10.2 of sum |a b|, where half a step of bfloat16 is 2^-8 of the result."""
+    lib = _lib.load()
+    M, K = _fp8_check(a, "a")
+    N, Kb = _fp8_check(b, "b")
+    if K != Kb:
+        raise ValueError(f"a has {K} columns and b {Kb}")
+    _fp8_bias(bias, N)
+    with _device_of(a.values, b.values, bias, out):
+        out = _fp8_out(M, N, out, out_dtype, a.values.device)
+        if M and N:
+            ws = _scratch(lib.mh_fp8_matmul_workspace_bytes(M, N, K), out)
+            with _timed("fp8_matmul", nbytes=(M + N) * K + M * N * out.element_size(), flops=2 * M * N * K):
+                check(lib.mh_fp8_matmul(_ptr(a.values), a.values.shape[1], _ptr(a.scales), a.scales.shape[1], _ptr(b.values),
+                                        b.values.shape[1], _ptr(b.scales), b.scales.shape[1], M, N, K, _ptr(bias), _FLOATS[out_dtype],
+                                        _ptr(out), _ld(out), _ptr(ws), ws.numel(), _stream()), "mh_fp8_matmul")
+    return out
+
+
+def fp8_linear(x: torch.Tensor, w: Fp8Matrix, bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A Dense layer with 8-bit operands: ``x`` [M, K] quantised by blocks of 128 and multiplied with ``w``, the layer's kernel as
+    ``fp8_quantize(kernel, transpose=True)`` (``[N, K]``), made once.  ``linear`` is the layer in 32 bits."""
+    lib = _lib.load()
+    dt = _float_2d(x, "x")
+    N, K = _fp8_check(w, "w")
+    M = x.shape[0]
+    if x.shape[1] != K:
+        raise ValueError(f"x has {x.shape[1]} columns and w {K}")
+    _fp8_bias(bias, N)
+    with _device_of(x, w.values, bias, out):
+        out = _fp8_out(M, N, out, out_dtype, x.device)
+        if M and N:
+            ws = _scratch(lib.mh_fp8_linear_workspace_bytes(M, N, K), x)
+            with _timed("fp8_linear", nbytes=M * K * x.element_size() + N * K + M * N * out.element_size(), flops=2 * M * N * K):
+                check(lib.mh_fp8_linear(_ptr(x), dt, _ld(x), _ptr(w.values), w.values.shape[1], _ptr(w.scales), w.scales.shape[1], M, N, K,
+                                        _ptr(bias), _FLOATS[out_dtype], _ptr(out), _ld(out), _ptr(ws), ws.numel(), _stream()),
+                      "mh_fp8_linear")
+    return out
+
+
+def fp8_linear_backward(x: torch.Tensor, w: Fp8Matrix, dy: torch.Tensor, need_dx: bool = True, need_dw: bool = True,
+                        need_db: bool = False):
+    """Gradients of a Dense layer ``y = x @ kernel + bias`` with 8-bit operands, in float32: ``(dx [M, K], dW [K, N])``, and ``db [N]`` third
+    with ``need_db=True`` (None for what is not asked for).  ``w`` is ``fp8_quantize(kernel)`` -- the kernel ``[K, N]`` with its blocks
+    along N, the axis that dx sums over; dy is quantised along N for dx, and x and dy along the batch for dW."""
+    _float_2d(x, "x")
+    _float_2d(dy, "dy")
+    M, K = x.shape
+    N = dy.shape[1]
+    if dy.shape[0] != M:
+        raise ValueError(f"x has {M} rows and dy {dy.shape[0]}")
+    dx = dw = db = None
+    if need_dx:
+        rows, cols = _fp8_check(w, "w")
+        if (rows, cols) != (K, N):
+            raise ValueError(f"w must be the 8-bit form of the [{K}, {N}] kernel, got [{rows}, {cols}]")
+    with _device_of(x, dy, w.values if need_dx else None):
+        if need_dx:
+            dx = fp8_matmul(fp8_quantize(dy), w)
+        if M == 0:
+            dw = torch.zeros((K, N), dtype=torch.float32, device=x.device) if need_dw else None
+            db = torch.zeros((N,), dtype=torch.float32, device=x.device) if need_db else None
+        elif need_dw or need_db:
+            dyt = fp8_quantize(dy, transpose=True, column_sums=need_db)
+            if need_db:
+                dyt, db = dyt
+            if need_dw:
+                dw = fp8_matmul(fp8_quantize(x, transpose=True), dyt)
+    return (dx, dw, db) if need_db else (dx, dw)
