@@ -724,6 +724,37 @@ int32_t mh_fp8_linear(const void* x, int32_t x_dtype, int64_t ldx, const void* w
                       int64_t M, int64_t N, int64_t K, const float* bias, int32_t out_dtype, void* out, int64_t ldo, void* workspace,
                       int64_t workspace_bytes, mh_stream_t stream);
 
+/* ---- softmax over a catalogue's logits: log probabilities, entropy, alternatives; distillation ------------------------------------
+ * logits [N, V] of type code dtype, leading dimension ld >= V, contiguous rows at any element's address; temperature in [1e-4, 1e4], z = logits /
+ * temperature; V < 2^31 - 65536.  A logit of -inf is masked (p = 0).  A row with nothing left has log p = -inf, entropy 0, lse -inf and a
+ * gradient of zero.  A NaN or +inf among a row's logits makes its values NaN.  Sums in 32 bits; no atomics on results: they do not change from
+ * call to call.
+ * mh_token_logprobs: logp[n] = log softmax(z[n])[ids[n]] (0 where ids[n] is outside [0, V): padding; ids and logp may be NULL), entropy[n],
+ * lse[n] = log sum exp z[n], and the k (<= 256, <= V) largest entries of each row, ties to the lowest index: top_ids [N, k] and their log
+ * probabilities top_logp [N, k]; places past the row's unmasked entries hold -1 and -inf, NaN is never an alternative.  stats [N, 2]: for _bwd.
+ * mh_token_logprobs_bwd: dlogits [N, V] (leading dimension ldd, type of logits, all V columns written; may be logits itself) =
+ * dlogp (onehot - p) - dentropy p (log p + entropy) + dlse p, over temperature.  dlogp / dentropy / dlse [N] or NULL (zero). */
+int64_t mh_token_logprobs_workspace_bytes(int64_t N, int64_t V, int32_t k);
+int32_t mh_token_logprobs(const void* logits, int32_t dtype, int64_t ld, int64_t N, int64_t V, const void* ids, int32_t ids_dtype, int32_t k,
+                          float temperature, float* logp, float* entropy, float* lse, float* top_logp, int32_t* top_ids, float* stats,
+                          void* workspace, int64_t workspace_bytes, mh_stream_t stream);
+int32_t mh_token_logprobs_bwd(const void* logits, int32_t dtype, int64_t ld, int64_t N, int64_t V, const void* ids, int32_t ids_dtype,
+                              float temperature, const float* stats, const float* entropy, const float* dlogp, const float* dentropy,
+                              const float* dlse, void* dlogits, int64_t ldd, mh_stream_t stream);
+/* CategoricalCrossEntropy against a teacher's few entries (tf/losses/listwise.py:38-52 with soft targets), as a Kullback-Leibler divergence.
+ * teacher_ids / teacher_logp [N, K], K <= 256: ids outside [0, V) are left out; an id given twice counts with both masses.  tail == 0: q =
+ * softmax of the row's entries of teacher_logp (any constant may be added to a row); tail != 0: q = exp(teacher_logp), and what is left of 1
+ * is held against the student's probability outside the entries.  loss[n] = sum q (log q - log p) (+ r (log r - log p_rest)); a row without
+ * entries has loss 0 and no gradient; one whose student row is masked throughout has loss +inf and no gradient.  stats [N, 3] and top_grad
+ * [N, K] (both or neither NULL) are for _bwd: dlogits = dloss[n] (1 where dloss is NULL) * d loss / d logits, may be logits itself. */
+int64_t mh_distill_topk_workspace_bytes(int64_t N, int64_t V, int32_t tail);
+int32_t mh_distill_topk(const void* logits, int32_t dtype, int64_t ld, int64_t N, int64_t V, const void* teacher_ids, int32_t ids_dtype,
+                        const float* teacher_logp, int32_t K, float temperature, int32_t tail, float* loss, float* stats, float* top_grad,
+                        void* workspace, int64_t workspace_bytes, mh_stream_t stream);
+int32_t mh_distill_topk_bwd(const void* logits, int32_t dtype, int64_t ld, int64_t N, int64_t V, const void* teacher_ids, int32_t ids_dtype,
+                            int32_t K, float temperature, const float* stats, const float* top_grad, const float* dloss, void* dlogits,
+                            int64_t ldd, mh_stream_t stream);
+
 /* ---- launch recorder: a train step traced once, replayed without re-entering the host language ----------------------------
  * Replaces the role of Keras' traced `train_function` (BaseModel.fit -> make_train_function, models/base.py:1361-1421): between
  * mh_record_begin and mh_record_end every kernel launch of this library is executed AND kept (kernel, geometry, stream, arguments by

@@ -119,6 +119,12 @@ SIGNATURES = {
     "mh_fp8_matmul": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _i32, _p, _i64, _p, _i64, _p]),
     "mh_fp8_linear_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "mh_fp8_linear": (_i32, [_p, _i32, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _i32, _p, _i64, _p, _i64, _p]),
+    "mh_token_logprobs_workspace_bytes": (_i64, [_i64, _i64, _i32]),
+    "mh_token_logprobs": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _i32, _i32, _f32, _p, _p, _p, _p, _p, _p, _p, _i64, _p]),
+    "mh_token_logprobs_bwd": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _i32, _f32, _p, _p, _p, _p, _p, _p, _i64, _p]),
+    "mh_distill_topk_workspace_bytes": (_i64, [_i64, _i64, _i32]),
+    "mh_distill_topk": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _i32, _p, _i32, _f32, _i32, _p, _p, _p, _p, _i64, _p]),
+    "mh_distill_topk_bwd": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _i32, _i32, _f32, _p, _p, _p, _p, _i64, _p]),
     "mh_record_begin": (_i32, []),
     "mh_record_end": (_i32, [C.POINTER(_p)]),
     "mh_record_abort": (_i32, []),

@@ -1,0 +1,883 @@
+// Softmax statistics of [N, V] logits and what is read off them, one pass over the logits:
+//   token_logprobs  log probability of a given id, entropy, log-sum-exp and the top alternatives of each row, and the gradient of the first three
+//   distill_topk    Kullback-Leibler divergence from a teacher's top entries (CategoricalCrossEntropy over soft targets,
+//                   tf/losses/listwise.py:38-52, where the targets are few of V), and its gradient
+//
+// With z = l / T, m = max l, c = log2(e) / T:  s = sum 2^((l - m) c),  log p = (l - m) / T - ln s,  H = ln2 (log2 s - u / s) with
+// u = sum 2^t t, t = (l - m) c.  A thread keeps a running maximum and rescales its sums when it rises; sums are fp32.  All kernels are
+// bound by reading the logits (and writing the gradient): 16-byte loads at whatever address a row starts, several in flight a thread.
+//
+// Masked entries (-inf) have p = 0.  A row with nothing left has log p = -inf, entropy 0 and no gradient.  NaN or +inf makes a row's values NaN.
+#include "mh_lowp.h"
+
+namespace {
+
+constexpr float LN2 = 0.693147180559945309f;
+// The pass works with l c up to a magnitude of 2^28 (see Run).  A thread's running maximum starts at -2^28 / c: entries below count as 0, and a row
+// whose entries all lie there (masks of the type's lowest value) comes out with a sum of zero; one with an entry beyond 2^29 / c is marked.  Both
+// are summed again against their true maximum.
+constexpr float FAR = 0x1p28f;
+constexpr float INF = __builtin_inff();
+constexpr int TOP_MOST = 256;        // most alternatives, and teacher entries, of a row
+constexpr int CAND = 2048;           // candidates of a row (or part of one) that LDS holds
+constexpr int JOIN_MOST = 16 * 512;  // candidates of all parts of a row that the joining kernel holds in registers
+constexpr int TAIL_CHUNK = 1 << 18;  // columns of a part whose membership bits lie in LDS (32 KB)
+
+struct Sum {
+    float m, s, u;  // maximum, sum 2^t, sum 2^t t with t = (l - m) c
+};
+
+__device__ __forceinline__ float ex2(float t) { return __builtin_amdgcn_exp2f(t); }
+
+// a's sums relative to the larger maximum m (>= a.m); the clamp keeps 0 * (d s) from being 0 * inf and loses nothing: 2^-200 is 0
+__device__ __forceinline__ void sum_to(Sum& a, float m, float c) {
+    const float d = fmaxf((a.m - m) * c, -200.f), f = ex2(d);
+    a.u = f * fmaf(d, a.s, a.u);
+    a.s *= f;
+    a.m = m;
+}
+__device__ __forceinline__ Sum sum_join(Sum a, Sum b, float c) {
+    const float m = fmaxf(a.m, b.m);
+    sum_to(a, m, c);
+    sum_to(b, m, c);
+    return Sum{m, a.s + b.s, a.u + b.u};
+}
+template <int NT>
+__device__ __forceinline__ Sum sum_block(Sum a, float c, Sum* red) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) a = sum_join(a, Sum{__shfl_xor(a.m, o), __shfl_xor(a.s, o), __shfl_xor(a.u, o)}, c);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
+    __syncthreads();
+    a = red[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) a = sum_join(a, red[w], c);
+    return a;
+}
+template <int NT>
+__device__ __forceinline__ float max_block(float v, float* red) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = red[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) v = fmaxf(v, red[w]);
+    return v;
+}
+template <int NT>
+__device__ __forceinline__ double add_block(double v, double* red) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = red[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) v += red[w];
+    return v;
+}
+template <int NT>
+__device__ __forceinline__ int count_block(int mine, int* red, int& phase) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) mine += __shfl_xor(mine, o);
+    int* r = red + (phase ^= 1) * (NT / 64);  // two sets in turn: one barrier a count
+    if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = mine;
+    __syncthreads();
+    int n = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) n += r[w];
+    return n;
+}
+
+// The sums of a thread while it reads: t = l c - B in one fused operation, B the rounded product m c.  What B lacks of m c -- 16 at most below 2^29 --
+// is put right once, at the end, exactly: fma(m, c, -B) is what the rounding took.
+struct Run {
+    float m, B, s = 0.f, u = 0.f;
+    __device__ __forceinline__ explicit Run(float c) : m(-FAR / c), B(m * c) {}
+    template <bool ENT, int N>
+    __device__ __forceinline__ void take(const float (&v)[N], float most, float c) {
+        if (most > m) {
+            const float nb = most * c, d = fmaxf(B - nb, -200.f), f = ex2(d);
+            if (ENT) u = f * fmaf(d, s, u);
+            s *= f;
+            m = most;
+            B = nb;
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float t = fmaf(v[i], c, -B), e = ex2(t);
+            s += e;
+            if (ENT) u = fmaf(e, fmaxf(t, -200.f), u);  // 0 * -inf is 0 here; a NaN stays one through e
+        }
+    }
+    __device__ __forceinline__ Sum sum(float c) const {
+        const float d = fmaf(m, c, -B), f = ex2(-d);
+        return Sum{m, s * f, f * fmaf(-d, s, u)};
+    }
+};
+
+template <int N>
+__device__ __forceinline__ float most_of(const float (&v)[N]) {
+    float a = v[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) a = fmaxf(a, v[i]);
+    return a;
+}
+
+// f(values, index of the first) over the n entries at x, in vectors and, at the end, single entries (the others of that call -inf)
+template <int NT, typename T, typename F>
+__device__ __forceinline__ void each_entry(const T* x, int n, F f) {
+    constexpr int VE = lp_vec<T>::N;
+    const int nv = n / VE;
+    for (int v = threadIdx.x; v < nv; v += NT) {
+        float a[VE];
+        lp_unpack(lp_load16(x + (int64_t)v * VE), a, x);
+        f(a, v * VE);
+    }
+    if (threadIdx.x < n - nv * VE) {
+        float a[VE];
+#pragma unroll
+        for (int i = 1; i < VE; ++i) a[i] = -INF;
+        a[0] = lp_float(x[nv * VE + threadIdx.x]);
+        f(a, nv * VE + threadIdx.x);
+    }
+}
+
+// The sums over the n entries at x.  `most` receives the thread's own largest entry (NaN left out).  SKIP: entries whose bit is set in `skip` do
+// not count.
+template <int NT, bool ENT, bool SKIP, typename T>
+__device__ __forceinline__ Sum read_sums(const T* x, int n, float c, const uint32_t* skip, float& most, Sum* red) {
+    constexpr int VE = lp_vec<T>::N, U = 4;
+    Run r(c);
+    most = -INF;
+    const int nv = n / VE;
+    auto masked = [&](float (&a)[VE], int v) {
+        const uint32_t w = VE == 8 ? (skip[v >> 2] >> (8 * (v & 3))) & 255u : (skip[v >> 3] >> (4 * (v & 7))) & 15u;
+        if (w) {
+#pragma unroll
+            for (int i = 0; i < VE; ++i)
+                if (w >> i & 1) a[i] = -INF;
+        }
+    };
+    int v = threadIdx.x;
+    for (; v + (U - 1) * NT < nv; v += U * NT) {
+        uint4 w[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) w[j] = lp_load16(x + (int64_t)(v + j * NT) * VE);
+        float a[U * VE];
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            float b[VE];
+            lp_unpack(w[j], b, x);
+            if (SKIP) masked(b, v + j * NT);
+#pragma unroll
+            for (int i = 0; i < VE; ++i) a[j * VE + i] = b[i];
+        }
+        const float b = most_of(a);
+        most = fmaxf(most, b);
+        r.template take<ENT>(a, b, c);
+    }
+    for (; v < nv; v += NT) {
+        float a[VE];
+        lp_unpack(lp_load16(x + (int64_t)v * VE), a, x);
+        if (SKIP) masked(a, v);
+        const float b = most_of(a);
+        most = fmaxf(most, b);
+        r.template take<ENT>(a, b, c);
+    }
+    if (threadIdx.x < n - nv * VE) {
+        const int i = nv * VE + threadIdx.x;
+        float a[1] = {lp_float(x[i])};
+        if (SKIP && (skip[i >> 5] >> (i & 31) & 1)) a[0] = -INF;
+        most = fmaxf(most, a[0]);
+        r.template take<ENT>(a, a[0], c);
+    }
+    const bool beyond = __syncthreads_or(!(r.B < 2.f * FAR));
+    Sum t = sum_block<NT>(r.sum(c), c, red);
+    if (t.s == 0.f || beyond) {
+        t = Sum{max_block<NT>(most, reinterpret_cast<float*>(red)), 0.f, 0.f};
+        if (t.m == -INF) return t;
+        Sum a = {t.m, 0.f, 0.f};
+        each_entry<NT>(x, n, [&](const float(&l)[VE], int at) {
+#pragma unroll
+            for (int i = 0; i < VE; ++i) {
+                if (SKIP && at + i < n && (skip[(at + i) >> 5] >> ((at + i) & 31) & 1)) continue;
+                const float d = (l[i] - t.m) * c, e = ex2(d);
+                a.s += e;
+                a.u = fmaf(e, fmaxf(d, -200.f), a.u);
+            }
+        });
+        t = sum_block<NT>(a, c, red);
+    }
+    return t;
+}
+
+// ---- top alternatives ------------------------------------------------------------------------------------------------------------------
+// An entry's key orders by value, then by place, the lowest first; places of -inf and NaN have none.
+__device__ __forceinline__ uint32_t key_of(float v) {
+    const uint32_t b = __float_as_uint(v);
+    return (b >> 31) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k); }
+constexpr uint32_t KEY_NONE = 0x007fffffu;  // the key of -inf
+__device__ __forceinline__ uint64_t key_at(float v, int at) {
+    return (v > -INF) ? (uint64_t)key_of(v + 0.f) << 32 | (uint32_t)~at : 0;  // + 0: -0 and 0 are one value
+}
+
+// The largest threshold found, from the high bits on, that at least k keys reach; ends as soon as no more than `most` do.
+template <typename C>
+__device__ __forceinline__ uint64_t key_threshold(int k, int most, C count) {
+    uint64_t t = 0;
+    for (int b = 63; b >= 0; --b) {
+        const uint64_t next = t | (uint64_t)1 << b;
+        const int n = count(next);
+        if (n >= k) {
+            t = next;
+            if (n <= most) break;
+        }
+    }
+    return t;
+}
+
+template <int NT>
+struct TopLds {
+    uint64_t cand[CAND];
+    int n, nq, red[2 * (NT / 64)];
+    uint16_t list[NT];
+};
+
+// The k largest keys of the n entries at x, in order, to emit(place, key).  `most` is the thread's own largest entry: the k-th largest of those
+// bounds the row's k-th largest from below, so only the entries of about k threads are read again -- k / NT of the row.
+template <int NT, typename T, typename E>
+__device__ __forceinline__ void top_entries(const T* x, int n, int first, int k, float most, TopLds<NT>& s, E emit) {
+    constexpr int VE = lp_vec<T>::N;
+    const int nv = n / VE, sweeps = (nv + NT - 1) / NT;
+    int phase = 0;
+    const uint32_t mine = key_of(most + 0.f);
+    uint32_t low = 0;
+    for (int b = 31; b >= 16; --b) {
+        const uint32_t next = low | 1u << b;
+        if (count_block<NT>(mine >= next ? 1 : 0, s.red, phase) >= k) low = next;
+    }
+    if (low <= KEY_NONE) low = KEY_NONE + 1;
+    if (threadIdx.x == 0) s.n = s.nq = 0;
+    __syncthreads();
+    if (mine >= low) s.list[atomicAdd(&s.nq, 1)] = (uint16_t)threadIdx.x;
+    __syncthreads();
+    const int nq = s.nq;
+    auto put = [&](uint64_t key) {
+        const int at = atomicAdd(&s.n, 1);
+        if (at < CAND) s.cand[at] = key;
+    };
+    for (int p = threadIdx.x; p < nq * sweeps; p += NT) {
+        const int v = s.list[p % nq] + p / nq * NT;
+        if (v < nv) {
+            float a[VE];
+            lp_unpack(lp_load16(x + (int64_t)v * VE), a, x);
+#pragma unroll
+            for (int i = 0; i < VE; ++i)
+                if (a[i] > -INF && key_of(a[i] + 0.f) >= low) put(key_at(a[i], first + v * VE + i));
+        }
+    }
+    if (threadIdx.x < n - nv * VE) {
+        const float a = lp_float(x[nv * VE + threadIdx.x]);
+        if (a > -INF && key_of(a + 0.f) >= low) put(key_at(a, first + nv * VE + threadIdx.x));
+    }
+    __syncthreads();
+    int have = s.n;
+    if (have > CAND) {  // ties, or large entries that fell to the same few threads: look for the threshold in the row itself
+        const uint64_t t = key_threshold(k, CAND, [&](uint64_t next) {
+            int c = 0;
+            each_entry<NT>(x, n, [&](const float(&l)[VE], int at) {
+#pragma unroll
+                for (int i = 0; i < VE; ++i) c += key_at(l[i], first + at + i) >= next ? 1 : 0;
+            });
+            return count_block<NT>(c, s.red, phase);
+        });
+        if (threadIdx.x == 0) s.n = 0;
+        __syncthreads();
+        each_entry<NT>(x, n, [&](const float(&l)[VE], int at) {
+#pragma unroll
+            for (int i = 0; i < VE; ++i) {
+                const uint64_t key = key_at(l[i], first + at + i);
+                if (key && key >= t) put(key);
+            }
+        });
+        __syncthreads();
+        have = s.n;
+    }
+    if (have > NT) {
+        const uint64_t t = key_threshold(k, NT, [&](uint64_t next) {
+            int c = 0;
+            for (int i = threadIdx.x; i < have; i += NT) c += s.cand[i] >= next ? 1 : 0;
+            return count_block<NT>(c, s.red, phase);
+        });
+        uint64_t keep[CAND / NT];
+#pragma unroll
+        for (int j = 0; j < CAND / NT; ++j) {
+            const int i = threadIdx.x + j * NT;
+            keep[j] = i < have ? s.cand[i] : 0;
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) s.n = 0;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < CAND / NT; ++j)
+            if (keep[j] && keep[j] >= t) s.cand[atomicAdd(&s.n, 1)] = keep[j];
+        __syncthreads();
+        have = s.n;
+    }
+    if (threadIdx.x < have) {
+        const uint64_t key = s.cand[threadIdx.x];
+        int place = 0;
+        for (int i = 0; i < have; ++i) place += s.cand[i] > key ? 1 : 0;
+        if (place < k) emit(place, key);
+    }
+    for (int i = have + threadIdx.x; i < k; i += NT) emit(i, (uint64_t)0);
+}
+
+// ---- token log probabilities --------------------------------------------------------------------------------------------------------------
+struct LpArgs {
+    const void* x;
+    int64_t ld, N;
+    int V, k, parts, chunk;
+    const void* ids;
+    int ids_dtype;
+    float inv_t, c;
+    float *logp, *entropy, *lse, *top_logp;
+    int32_t* top_ids;
+    float* stats;   // [N, 2]: maximum, log2 of the sum
+    float4* part;   // [N, parts] sums
+    uint64_t* tops;  // [N, parts, k] keys
+};
+
+__device__ __forceinline__ int64_t id_at(const void* ids, int dtype, int64_t i) {
+    return dtype == MH_I32 ? (int64_t)static_cast<const int32_t*>(ids)[i] : static_cast<const int64_t*>(ids)[i];
+}
+
+__device__ __forceinline__ float lp_value(float l, const Sum& t, float inv_t) {
+    return t.m == -INF ? -INF : fmaf(l - t.m, inv_t, -logf(t.s));
+}
+
+template <typename T>
+__device__ __forceinline__ void lp_finish(const LpArgs& g, int64_t row, const Sum& t) {
+    const float ls = log2f(t.s);
+    const bool none = t.m == -INF;
+    if (g.ids) {
+        const int64_t id = id_at(g.ids, g.ids_dtype, row);
+        g.logp[row] = id >= 0 && id < g.V ? lp_value(lp_float(static_cast<const T*>(g.x)[row * g.ld + id]), t, g.inv_t) : 0.f;
+    }
+    g.entropy[row] = none ? 0.f : LN2 * (ls - t.u / t.s);
+    g.lse[row] = none ? -INF : fmaf(t.m, g.inv_t, logf(t.s));
+    g.stats[2 * row] = t.m;
+    g.stats[2 * row + 1] = none ? 0.f : ls;
+}
+
+__device__ __forceinline__ void lp_emit(const LpArgs& g, int64_t row, const Sum& t, int place, uint64_t key) {
+    g.top_ids[row * g.k + place] = key ? (int32_t)~(uint32_t)key : -1;
+    g.top_logp[row * g.k + place] = key ? lp_value(key_value((uint32_t)(key >> 32)), t, g.inv_t) : -INF;
+}
+
+template <int NT, typename T, bool TOP>
+__global__ __launch_bounds__(NT) void token_logprobs_kernel(const LpArgs g) {
+    __shared__ Sum red[NT / 64];
+    __shared__ TopLds<TOP ? NT : 64> lds;
+    const int64_t row = blockIdx.x / (uint32_t)g.parts;
+    const int part = (int)(blockIdx.x % (uint32_t)g.parts), c0 = part * g.chunk, n = g.V - c0 < g.chunk ? g.V - c0 : g.chunk;
+    const T* x = static_cast<const T*>(g.x) + row * g.ld + c0;
+    float most;
+    const Sum t = read_sums<NT, true, false>(x, n, g.c, nullptr, most, red);
+    if (threadIdx.x == 0) {
+        if (g.parts == 1) lp_finish<T>(g, row, t);
+        else g.part[row * g.parts + part] = make_float4(t.m, t.s, t.u, 0.f);
+    }
+    if constexpr (TOP) {
+        top_entries<NT>(x, n, c0, g.k, most, lds, [&](int place, uint64_t key) {
+            if (g.parts == 1) lp_emit(g, row, t, place, key);
+            else g.tops[(row * g.parts + part) * g.k + place] = key;
+        });
+    }
+}
+
+// The sums of a row's parts put together.
+template <int NT>
+__device__ __forceinline__ Sum join_parts(const float4* part, int parts, float c, Sum* red) {
+    Sum a = {-3.402823466e38f, 0.f, 0.f};
+    for (int i = threadIdx.x; i < parts; i += NT) {
+        const float4 v = part[i];
+        if (v.x != -INF) a = sum_join(a, Sum{v.x, v.y, v.z}, c);
+    }
+    a = sum_block<NT>(a, c, red);
+    if (a.s == 0.f) a.m = -INF;
+    return a;
+}
+
+template <typename T>
+__global__ __launch_bounds__(512) void token_logprobs_join_kernel(const LpArgs g) {
+    __shared__ uint64_t cand[512];
+    __shared__ Sum sums[8];
+    __shared__ int red[16], have;
+    const int64_t row = blockIdx.x;
+    const Sum t = join_parts<512>(g.part + row * g.parts, g.parts, g.c, sums);
+    if (threadIdx.x == 0) lp_finish<T>(g, row, t);
+    if (!g.k) return;
+    const int n = g.parts * g.k;
+    const uint64_t* in = g.tops + row * n;
+    uint64_t key[JOIN_MOST / 512];
+#pragma unroll
+    for (int j = 0; j < JOIN_MOST / 512; ++j) key[j] = (int)threadIdx.x + 512 * j < n ? in[threadIdx.x + 512 * j] : 0;
+    int phase = 0;
+    uint64_t th = 1;
+    if (n > 512)
+        th = key_threshold(g.k, 512, [&](uint64_t next) {
+            int c = 0;
+#pragma unroll
+            for (int j = 0; j < JOIN_MOST / 512; ++j) c += key[j] >= next ? 1 : 0;
+            return count_block<512>(c, red, phase);
+        });
+    if (th == 0) th = 1;  // fewer than k keys in all
+    if (threadIdx.x == 0) have = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < JOIN_MOST / 512; ++j)
+        if (key[j] >= th) cand[atomicAdd(&have, 1)] = key[j];
+    __syncthreads();
+    if (threadIdx.x < have) {
+        const uint64_t mine = cand[threadIdx.x];
+        int place = 0;
+        for (int i = 0; i < have; ++i) place += cand[i] > mine ? 1 : 0;
+        if (place < g.k) lp_emit(g, row, t, place, mine);
+    }
+    for (int i = have + threadIdx.x; i < g.k; i += 512) lp_emit(g, row, t, i, (uint64_t)0);
+}
+
+// ---- gradients -------------------------------------------------------------------------------------------------------------------------------
+// d[v] = p (A + B log2 p) with p = 2^((l - m) c - L), then the places that differ: the given id (g added) or the teacher's entries.
+struct GradArgs {
+    const void* x;
+    int64_t ld, N, ldd;
+    int V, K, parts, chunk;
+    const void* ids;
+    int ids_dtype;
+    float inv_t, c;
+    const float *stats, *entropy, *dlogp, *dentropy, *dlse;  // token_logprobs: stats [N, 2]
+    const float *top_grad, *dloss;                           // distill_topk: stats [N, 3] (maximum, log2 sum, weight)
+    void* d;
+};
+
+template <typename T, int N>
+__device__ __forceinline__ void grad_values(const float (&l)[N], float (&o)[N], float m, float c, float L, float A, float B, bool ent) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float t = fmaf(l[i] - m, c, -L), e = ex2(t);
+        o[i] = ent ? e * fmaf(B, fmaxf(t, -200.f), A) : e * A;
+    }
+}
+
+template <int NT, typename T, bool ENT>
+__device__ __forceinline__ void grad_row(const T* x, T* d, int n, float m, float c, float L, float A, float B) {
+    constexpr int VE = lp_vec<T>::N, U = 4;
+    const int nv = n / VE;
+    int v = threadIdx.x;
+    for (; v + (U - 1) * NT < nv; v += U * NT) {
+        uint4 w[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) w[j] = lp_load16(x + (int64_t)(v + j * NT) * VE);
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            float l[VE], o[VE];
+            lp_unpack(w[j], l, x);
+            grad_values<T>(l, o, m, c, L, A, B, ENT);
+            lp_store16(d + (int64_t)(v + j * NT) * VE, o);
+        }
+    }
+    for (; v < nv; v += NT) {
+        float l[VE], o[VE];
+        lp_unpack(lp_load16(x + (int64_t)v * VE), l, x);
+        grad_values<T>(l, o, m, c, L, A, B, ENT);
+        lp_store16(d + (int64_t)v * VE, o);
+    }
+    if (threadIdx.x < n - nv * VE) {
+        const int i = nv * VE + threadIdx.x;
+        float l[1] = {lp_float(x[i])}, o[1];
+        grad_values<T>(l, o, m, c, L, A, B, ENT);
+        lp_store(d + i, o[0]);
+    }
+}
+template <int NT, typename T>
+__device__ __forceinline__ void zero_row(T* d, int n) {
+    constexpr int VE = lp_vec<T>::N;
+    float z[VE];
+#pragma unroll
+    for (int i = 0; i < VE; ++i) z[i] = 0.f;
+    const int nv = n / VE;
+    for (int v = threadIdx.x; v < nv; v += NT) lp_store16(d + (int64_t)v * VE, z);
+    if (threadIdx.x < n - nv * VE) lp_store(d + nv * VE + threadIdx.x, 0.f);
+}
+
+template <int NT, typename T>
+__global__ __launch_bounds__(NT) void token_logprobs_bwd_kernel(const GradArgs g) {
+    const int64_t row = blockIdx.x / (uint32_t)g.parts;
+    const int c0 = (int)(blockIdx.x % (uint32_t)g.parts) * g.chunk, n = g.V - c0 < g.chunk ? g.V - c0 : g.chunk;
+    const T* x = static_cast<const T*>(g.x) + row * g.ld + c0;
+    T* d = static_cast<T*>(g.d) + row * g.ldd + c0;
+    const int64_t id = g.ids ? id_at(g.ids, g.ids_dtype, row) : -1;
+    const float gr = g.dlogp && id >= 0 && id < g.V ? g.dlogp[row] : 0.f, h = g.dentropy ? g.dentropy[row] : 0.f, z = g.dlse ? g.dlse[row] : 0.f;
+    const float m = g.stats[2 * row], L = g.stats[2 * row + 1];
+    if (m == -INF || (gr == 0.f && h == 0.f && z == 0.f)) {
+        zero_row<NT>(d, n);
+        return;
+    }
+    const float A = (z - gr - h * g.entropy[row]) * g.inv_t, B = -h * LN2 * g.inv_t;
+    const bool here = gr != 0.f && id >= c0 && id < c0 + n;
+    const float lt = here && threadIdx.x == 0 ? lp_float(x[id - c0]) : 0.f;  // before d, which may be x, is written
+    __syncthreads();
+    if (h != 0.f) grad_row<NT, T, true>(x, d, n, m, g.c, L, A, B);
+    else grad_row<NT, T, false>(x, d, n, m, g.c, L, A, 0.f);
+    if (here) {
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            float l[1] = {lt}, o[1];
+            grad_values<T>(l, o, m, g.c, L, A, B, h != 0.f);
+            lp_store(d + (id - c0), fmaf(gr, g.inv_t, o[0]));
+        }
+    }
+}
+
+// ---- distillation ------------------------------------------------------------------------------------------------------------------------------
+// q_k: the teacher's mass on its entries -- softmax of the K log probabilities (tail = 0), or their exponentials, with r = 1 - sum q for the rest of
+// the catalogue (tail = 1).  loss = sum q_k (ln q_k - ln p_k) + r (ln r - ln p_rest);  d loss / d z = c p - sum of its q at an entry, c = sum q + r,
+// and (c p_rest - r) p / p_rest elsewhere.  With a tail the pass leaves the entries out, by a bit for each column in LDS, so p_rest is a sum of its
+// own and not what is left of 1.  The K entries themselves are done in fp64: few, and 1 - sum q cancels.
+struct DsArgs {
+    const void* x;
+    int64_t ld, N;
+    int V, K, parts, chunk, tail;
+    const void* ids;
+    int ids_dtype;
+    const float* tlp;
+    float inv_t, c;
+    float *loss, *stats, *top_grad;
+    float4* part;
+};
+
+template <int NT>
+struct DsLds {
+    double red[NT / 64], q[TOP_MOST];
+    float fred[NT / 64];
+    int id[TOP_MOST];
+};
+
+// t: the sums over the row (tail: over the row without the teacher's entries).  Returns the row's weight, with t what it belongs to.
+template <int NT, typename T>
+__device__ __forceinline__ float ds_finish(const DsArgs& g, int64_t row, Sum& t, DsLds<NT>& s, float* my_grad) {
+    static_assert(NT >= TOP_MOST, "a thread for each entry");
+    const int j = threadIdx.x;
+    int id = -1;
+    float l = -INF, tl = -INF;
+    if (j < g.K) {
+        const int64_t v = id_at(g.ids, g.ids_dtype, row * g.K + j);
+        if (v >= 0 && v < g.V) {
+            id = (int)v;
+            tl = g.tlp[row * g.K + j];
+            l = lp_float(static_cast<const T*>(g.x)[row * g.ld + id]);
+        }
+        s.id[j] = id;
+    }
+    const bool ok = id >= 0;
+    const float tm = max_block<NT>(tl, s.fred);  // its barriers publish s.id
+    bool first = ok;
+    for (int i = 0; i < j && first; ++i)
+        if (i < g.K && s.id[i] == id) first = false;
+    float m = t.m;
+    double sum = t.s;
+    if (g.tail) {
+        m = fmaxf(m, max_block<NT>(l, s.fred));
+        const double e = first && l > -INF ? exp((double)(l - m) * g.inv_t) : first && l != l ? (double)l : 0.0;
+        sum = add_block<NT>(e, s.red) + (t.m == -INF ? 0.0 : (double)t.s * exp((double)(t.m - m) * g.inv_t));
+    }
+    const bool any = __syncthreads_or(ok && (g.tail || !(tl == -INF)));  // the row has a teacher; NaN counts: it has to show
+    const double ln_s = log(sum);
+    double q, lq, r = 0.0;
+    if (g.tail) {
+        lq = tl;
+        q = ok ? exp(lq) : 0.0;
+    } else {
+        lq = any ? (double)tl - tm : 0.0;
+        q = ok && any ? exp(lq) : 0.0;
+    }
+    double Q = add_block<NT>(q, s.red);
+    if (!g.tail) {
+        if (any) {
+            q /= Q;
+            lq -= log(Q);
+            Q = 1.0;
+        }
+    } else if (any && t.m > -INF && t.s != 0.f) {
+        r = 1.0 - Q;
+        if (r < 0.0) r = 0.0;
+    }
+    if (j < g.K) s.q[j] = q;
+    const bool none = m == -INF;  // the student's row is masked throughout
+    const double lp = none ? -(double)INF : (double)(l - m) * g.inv_t - ln_s;
+    double term = q > 0.0 || q != q ? q * (lq - lp) : 0.0;
+    double loss = add_block<NT>(term, s.red);  // its barriers publish s.q
+    double pr = 1.0;
+    if (g.tail && r > 0.0) {
+        const double lpr = (double)(t.m - m) * g.inv_t + log((double)t.s) - ln_s;
+        pr = exp(lpr);
+        loss += r * (log(r) - lpr);
+    }
+    const bool live = any && !none;
+    if (j == 0) g.loss[row] = any ? (float)loss : 0.f;
+    const double c = Q + r;
+    if (j < g.K && ok) {
+        double mine = 0.0;
+        for (int i = 0; i < g.K; ++i) mine += s.id[i] == id ? s.q[i] : 0.0;
+        *my_grad = live ? (float)(c * exp(lp) - mine) : 0.f;
+    }
+    if (!live) return 0.f;
+    if (!g.tail) return 1.f;
+    if (t.m == -INF || t.s == 0.f) return 0.f;  // no column besides the entries
+    return (float)(c * (r > 0.0 ? pr : exp((double)(t.m - m) * g.inv_t + log((double)t.s) - ln_s)) - r);
+}
+
+template <int NT, typename T>
+__device__ __forceinline__ void ds_store(const DsArgs& g, int64_t row, Sum t, DsLds<NT>& s) {
+    float grad = 0.f;
+    const float w = ds_finish<NT, T>(g, row, t, s, &grad);
+    if (g.stats) {
+        if (threadIdx.x < g.K) g.top_grad[row * g.K + threadIdx.x] = grad;
+        if (threadIdx.x == 0) {
+            g.stats[3 * row] = t.m;
+            g.stats[3 * row + 1] = t.s > 0.f || t.s != t.s ? log2f(t.s) : 0.f;
+            g.stats[3 * row + 2] = w;
+        }
+    }
+}
+
+// bit i of `bits`: column c0 + i is one of the row's teacher entries
+template <int NT>
+__device__ __forceinline__ void ds_bits(const DsArgs& g, int64_t row, int c0, int n, uint32_t* bits) {
+    for (int i = threadIdx.x; i < (n + 31) / 32; i += NT) bits[i] = 0;
+    __syncthreads();
+    for (int j = threadIdx.x; j < g.K; j += NT) {
+        const int64_t v = id_at(g.ids, g.ids_dtype, row * g.K + j);
+        if (v >= c0 && v < c0 + n) atomicOr(&bits[(v - c0) >> 5], 1u << ((v - c0) & 31));
+    }
+    __syncthreads();
+}
+
+template <int NT, typename T, bool TAIL>
+__global__ __launch_bounds__(NT) void distill_topk_kernel(const DsArgs g) {
+    extern __shared__ uint32_t bits[];
+    __shared__ Sum red[NT / 64];
+    __shared__ DsLds<NT> lds;
+    const int64_t row = blockIdx.x / (uint32_t)g.parts;
+    const int part = (int)(blockIdx.x % (uint32_t)g.parts), c0 = part * g.chunk, n = g.V - c0 < g.chunk ? g.V - c0 : g.chunk;
+    const T* x = static_cast<const T*>(g.x) + row * g.ld + c0;
+    if (TAIL) ds_bits<NT>(g, row, c0, n, bits);
+    float most;
+    const Sum t = read_sums<NT, false, TAIL>(x, n, g.c, bits, most, red);
+    if (g.parts == 1) ds_store<NT, T>(g, row, t, lds);
+    else if (threadIdx.x == 0) g.part[row * g.parts + part] = make_float4(t.m, t.s, t.u, 0.f);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void distill_topk_join_kernel(const DsArgs g) {
+    __shared__ DsLds<256> lds;
+    __shared__ Sum sums[4];
+    const int64_t row = blockIdx.x;
+    ds_store<256, T>(g, row, join_parts<256>(g.part + row * g.parts, g.parts, g.c, sums), lds);
+}
+
+template <int NT, typename T>
+__global__ __launch_bounds__(NT) void distill_topk_bwd_kernel(const GradArgs g) {
+    const int64_t row = blockIdx.x / (uint32_t)g.parts;
+    const int c0 = (int)(blockIdx.x % (uint32_t)g.parts) * g.chunk, n = g.V - c0 < g.chunk ? g.V - c0 : g.chunk;
+    const T* x = static_cast<const T*>(g.x) + row * g.ld + c0;
+    T* d = static_cast<T*>(g.d) + row * g.ldd + c0;
+    const float f = (g.dloss ? g.dloss[row] : 1.f) * g.inv_t, A = g.stats[3 * row + 2] * f;
+    if (A == 0.f) zero_row<NT>(d, n);
+    else grad_row<NT, T, false>(x, d, n, g.stats[3 * row], g.c, g.stats[3 * row + 1], A, 0.f);
+    __syncthreads();
+    for (int j = threadIdx.x; j < g.K; j += NT) {
+        const int64_t v = id_at(g.ids, g.ids_dtype, row * g.K + j);
+        if (v >= c0 && v < c0 + n) lp_store(d + (v - c0), f == 0.f ? 0.f : g.top_grad[row * g.K + j] * f);  // an id given twice has one value
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------------------------
+// Parts of a row: one, unless the rows alone do not fill the chip.
+void plan_parts(int64_t N, int64_t V, int64_t most, int64_t least, int& parts, int& chunk) {
+    int64_t p = mh_ceil_div(1024, N);
+    if (p > mh_ceil_div(V, 8192)) p = mh_ceil_div(V, 8192);
+    if (p > most) p = most;
+    if (p < least) p = least;
+    const int64_t c = mh_ceil_div(mh_ceil_div(V, p), 64) * 64;
+    chunk = (int)c;
+    parts = (int)mh_ceil_div(V, c);
+}
+void lp_plan(int64_t N, int64_t V, int k, int& parts, int& chunk) { plan_parts(N, V, k ? JOIN_MOST / k : 1024, 1, parts, chunk); }
+void ds_plan(int64_t N, int64_t V, bool tail, int& parts, int& chunk) { plan_parts(N, V, 1024, tail ? mh_ceil_div(V, TAIL_CHUNK - 64) : 1, parts, chunk); }
+
+int32_t ts_check(const char* who, const void* x, int32_t dtype, int64_t ld, int64_t N, int64_t V, int32_t ids_dtype, float T) {
+    MH_REQUIRE(N >= 0 && V >= 1 && V < ((int64_t)1 << 31) - 65536 && N < (int64_t)1 << 31 && ld >= V, "%s: sizes N=%lld V=%lld ld=%lld", who, (long long)N,
+               (long long)V, (long long)ld);
+    MH_REQUIRE(dtype == MH_F32 || dtype == MH_BF16 || dtype == MH_F16, "%s: unknown type %d", who, (int)dtype);
+    MH_REQUIRE(ids_dtype == MH_I32 || ids_dtype == MH_I64, "%s: ids must be int32 or int64", who);
+    MH_REQUIRE(T >= 1e-4f && T <= 1e4f, "%s: temperature %g is outside [1e-4, 1e4]", who, (double)T);
+    MH_REQUIRE(N == 0 || x, "%s: logits is NULL", who);
+    return MH_OK;
+}
+int32_t ts_grid(const char* who, int64_t N, int parts) {
+    MH_REQUIRE(N * parts < (int64_t)1 << 31, "%s: %lld rows in %d parts are too many", who, (long long)N, parts);
+    return MH_OK;
+}
+int32_t ts_workspace(const char* who, const void* ws, int64_t bytes, int64_t need) {
+    if (need > 0 && (!ws || bytes < need || (reinterpret_cast<uintptr_t>(ws) & 15))) {
+        mh_set_error("%s: workspace too small or not 16-byte aligned (%lld bytes, %lld needed)", who, (long long)bytes, (long long)need);
+        return MH_ERR_WORKSPACE;
+    }
+    return MH_OK;
+}
+
+// threads of a row's (or part's) workgroup
+constexpr int64_t SHORT_ROW = 4096;
+
+template <typename T>
+void lp_launch(const LpArgs& g, hipStream_t s) {
+    const dim3 grid((unsigned)(g.N * g.parts));
+    if (g.chunk <= SHORT_ROW) {
+        if (g.k) MH_LAUNCH((token_logprobs_kernel<256, T, true>), grid, dim3(256), 0, s, g);
+        else MH_LAUNCH((token_logprobs_kernel<256, T, false>), grid, dim3(256), 0, s, g);
+    } else {
+        if (g.k) MH_LAUNCH((token_logprobs_kernel<512, T, true>), grid, dim3(512), 0, s, g);
+        else MH_LAUNCH((token_logprobs_kernel<512, T, false>), grid, dim3(512), 0, s, g);
+    }
+    if (g.parts > 1) MH_LAUNCH(token_logprobs_join_kernel<T>, dim3((unsigned)g.N), dim3(512), 0, s, g);
+}
+template <typename T>
+void ds_launch(const DsArgs& g, hipStream_t s) {
+    const dim3 grid((unsigned)(g.N * g.parts));
+    const size_t lds = g.tail ? (size_t)(g.chunk + 31) / 32 * 4 : 0;
+    if (g.chunk <= SHORT_ROW) {
+        if (g.tail) MH_LAUNCH((distill_topk_kernel<256, T, true>), grid, dim3(256), lds, s, g);
+        else MH_LAUNCH((distill_topk_kernel<256, T, false>), grid, dim3(256), lds, s, g);
+    } else {
+        if (g.tail) MH_LAUNCH((distill_topk_kernel<512, T, true>), grid, dim3(512), lds, s, g);
+        else MH_LAUNCH((distill_topk_kernel<512, T, false>), grid, dim3(512), lds, s, g);
+    }
+    if (g.parts > 1) MH_LAUNCH(distill_topk_join_kernel<T>, dim3((unsigned)g.N), dim3(256), 0, s, g);
+}
+template <typename T>
+void grad_launch(GradArgs g, bool distill, hipStream_t s) {
+    plan_parts(g.N, g.V, 1 << 20, 1, g.parts, g.chunk);
+    const dim3 grid((unsigned)(g.N * g.parts));
+    if (distill) MH_LAUNCH((distill_topk_bwd_kernel<512, T>), grid, dim3(512), 0, s, g);
+    else MH_LAUNCH((token_logprobs_bwd_kernel<512, T>), grid, dim3(512), 0, s, g);
+}
+int32_t grad_any(const char* who, const GradArgs& g, int32_t dtype, bool distill, hipStream_t s) {
+    if (dtype == MH_F32) grad_launch<float>(g, distill, s);
+    else if (dtype == MH_BF16) grad_launch<lp_bf16>(g, distill, s);
+    else grad_launch<lp_f16>(g, distill, s);
+    MH_CHECK_LAUNCH(who);
+    return MH_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t mh_token_logprobs_workspace_bytes(int64_t N, int64_t V, int32_t k) {
+    if (N <= 0 || V <= 0 || V >= (int64_t)1 << 31 || k < 0 || k > TOP_MOST) return 0;
+    int parts, chunk;
+    lp_plan(N, V, k, parts, chunk);
+    return parts == 1 ? 0 : N * parts * (16 + 8 * (int64_t)k);
+}
+
+int32_t mh_token_logprobs(const void* logits, int32_t dtype, int64_t ld, int64_t N, int64_t V, const void* ids, int32_t ids_dtype, int32_t k,
+                          float temperature, float* logp, float* entropy, float* lse, float* top_logp, int32_t* top_ids, float* stats, void* workspace,
+                          int64_t workspace_bytes, mh_stream_t stream) {
+    if (int32_t rc = ts_check("mh_token_logprobs", logits, dtype, ld, N, V, ids_dtype, temperature)) return rc;
+    MH_REQUIRE(k >= 0 && k <= TOP_MOST && k <= V, "mh_token_logprobs: %d alternatives of %lld entries (at most %d)", (int)k, (long long)V, TOP_MOST);
+    if (N == 0) return MH_OK;
+    MH_REQUIRE(entropy && lse && stats && (!ids || logp) && (k == 0 || (top_logp && top_ids)), "mh_token_logprobs: an output is NULL");
+    LpArgs g = {};
+    g.x = logits, g.ld = ld, g.N = N, g.V = (int)V, g.k = k, g.ids = ids, g.ids_dtype = ids_dtype;
+    g.inv_t = 1.f / temperature, g.c = (float)(1.4426950408889634074 / (double)temperature);
+    g.logp = logp, g.entropy = entropy, g.lse = lse, g.top_logp = top_logp, g.top_ids = top_ids, g.stats = stats;
+    lp_plan(N, V, k, g.parts, g.chunk);
+    if (int32_t rc = ts_grid("mh_token_logprobs", N, g.parts)) return rc;
+    if (int32_t rc = ts_workspace("mh_token_logprobs", workspace, workspace_bytes, mh_token_logprobs_workspace_bytes(N, V, k))) return rc;
+    g.part = static_cast<float4*>(workspace);
+    g.tops = reinterpret_cast<uint64_t*>(g.part + N * g.parts);
+    hipStream_t s = mh_stream(stream);
+    if (dtype == MH_F32) lp_launch<float>(g, s);
+    else if (dtype == MH_BF16) lp_launch<lp_bf16>(g, s);
+    else lp_launch<lp_f16>(g, s);
+    MH_CHECK_LAUNCH("mh_token_logprobs");
+    return MH_OK;
+}
+
+int32_t mh_token_logprobs_bwd(const void* logits, int32_t dtype, int64_t ld, int64_t N, int64_t V, const void* ids, int32_t ids_dtype, float temperature,
+                              const float* stats, const float* entropy, const float* dlogp, const float* dentropy, const float* dlse, void* dlogits,
+                              int64_t ldd, mh_stream_t stream) {
+    if (int32_t rc = ts_check("mh_token_logprobs_bwd", logits, dtype, ld, N, V, ids_dtype, temperature)) return rc;
+    if (N == 0) return MH_OK;
+    MH_REQUIRE(stats && dlogits && ldd >= V && (!dentropy || entropy) && (!dlogp || ids), "mh_token_logprobs_bwd: an argument is NULL, or rows of %lld entries",
+               (long long)ldd);
+    GradArgs g = {};
+    g.x = logits, g.ld = ld, g.N = N, g.ldd = ldd, g.V = (int)V, g.ids = ids, g.ids_dtype = ids_dtype;
+    g.inv_t = 1.f / temperature, g.c = (float)(1.4426950408889634074 / (double)temperature);
+    g.stats = stats, g.entropy = entropy, g.dlogp = dlogp, g.dentropy = dentropy, g.dlse = dlse, g.d = dlogits;
+    return grad_any("mh_token_logprobs_bwd", g, dtype, false, mh_stream(stream));
+}
+
+int64_t mh_distill_topk_workspace_bytes(int64_t N, int64_t V, int32_t tail) {
+    if (N <= 0 || V <= 0 || V >= (int64_t)1 << 31) return 0;
+    int parts, chunk;
+    ds_plan(N, V, tail != 0, parts, chunk);
+    return parts == 1 ? 0 : N * parts * 16;
+}
+
+int32_t mh_distill_topk(const void* logits, int32_t dtype, int64_t ld, int64_t N, int64_t V, const void* teacher_ids, int32_t ids_dtype,
+                        const float* teacher_logp, int32_t K, float temperature, int32_t tail, float* loss, float* stats, float* top_grad, void* workspace,
+                        int64_t workspace_bytes, mh_stream_t stream) {
+    if (int32_t rc = ts_check("mh_distill_topk", logits, dtype, ld, N, V, ids_dtype, temperature)) return rc;
+    MH_REQUIRE(K >= 1 && K <= TOP_MOST, "mh_distill_topk: %d teacher entries a row (1 to %d)", (int)K, TOP_MOST);
+    if (N == 0) return MH_OK;
+    MH_REQUIRE(teacher_ids && teacher_logp && loss && (!stats == !top_grad), "mh_distill_topk: an argument is NULL");
+    DsArgs g = {};
+    g.x = logits, g.ld = ld, g.N = N, g.V = (int)V, g.K = K, g.tail = tail != 0, g.ids = teacher_ids, g.ids_dtype = ids_dtype, g.tlp = teacher_logp;
+    g.inv_t = 1.f / temperature, g.c = (float)(1.4426950408889634074 / (double)temperature);
+    g.loss = loss, g.stats = stats, g.top_grad = top_grad;
+    ds_plan(N, V, tail != 0, g.parts, g.chunk);
+    if (int32_t rc = ts_grid("mh_distill_topk", N, g.parts)) return rc;
+    if (int32_t rc = ts_workspace("mh_distill_topk", workspace, workspace_bytes, mh_distill_topk_workspace_bytes(N, V, tail))) return rc;
+    g.part = static_cast<float4*>(workspace);
+    hipStream_t s = mh_stream(stream);
+    if (dtype == MH_F32) ds_launch<float>(g, s);
+    else if (dtype == MH_BF16) ds_launch<lp_bf16>(g, s);
+    else ds_launch<lp_f16>(g, s);
+    MH_CHECK_LAUNCH("mh_distill_topk");
+    return MH_OK;
+}
+
+int32_t mh_distill_topk_bwd(const void* logits, int32_t dtype, int64_t ld, int64_t N, int64_t V, const void* teacher_ids, int32_t ids_dtype, int32_t K,
+                            float temperature, const float* stats, const float* top_grad, const float* dloss, void* dlogits, int64_t ldd,
+                            mh_stream_t stream) {
+    if (int32_t rc = ts_check("mh_distill_topk_bwd", logits, dtype, ld, N, V, ids_dtype, temperature)) return rc;
+    MH_REQUIRE(K >= 1 && K <= TOP_MOST, "mh_distill_topk_bwd: %d teacher entries a row (1 to %d)", (int)K, TOP_MOST);
+    if (N == 0) return MH_OK;
+    MH_REQUIRE(teacher_ids && stats && top_grad && dlogits && ldd >= V, "mh_distill_topk_bwd: an argument is NULL, or rows of %lld entries", (long long)ldd);
+    GradArgs g = {};
+    g.x = logits, g.ld = ld, g.N = N, g.ldd = ldd, g.V = (int)V, g.K = K, g.ids = teacher_ids, g.ids_dtype = ids_dtype;
+    g.inv_t = 1.f / temperature, g.c = (float)(1.4426950408889634074 / (double)temperature);
+    g.stats = stats, g.top_grad = top_grad, g.dloss = dloss, g.d = dlogits;
+    return grad_any("mh_distill_topk_bwd", g, dtype, true, mh_stream(stream));
+}
+
+}  // extern "C"

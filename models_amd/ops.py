@@ -27,6 +27,13 @@ __all__ = [
     "fp8_matmul",
     "fp8_linear",
     "fp8_linear_backward",
+    "TokenLogProbs",
+    "token_logprobs",
+    "token_logprobs_backward",
+    "DistillResult",
+    "distill_topk",
+    "distill_topk_train",
+    "distill_topk_backward",
 ]
 
 
@@ -2308,3 +2315,179 @@ def fp8_linear_backward(x: torch.Tensor, w: Fp8Matrix, dy: torch.Tensor, need_dx
             if need_dw:
                 dw = fp8_matmul(fp8_quantize(x, transpose=True), dyt)
     return (dx, dw, db) if need_db else (dx, dw)
+
+
+# --------------------------------------------------------------------------------------------
+# softmax over a catalogue's logits: log probabilities, entropy, alternatives; distillation
+# --------------------------------------------------------------------------------------------
+class TokenLogProbs(NamedTuple):
+    """Of each row of logits (``token_logprobs``), in float32."""
+
+    logp: Optional[torch.Tensor]      # [N] log probability of the given id (0 where the id is outside [0, V)); None without ids
+    entropy: torch.Tensor             # [N]
+    lse: torch.Tensor                 # [N] log-sum-exp of logits / temperature
+    top_logp: Optional[torch.Tensor]  # [N, k] log probabilities of the k largest, falling; -inf past the unmasked entries
+    top_ids: Optional[torch.Tensor]   # [N, k] int32; ties to the lowest index; -1 past the unmasked entries
+    stats: torch.Tensor               # [N, 2] for token_logprobs_backward
+
+
+def _row_ids(ids: Optional[torch.Tensor], shape, name: str):
+    """(ids, dtype code) of int32 / int64 ids of a given shape; None is allowed."""
+    if ids is None:
+        return None, MH_I32
+    _dev(ids, name)
+    code = _ids_dtype(ids, name)
+    if tuple(ids.shape) != tuple(shape) or not ids.is_contiguous():
+        raise ValueError(f"{name} must be contiguous {list(shape)}, got {tuple(ids.shape)}")
+    return ids, code
+
+
+def _row_floats(t: Optional[torch.Tensor], shape, name: str) -> Optional[torch.Tensor]:
+    if t is not None:
+        _dev(t, name, torch.float32)
+        if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous {list(shape)}, got {tuple(t.shape)}")
+    return t
+
+
+def _catalogue(logits: torch.Tensor, temperature: float):
+    """(type code, N, V) of catalogue logits, with the checks all of the following share."""
+    dt = _float_2d(logits, "logits")
+    N, V = logits.shape
+    if V < 1:
+        raise ValueError(f"logits must have at least one column, got shape {tuple(logits.shape)}")
+    if not 1e-4 <= float(temperature) <= 1e4:
+        raise ValueError(f"temperature must lie in [1e-4, 1e4], got {temperature}")
+    return dt, N, V
+
+
+def _dlogits(logits: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
+    """The gradient's buffer: ``out`` (``logits`` itself is allowed), or a new contiguous one."""
+    if out is None:
+        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    _float_2d(out, "out")
+    if out.shape != logits.shape or out.dtype != logits.dtype:
+        raise ValueError(f"out must be {list(logits.shape)} of {logits.dtype}, got {list(out.shape)} of {out.dtype}")
+    if out.data_ptr() == logits.data_ptr() and _ld(out) != _ld(logits):
+        raise ValueError("out may be the logits themselves, but not other rows that start where they start")
+    return out
+
+
+def token_logprobs(logits: torch.Tensor, ids: Optional[torch.Tensor] = None, k: int = 0, temperature: float = 1.0) -> TokenLogProbs:
+    """Log probability of ``ids[n]`` under ``softmax(logits[n] / temperature)``, the entropy, the log-sum-exp and the ``k`` largest entries
+    (at most 256) of each row, from one pass over ``logits`` [N, V] (float32 / bfloat16 / float16; rows may be parts of wider ones, as the
+    logits that ``inbatch_softmax`` or ``fp8_matmul`` returns).  Logits of -inf are masked; ids outside [0, V) are padding."""
+    lib = _lib.load()
+    dt, N, V = _catalogue(logits, temperature)
+    ids, idt = _row_ids(ids, (N,), "ids")
+    k = int(k)
+    if not 0 <= k <= min(V, 256):
+        raise ValueError(f"k must lie in [0, {min(V, 256)}], got {k}")
+    with _device_of(logits, ids):
+        f = torch.empty((5, N), dtype=torch.float32, device=logits.device)
+        logp, entropy, lse, stats = (f[0] if ids is not None else None), f[1], f[2], f[3:].view(N, 2)
+        top_logp = torch.empty((N, k), dtype=torch.float32, device=logits.device) if k else None
+        top_ids = torch.empty((N, k), dtype=torch.int32, device=logits.device) if k else None
+        if N:
+            need = lib.mh_token_logprobs_workspace_bytes(N, V, k)
+            ws = _scratch(need, logits) if need else None
+            with _timed("token_logprobs", nbytes=N * V * logits.element_size()):
+                check(lib.mh_token_logprobs(_ptr(logits), dt, _ld(logits), N, V, _ptr(ids), idt, k, float(temperature), _ptr(logp),
+                                            _ptr(entropy), _ptr(lse), _ptr(top_logp), _ptr(top_ids), _ptr(stats), _ptr(ws), need, _stream()),
+                      "mh_token_logprobs")
+    return TokenLogProbs(logp, entropy, lse, top_logp, top_ids, stats)
+
+
+def token_logprobs_backward(logits: torch.Tensor, ids: Optional[torch.Tensor], result: TokenLogProbs, dlogp: Optional[torch.Tensor] = None,
+                            dentropy: Optional[torch.Tensor] = None, dlse: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                            out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """d / d logits of ``sum(dlogp * logp + dentropy * entropy + dlse * lse)`` for the ``result`` of ``token_logprobs`` on the same logits,
+    ids and temperature; each of the three is ``[N]`` float32 or None.  ``out`` may be ``logits`` itself.  Padded ids take no ``dlogp``;
+    the top alternatives are to be read and have no gradient."""
+    lib = _lib.load()
+    dt, N, V = _catalogue(logits, temperature)
+    ids, idt = _row_ids(ids, (N,), "ids")
+    if dlogp is not None and ids is None:
+        raise ValueError("dlogp needs ids")
+    for t, n in ((dlogp, "dlogp"), (dentropy, "dentropy"), (dlse, "dlse"), (result.entropy, "result.entropy")):
+        _row_floats(t, (N,), n)
+    _row_floats(result.stats, (N, 2), "result.stats")
+    with _device_of(logits, ids, result.stats, dlogp, dentropy, dlse, out):
+        out = _dlogits(logits, out)
+        if N:
+            with _timed("token_logprobs_backward", nbytes=2 * N * V * logits.element_size()):
+                check(lib.mh_token_logprobs_bwd(_ptr(logits), dt, _ld(logits), N, V, _ptr(ids), idt, float(temperature), _ptr(result.stats),
+                                                _ptr(result.entropy), _ptr(dlogp), _ptr(dentropy), _ptr(dlse), _ptr(out), _ld(out), _stream()),
+                      "mh_token_logprobs_bwd")
+    return out
+
+
+class DistillResult(NamedTuple):
+    """Of each row (``distill_topk``), in float32."""
+
+    loss: torch.Tensor                # [N]
+    stats: Optional[torch.Tensor]     # [N, 3] and
+    top_grad: Optional[torch.Tensor]  # [N, K]: for distill_topk_backward; None without ``need_grad``
+
+
+def _teacher(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logp: torch.Tensor):
+    N = logits.shape[0]
+    if not isinstance(teacher_ids, torch.Tensor) or teacher_ids.dim() != 2 or not 1 <= teacher_ids.shape[1] <= 256:
+        raise ValueError("teacher_ids must be [N, K] with 1 to 256 entries a row")
+    K = teacher_ids.shape[1]
+    ids, idt = _row_ids(teacher_ids, (N, K), "teacher_ids")
+    if teacher_logp is not None:
+        _row_floats(teacher_logp, (N, K), "teacher_logp")
+    return ids, idt, K
+
+
+def distill_topk(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logp: torch.Tensor, temperature: float = 1.0, tail: bool = False,
+                 need_grad: bool = True) -> DistillResult:
+    """Kullback-Leibler divergence of ``softmax(logits / temperature)`` from a teacher of whom each row's top entries are known:
+    ``teacher_ids`` [N, K] and ``teacher_logp`` [N, K], as ``token_logprobs(teacher_logits, k=K, temperature=temperature)`` gives them.
+    ``tail=False``: the teacher's mass is the softmax of its K entries.  ``tail=True``: it is ``exp(teacher_logp)``, and what is left of 1 is
+    held against the student's probability outside the entries.  Ids outside [0, V) are left out; a row without any has loss 0."""
+    lib = _lib.load()
+    dt, N, V = _catalogue(logits, temperature)
+    if teacher_logp is None:
+        raise ValueError("teacher_logp is needed")
+    ids, idt, K = _teacher(logits, teacher_ids, teacher_logp)
+    with _device_of(logits, ids, teacher_logp):
+        loss = torch.empty((N,), dtype=torch.float32, device=logits.device)
+        stats = torch.empty((N, 3), dtype=torch.float32, device=logits.device) if need_grad else None
+        top_grad = torch.empty((N, K), dtype=torch.float32, device=logits.device) if need_grad else None
+        if N:
+            need = lib.mh_distill_topk_workspace_bytes(N, V, int(tail))
+            ws = _scratch(need, logits) if need else None
+            with _timed("distill_topk", nbytes=N * V * logits.element_size()):
+                check(lib.mh_distill_topk(_ptr(logits), dt, _ld(logits), N, V, _ptr(ids), idt, _ptr(teacher_logp), K, float(temperature),
+                                          int(tail), _ptr(loss), _ptr(stats), _ptr(top_grad), _ptr(ws), need, _stream()), "mh_distill_topk")
+    return DistillResult(loss, stats, top_grad)
+
+
+def distill_topk_backward(logits: torch.Tensor, teacher_ids: torch.Tensor, result: DistillResult, dloss: Optional[torch.Tensor] = None,
+                          temperature: float = 1.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """d / d logits of ``sum(dloss * loss)`` (``dloss`` [N] float32; None: ones) for the ``result`` of ``distill_topk`` on the same logits, ids
+    and temperature.  ``out`` may be ``logits`` itself."""
+    lib = _lib.load()
+    dt, N, V = _catalogue(logits, temperature)
+    ids, idt, K = _teacher(logits, teacher_ids, None)
+    if result.stats is None or result.top_grad is None:
+        raise ValueError("the result of distill_topk(..., need_grad=False) has no gradient")
+    _row_floats(result.stats, (N, 3), "result.stats")
+    _row_floats(result.top_grad, (N, K), "result.top_grad")
+    _row_floats(dloss, (N,), "dloss")
+    with _device_of(logits, ids, result.stats, result.top_grad, dloss, out):
+        out = _dlogits(logits, out)
+        if N:
+            with _timed("distill_topk_backward", nbytes=2 * N * V * logits.element_size()):
+                check(lib.mh_distill_topk_bwd(_ptr(logits), dt, _ld(logits), N, V, _ptr(ids), idt, K, float(temperature), _ptr(result.stats),
+                                              _ptr(result.top_grad), _ptr(dloss), _ptr(out), _ld(out), _stream()), "mh_distill_topk_bwd")
+    return out
+
+
+def distill_topk_train(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logp: torch.Tensor, dloss: Optional[torch.Tensor] = None,
+                       temperature: float = 1.0, tail: bool = False, out: Optional[torch.Tensor] = None) -> Tuple[DistillResult, torch.Tensor]:
+    """A training step's ``(distill_topk(...), distill_topk_backward(..., dloss))`` where the row weights ``dloss`` [N] are known beforehand."""
+    result = distill_topk(logits, teacher_ids, teacher_logp, temperature, tail)
+    return result, distill_topk_backward(logits, teacher_ids, result, dloss, temperature, out)
