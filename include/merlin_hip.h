@@ -742,17 +742,17 @@ int32_t mh_token_logprobs_bwd(const void* logits, int32_t dtype, int64_t ld, int
                               float temperature, const float* stats, const float* entropy, const float* dlogp, const float* dentropy,
                               const float* dlse, void* dlogits, int64_t ldd, mh_stream_t stream);
 /* CategoricalCrossEntropy against a teacher's few entries (tf/losses/listwise.py:38-52 with soft targets), as a Kullback-Leibler divergence.
- * teacher_ids / teacher_logp [N, K], K <= 256: ids outside [0, V) are left out; an id given twice counts with both masses.  tail == 0: q =
+ * teacher_ids / teacher_logp [N, K], K <= 256, leading dimensions ld_ids / ld_logp: ids outside [0, V) are left out; an id given twice counts with both masses.  tail == 0: q =
  * softmax of the row's entries of teacher_logp (any constant may be added to a row); tail != 0: q = exp(teacher_logp), and what is left of 1
  * is held against the student's probability outside the entries.  loss[n] = sum q (log q - log p) (+ r (log r - log p_rest)); a row without
  * entries has loss 0 and no gradient; one whose student row is masked throughout has loss +inf and no gradient.  stats [N, 3] and top_grad
  * [N, K] (both or neither NULL) are for _bwd: dlogits = dloss[n] (1 where dloss is NULL) * d loss / d logits, may be logits itself. */
 int64_t mh_distill_topk_workspace_bytes(int64_t N, int64_t V, int32_t tail);
 int32_t mh_distill_topk(const void* logits, int32_t dtype, int64_t ld, int64_t N, int64_t V, const void* teacher_ids, int32_t ids_dtype,
-                        const float* teacher_logp, int32_t K, float temperature, int32_t tail, float* loss, float* stats, float* top_grad,
-                        void* workspace, int64_t workspace_bytes, mh_stream_t stream);
+                        int64_t ld_ids, const float* teacher_logp, int64_t ld_logp, int32_t K, float temperature, int32_t tail, float* loss,
+                        float* stats, float* top_grad, void* workspace, int64_t workspace_bytes, mh_stream_t stream);
 int32_t mh_distill_topk_bwd(const void* logits, int32_t dtype, int64_t ld, int64_t N, int64_t V, const void* teacher_ids, int32_t ids_dtype,
-                            int32_t K, float temperature, const float* stats, const float* top_grad, const float* dloss, void* dlogits,
+                            int64_t ld_ids, int32_t K, float temperature, const float* stats, const float* top_grad, const float* dloss, void* dlogits,
                             int64_t ldd, mh_stream_t stream);
 
 /* ---- launch recorder: a train step traced once, replayed without re-entering the host language ----------------------------

@@ -461,6 +461,7 @@ struct GradArgs {
     int V, K, parts, chunk;
     const void* ids;
     int ids_dtype;
+    int64_t ld_ids;  // distill_topk
     float inv_t, c;
     const float *stats, *entropy, *dlogp, *dentropy, *dlse;  // token_logprobs: stats [N, 2]
     const float *top_grad, *dloss;                           // distill_topk: stats [N, 3] (maximum, log2 sum, weight)
@@ -557,6 +558,7 @@ struct DsArgs {
     int V, K, parts, chunk, tail;
     const void* ids;
     int ids_dtype;
+    int64_t ld_ids, ld_tlp;
     const float* tlp;
     float inv_t, c;
     float *loss, *stats, *top_grad;
@@ -578,10 +580,10 @@ __device__ __forceinline__ float ds_finish(const DsArgs& g, int64_t row, Sum& t,
     int id = -1;
     float l = -INF, tl = -INF;
     if (j < g.K) {
-        const int64_t v = id_at(g.ids, g.ids_dtype, row * g.K + j);
+        const int64_t v = id_at(g.ids, g.ids_dtype, row * g.ld_ids + j);
         if (v >= 0 && v < g.V) {
             id = (int)v;
-            tl = g.tlp[row * g.K + j];
+            tl = g.tlp[row * g.ld_tlp + j];
             l = lp_float(static_cast<const T*>(g.x)[row * g.ld + id]);
         }
         s.id[j] = id;
@@ -664,7 +666,7 @@ __device__ __forceinline__ void ds_bits(const DsArgs& g, int64_t row, int c0, in
     for (int i = threadIdx.x; i < (n + 31) / 32; i += NT) bits[i] = 0;
     __syncthreads();
     for (int j = threadIdx.x; j < g.K; j += NT) {
-        const int64_t v = id_at(g.ids, g.ids_dtype, row * g.K + j);
+        const int64_t v = id_at(g.ids, g.ids_dtype, row * g.ld_ids + j);
         if (v >= c0 && v < c0 + n) atomicOr(&bits[(v - c0) >> 5], 1u << ((v - c0) & 31));
     }
     __syncthreads();
@@ -704,7 +706,7 @@ __global__ __launch_bounds__(NT) void distill_topk_bwd_kernel(const GradArgs g) 
     else grad_row<NT, T, false>(x, d, n, g.stats[3 * row], g.c, g.stats[3 * row + 1], A, 0.f);
     __syncthreads();
     for (int j = threadIdx.x; j < g.K; j += NT) {
-        const int64_t v = id_at(g.ids, g.ids_dtype, row * g.K + j);
+        const int64_t v = id_at(g.ids, g.ids_dtype, row * g.ld_ids + j);
         if (v >= c0 && v < c0 + n) lp_store(d + (v - c0), f == 0.f ? 0.f : g.top_grad[row * g.K + j] * f);  // an id given twice has one value
     }
 }
@@ -844,14 +846,15 @@ int64_t mh_distill_topk_workspace_bytes(int64_t N, int64_t V, int32_t tail) {
 }
 
 int32_t mh_distill_topk(const void* logits, int32_t dtype, int64_t ld, int64_t N, int64_t V, const void* teacher_ids, int32_t ids_dtype,
-                        const float* teacher_logp, int32_t K, float temperature, int32_t tail, float* loss, float* stats, float* top_grad, void* workspace,
-                        int64_t workspace_bytes, mh_stream_t stream) {
+                        int64_t ld_ids, const float* teacher_logp, int64_t ld_logp, int32_t K, float temperature, int32_t tail, float* loss, float* stats,
+                        float* top_grad, void* workspace, int64_t workspace_bytes, mh_stream_t stream) {
     if (int32_t rc = ts_check("mh_distill_topk", logits, dtype, ld, N, V, ids_dtype, temperature)) return rc;
     MH_REQUIRE(K >= 1 && K <= TOP_MOST, "mh_distill_topk: %d teacher entries a row (1 to %d)", (int)K, TOP_MOST);
     if (N == 0) return MH_OK;
-    MH_REQUIRE(teacher_ids && teacher_logp && loss && (!stats == !top_grad), "mh_distill_topk: an argument is NULL");
+    MH_REQUIRE(teacher_ids && teacher_logp && loss && (!stats == !top_grad) && ld_ids >= K && ld_logp >= K,
+               "mh_distill_topk: an argument is NULL, or the teacher's rows are shorter than %d", (int)K);
     DsArgs g = {};
-    g.x = logits, g.ld = ld, g.N = N, g.V = (int)V, g.K = K, g.tail = tail != 0, g.ids = teacher_ids, g.ids_dtype = ids_dtype, g.tlp = teacher_logp;
+    g.x = logits, g.ld = ld, g.N = N, g.V = (int)V, g.K = K, g.tail = tail != 0, g.ids = teacher_ids, g.ids_dtype = ids_dtype, g.tlp = teacher_logp, g.ld_ids = ld_ids, g.ld_tlp = ld_logp;
     g.inv_t = 1.f / temperature, g.c = (float)(1.4426950408889634074 / (double)temperature);
     g.loss = loss, g.stats = stats, g.top_grad = top_grad;
     ds_plan(N, V, tail != 0, g.parts, g.chunk);
@@ -866,15 +869,16 @@ int32_t mh_distill_topk(const void* logits, int32_t dtype, int64_t ld, int64_t N
     return MH_OK;
 }
 
-int32_t mh_distill_topk_bwd(const void* logits, int32_t dtype, int64_t ld, int64_t N, int64_t V, const void* teacher_ids, int32_t ids_dtype, int32_t K,
+int32_t mh_distill_topk_bwd(const void* logits, int32_t dtype, int64_t ld, int64_t N, int64_t V, const void* teacher_ids, int32_t ids_dtype, int64_t ld_ids, int32_t K,
                             float temperature, const float* stats, const float* top_grad, const float* dloss, void* dlogits, int64_t ldd,
                             mh_stream_t stream) {
     if (int32_t rc = ts_check("mh_distill_topk_bwd", logits, dtype, ld, N, V, ids_dtype, temperature)) return rc;
     MH_REQUIRE(K >= 1 && K <= TOP_MOST, "mh_distill_topk_bwd: %d teacher entries a row (1 to %d)", (int)K, TOP_MOST);
     if (N == 0) return MH_OK;
-    MH_REQUIRE(teacher_ids && stats && top_grad && dlogits && ldd >= V, "mh_distill_topk_bwd: an argument is NULL, or rows of %lld entries", (long long)ldd);
+    MH_REQUIRE(teacher_ids && stats && top_grad && dlogits && ldd >= V && ld_ids >= K, "mh_distill_topk_bwd: an argument is NULL, or rows of %lld entries",
+               (long long)ldd);
     GradArgs g = {};
-    g.x = logits, g.ld = ld, g.N = N, g.ldd = ldd, g.V = (int)V, g.K = K, g.ids = teacher_ids, g.ids_dtype = ids_dtype;
+    g.x = logits, g.ld = ld, g.N = N, g.ldd = ldd, g.V = (int)V, g.K = K, g.ids = teacher_ids, g.ids_dtype = ids_dtype, g.ld_ids = ld_ids;
     g.inv_t = 1.f / temperature, g.c = (float)(1.4426950408889634074 / (double)temperature);
     g.stats = stats, g.top_grad = top_grad, g.dloss = dloss, g.d = dlogits;
     return grad_any("mh_distill_topk_bwd", g, dtype, true, mh_stream(stream));

@@ -2430,15 +2430,21 @@ class DistillResult(NamedTuple):
     top_grad: Optional[torch.Tensor]  # [N, K]: for distill_topk_backward; None without ``need_grad``
 
 
-def _teacher(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logp: torch.Tensor):
+def _teacher(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logp: Optional[torch.Tensor] = None):
+    """(id dtype code, K) of a teacher's entries ``[N, K]``, whose rows may be parts of wider ones."""
     N = logits.shape[0]
-    if not isinstance(teacher_ids, torch.Tensor) or teacher_ids.dim() != 2 or not 1 <= teacher_ids.shape[1] <= 256:
-        raise ValueError("teacher_ids must be [N, K] with 1 to 256 entries a row")
-    K = teacher_ids.shape[1]
-    ids, idt = _row_ids(teacher_ids, (N, K), "teacher_ids")
+    _dev(teacher_ids, "teacher_ids")
+    idt = _ids_dtype(teacher_ids, "teacher_ids")
     if teacher_logp is not None:
-        _row_floats(teacher_logp, (N, K), "teacher_logp")
-    return ids, idt, K
+        _dev(teacher_logp, "teacher_logp", torch.float32)
+    for t, n in ((teacher_ids, "teacher_ids"), (teacher_logp, "teacher_logp")):
+        if t is None:
+            continue
+        if t.dim() != 2 or t.shape[0] != N or not 1 <= t.shape[1] <= 256 or t.shape[1] != teacher_ids.shape[1]:
+            raise ValueError(f"{n} must be [{N}, K] with 1 to 256 entries a row, got {list(t.shape)}")
+        if (t.shape[1] > 1 and t.stride(1) != 1) or (N > 1 and t.stride(0) < t.shape[1]):
+            raise ValueError(f"{n} must have contiguous rows that do not overlap, got strides {t.stride()}")
+    return idt, teacher_ids.shape[1]
 
 
 def distill_topk(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logp: torch.Tensor, temperature: float = 1.0, tail: bool = False,
@@ -2451,8 +2457,8 @@ def distill_topk(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logp: 
     dt, N, V = _catalogue(logits, temperature)
     if teacher_logp is None:
         raise ValueError("teacher_logp is needed")
-    ids, idt, K = _teacher(logits, teacher_ids, teacher_logp)
-    with _device_of(logits, ids, teacher_logp):
+    idt, K = _teacher(logits, teacher_ids, teacher_logp)
+    with _device_of(logits, teacher_ids, teacher_logp):
         loss = torch.empty((N,), dtype=torch.float32, device=logits.device)
         stats = torch.empty((N, 3), dtype=torch.float32, device=logits.device) if need_grad else None
         top_grad = torch.empty((N, K), dtype=torch.float32, device=logits.device) if need_grad else None
@@ -2460,8 +2466,9 @@ def distill_topk(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logp: 
             need = lib.mh_distill_topk_workspace_bytes(N, V, int(tail))
             ws = _scratch(need, logits) if need else None
             with _timed("distill_topk", nbytes=N * V * logits.element_size()):
-                check(lib.mh_distill_topk(_ptr(logits), dt, _ld(logits), N, V, _ptr(ids), idt, _ptr(teacher_logp), K, float(temperature),
-                                          int(tail), _ptr(loss), _ptr(stats), _ptr(top_grad), _ptr(ws), need, _stream()), "mh_distill_topk")
+                check(lib.mh_distill_topk(_ptr(logits), dt, _ld(logits), N, V, _ptr(teacher_ids), idt, _ld(teacher_ids),
+                                          _ptr(teacher_logp), _ld(teacher_logp), K, float(temperature), int(tail), _ptr(loss), _ptr(stats),
+                                          _ptr(top_grad), _ptr(ws), need, _stream()), "mh_distill_topk")
     return DistillResult(loss, stats, top_grad)
 
 
@@ -2471,18 +2478,18 @@ def distill_topk_backward(logits: torch.Tensor, teacher_ids: torch.Tensor, resul
     and temperature.  ``out`` may be ``logits`` itself."""
     lib = _lib.load()
     dt, N, V = _catalogue(logits, temperature)
-    ids, idt, K = _teacher(logits, teacher_ids, None)
+    idt, K = _teacher(logits, teacher_ids)
     if result.stats is None or result.top_grad is None:
         raise ValueError("the result of distill_topk(..., need_grad=False) has no gradient")
     _row_floats(result.stats, (N, 3), "result.stats")
     _row_floats(result.top_grad, (N, K), "result.top_grad")
     _row_floats(dloss, (N,), "dloss")
-    with _device_of(logits, ids, result.stats, result.top_grad, dloss, out):
+    with _device_of(logits, teacher_ids, result.stats, result.top_grad, dloss, out):
         out = _dlogits(logits, out)
         if N:
             with _timed("distill_topk_backward", nbytes=2 * N * V * logits.element_size()):
-                check(lib.mh_distill_topk_bwd(_ptr(logits), dt, _ld(logits), N, V, _ptr(ids), idt, K, float(temperature), _ptr(result.stats),
-                                              _ptr(result.top_grad), _ptr(dloss), _ptr(out), _ld(out), _stream()), "mh_distill_topk_bwd")
+                check(lib.mh_distill_topk_bwd(_ptr(logits), dt, _ld(logits), N, V, _ptr(teacher_ids), idt, _ld(teacher_ids), K,
+                                              float(temperature), _ptr(result.stats), _ptr(result.top_grad), _ptr(dloss), _ptr(out), _ld(out), _stream()), "mh_distill_topk_bwd")
     return out
 
 

@@ -284,6 +284,9 @@ def check_distill(x, ids, tlp, T, tail, rng):
     ones = ops.distill_topk_backward(x, ids, parts, temperature=T)
     gt1 = (rel * mag + 2.0 ** -126 * 3 / T) * (1 + HALF[x.dtype]) + HALF[x.dtype] * np.abs(grad) + LEAST[x.dtype]
     close(ones.double().cpu().numpy(), grad, gt1)
+    i2, t2 = (torch.cat([a, a.flip(1)], 1)[:, : a.shape[1]] for a in (ids, tlp))  # parts of wider rows
+    r2, d2 = ops.distill_topk_train(x, i2, t2, w, T, tail)
+    assert torch.equal(d2, d) and torch.equal(r2.loss, res.loss)
     y = x.clone()
     _, inplace = ops.distill_topk_train(y, ids, tlp, w, T, tail, out=y)
     assert inplace.data_ptr() == y.data_ptr() and torch.equal(inplace, d)
@@ -429,7 +432,8 @@ def test_refusals(device):
                 lambda: ops.token_logprobs_backward(x, ids, r, dlogp=one, out=x[:, :9]),
                 lambda: ops.token_logprobs_backward(x[:3], ids[:3], r, dlogp=one[:3]),
                 lambda: ops.distill_topk(x, tid[:3], tlp), lambda: ops.distill_topk(x, tid, tlp[:, :2]), lambda: ops.distill_topk(x, tid, None),
-                lambda: ops.distill_topk(x, tid[:, :0], tlp[:, :0]), lambda: ops.distill_topk(x, tid[:, 0], tlp),
+                lambda: ops.distill_topk(x, tid[:, :0], tlp[:, :0]), lambda: ops.distill_topk(x, tid[:, 0], tlp), lambda: ops.distill_topk(x, tid[:, ::2], tlp[:, :2]),
+                lambda: ops.distill_topk(x, tid, tlp[:1].expand(4, 3)),
                 lambda: ops.distill_topk(x, torch.zeros(4, 257, dtype=torch.int64, device=device), torch.zeros(4, 257, device=device)),
                 lambda: ops.distill_topk_backward(x, tid, ops.distill_topk(x, tid, tlp, need_grad=False)),
                 lambda: ops.distill_topk_backward(x, tid, s, dloss=one[:3]), lambda: ops.distill_topk_train(x, tid, tlp, one[:3])):

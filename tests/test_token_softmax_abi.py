@@ -18,8 +18,8 @@ def call(name, order, defaults, **kw):
 POINTERS = {"x", "ids", "logp", "ent", "lse", "tlogp", "tids", "stats", "ws", "stream", "g", "h", "c", "d", "tlp", "loss", "top", "w"}
 LP = dict(x=A, dt=0, ld=1000, N=2, V=1000, ids=A, idt=1, k=5, T=1.0, logp=A, ent=A, lse=A, tlogp=A, tids=A, stats=A, ws=A, nws=1 << 20, stream=0)
 LPB = dict(x=A, dt=0, ld=1000, N=2, V=1000, ids=A, idt=1, T=1.0, stats=A, ent=A, g=A, h=A, c=A, d=A, ldd=1000, stream=0)
-DS = dict(x=A, dt=0, ld=1000, N=2, V=1000, ids=A, idt=1, tlp=A, K=5, T=1.0, tail=1, loss=A, stats=A, top=A, ws=A, nws=1 << 20, stream=0)
-DSB = dict(x=A, dt=0, ld=1000, N=2, V=1000, ids=A, idt=1, K=5, T=1.0, stats=A, top=A, w=A, d=A, ldd=1000, stream=0)
+DS = dict(x=A, dt=0, ld=1000, N=2, V=1000, ids=A, idt=1, ldi=5, tlp=A, ldt=5, K=5, T=1.0, tail=1, loss=A, stats=A, top=A, ws=A, nws=1 << 20, stream=0)
+DSB = dict(x=A, dt=0, ld=1000, N=2, V=1000, ids=A, idt=1, ldi=5, K=5, T=1.0, stats=A, top=A, w=A, d=A, ldd=1000, stream=0)
 COMMON = [dict(x=None), dict(dt=3), dict(ld=999), dict(N=-1), dict(V=0), dict(V=(1 << 31) - 1, ld=1 << 31), dict(idt=2), dict(T=0.0), dict(T=float("nan")),
           dict(T=-1.0), dict(T=1e5), dict(stats=None)]
 
@@ -35,12 +35,12 @@ def test_logprobs_bwd_refuses(kw):
     assert call("mh_token_logprobs_bwd", LPB, LPB, **kw) == -1
 
 
-@pytest.mark.parametrize("kw", COMMON + [dict(K=0), dict(K=257), dict(ids=None), dict(tlp=None), dict(loss=None), dict(top=None)])
+@pytest.mark.parametrize("kw", COMMON + [dict(K=0), dict(K=257), dict(ids=None), dict(tlp=None), dict(loss=None), dict(top=None), dict(ldi=4), dict(ldt=4)])
 def test_distill_refuses(kw):
     assert call("mh_distill_topk", DS, DS, **kw) == -1
 
 
-@pytest.mark.parametrize("kw", COMMON + [dict(K=0), dict(K=257), dict(ids=None), dict(top=None), dict(d=None), dict(ldd=10)])
+@pytest.mark.parametrize("kw", COMMON + [dict(K=0), dict(K=257), dict(ids=None), dict(top=None), dict(d=None), dict(ldd=10), dict(ldi=4)])
 def test_distill_bwd_refuses(kw):
     assert call("mh_distill_topk_bwd", DSB, DSB, **kw) == -1
 
