@@ -9,6 +9,8 @@
 // summed axis contiguous and padded with zeros to whole blocks, so the loop has no tail in k.
 #include "mh_lowp.h"
 
+#include <type_traits>
+
 namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -208,33 +210,29 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_gemm_kernel(const F8Args 
     const int64_t m0 = (int64_t)(group * 8 + in % rows) * BM, n0 = (int64_t)(in / rows) * BN;
     const int kb0 = blockIdx.y * g.kb_split, kb1 = kb0 + g.kb_split < g.kblocks ? kb0 + g.kb_split : g.kblocks;
 
-    const uint8_t* src[DMA];
+    // sources of this thread's loads as 32-bit offsets from the tile's first rows (rows past the end repeat the last: never stored)
+    const uint8_t *const ta = g.a + m0 * g.lda, *const tb = g.b + n0 * g.ldb, *const tas = g.as + m0 * g.ldas, *const tbs = g.bs + n0 * g.ldbs;
+    const int ma = g.M - m0 < BM ? (int)(g.M - m0) - 1 : BM - 1, nb = g.N - n0 < BN ? (int)(g.N - n0) - 1 : BN - 1;
+    constexpr int DA = BM * 8 / NT;
+    uint32_t src[DMA];
 #pragma unroll
     for (int j = 0; j < DMA; ++j) {
-        const int L = j * NT + threadIdx.x, r = L >> 3, c = (L & 7) ^ ((r >> 1) & 7);
-        if (r < BM) {
-            const int64_t row = m0 + r < g.M ? m0 + r : g.M - 1;  // rows past the end repeat the last: never stored
-            src[j] = g.a + row * g.lda + c * 16;
-        } else {
-            const int64_t row = n0 + r - BM < g.N ? n0 + r - BM : g.N - 1;
-            src[j] = g.b + row * g.ldb + c * 16;
-        }
-    }
-    const uint8_t* ssrc[SDMA];
-#pragma unroll
-    for (int j = 0; j < SDMA; ++j) {
-        const int r = j * NT + threadIdx.x;
-        if (r < BM) ssrc[j] = g.as + (m0 + r < g.M ? m0 + r : g.M - 1) * g.ldas;
-        else ssrc[j] = g.bs + (n0 + r - BM < g.N ? n0 + r - BM : g.N - 1) * g.ldbs;
+        const int L = (j < DA ? j : j - DA) * NT + threadIdx.x, r = L >> 3, c = (L & 7) ^ ((r >> 1) & 7);
+        src[j] = j < DA ? (uint32_t)((r < ma ? r : ma) * g.lda) + c * 16 : (uint32_t)((r < nb ? r : nb) * g.ldb) + c * 16;
     }
     uint8_t* const sbase = smem + 2 * STAGE;
-    auto issue = [&](int kb) {
-        uint8_t* st = smem + (kb & 1) * STAGE;
+    auto issue = [&](int kb, int stage) {
+        uint8_t* st = smem + (stage & 1) * STAGE;
+        const uint8_t *pa = ta + (int64_t)kb * 128, *pb = tb + (int64_t)kb * 128;
 #pragma unroll
-        for (int j = 0; j < DMA; ++j) f8_dma16(src[j] + (int64_t)kb * 128, st + (j * NT + wave * 64) * 16);
-        if ((kb & 3) == 0) {  // four blocks' scales, one word a row
+        for (int j = 0; j < DMA; ++j) f8_dma16((j < DA ? pa : pb) + src[j], st + (j * NT + wave * 64) * 16);
+    };
+    auto issue_scales = [&](int kb, int group) {  // of four blocks, one word a row
 #pragma unroll
-            for (int j = 0; j < SDMA; ++j) f8_dma4(ssrc[j] + kb, sbase + ((kb >> 2) & 1) * SCALES + (j * NT + wave * 64) * 4);
+        for (int j = 0; j < SDMA; ++j) {
+            const int r = j * NT + threadIdx.x;
+            const uint8_t* p = r < BM ? tas + (r < ma ? r : ma) * g.ldas : tbs + (r - BM < nb ? r - BM : nb) * g.ldbs;
+            f8_dma4(p + (kb & ~3), sbase + (group & 1) * SCALES + (j * NT + wave * 64) * 4);
         }
     };
     f32x16 acc[TM][TN];
@@ -244,61 +242,98 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_gemm_kernel(const F8Args 
         for (int j = 0; j < TN; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    int ar[TM], br[TN];
+    // where this lane's fragments lie in a stage: its row, and in it the two chunks of each half of the block
+    const int arow = (wm * (BM / WM) + l31) * 128, brow = (BM + wn * (BN / WN) + l31) * 128, sw = (l31 >> 1) & 7;
+    const int chunk[2][2] = {{((2 * h) ^ sw) << 4, ((2 * h + 1) ^ sw) << 4}, {((4 + 2 * h) ^ sw) << 4, ((5 + 2 * h) ^ sw) << 4}};
+    auto read = [&](int kb, int half, int row) {
+        const uint8_t* st = smem + (kb & 1) * STAGE + row;
+        const i32x4 x = *reinterpret_cast<const i32x4*>(st + chunk[half][0]);
+        const i32x4 y = *reinterpret_cast<const i32x4*>(st + chunk[half][1]);
+        return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    int sa[TM], sb[TN], ta_[TM], tb_[TN];
+    auto read_scales = [&](int kb, int (&x)[TM], int (&y)[TN]) {
+        const uint8_t* sp = sbase + ((kb >> 2) & 1) * SCALES + (kb & 3);
 #pragma unroll
-    for (int i = 0; i < TM; ++i) ar[i] = wm * (BM / WM) + i * 32 + l31;
+        for (int i = 0; i < TM; ++i) x[i] = sp[arow / 32 + i * 128];
 #pragma unroll
-    for (int j = 0; j < TN; ++j) br[j] = BM + wn * (BN / WN) + j * 32 + l31;
-    uint32_t sa[TM], sb[TN];
-    issue(kb0);
-    for (int kb = kb0; kb < kb1; ++kb) {
-        // block kb has arrived, and every wavefront is done with the stage that block kb + 1 takes
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (kb + 1 < kb1) issue(kb + 1);
-        const uint8_t* st = smem + (kb & 1) * STAGE;
-        if ((kb & 3) == 0) {
-            const uint32_t* sp = reinterpret_cast<const uint32_t*>(sbase + ((kb >> 2) & 1) * SCALES);
+        for (int j = 0; j < TN; ++j) y[j] = sp[brow / 32 + j * 128];
+    };
+    // A block is 2 TM steps: a step multiplies one 32-row fragment of a with the TN fragments of b, over half of the block.  a's fragments
+    // are read two steps ahead into a ring of four, b's for the next half within the half before.  The barrier of a block lies two steps
+    // before the end of the block before it, so the matrix pipe has work on both sides of it.
+    constexpr int S = 2 * TM;
+    i32x8 fa[4], fb[2][TN];
+    bf16x8 wb[TN][4];
+    auto widen_b = [&](int half) {
+        if (WIDE) {
 #pragma unroll
-            for (int i = 0; i < TM; ++i) sa[i] = sp[ar[i]];
-#pragma unroll
-            for (int j = 0; j < TN; ++j) sb[j] = sp[br[j]];
+            for (int j = 0; j < TN; ++j) f8_widen(fb[half][j], __uint_as_float((uint32_t)sb[j] << 23), wb[j]);
         }
-        const int sh = (kb & 3) * 8;
+    };
+    auto multiply = [&](int step) {
+        const int i = step % TM, half = step / TM;
+        if (!WIDE) {
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-            const int c = 4 * hh + 2 * h;
-            auto frag = [&](int r) {
-                const i32x4 lo = *reinterpret_cast<const i32x4*>(st + r * 128 + ((c ^ ((r >> 1) & 7)) << 4));
-                const i32x4 hi = *reinterpret_cast<const i32x4*>(st + r * 128 + (((c + 1) ^ ((r >> 1) & 7)) << 4));
-                return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-            };
-            if (!WIDE) {
-                i32x8 fa[TM], fb[TN];
+            for (int j = 0; j < TN; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[half][j], fa[step & 3], acc[i][j], 0, 0, 0, sb[j], 0, sa[i]);
+        } else {
+            bf16x8 wa[4];
+            f8_widen(fa[step & 3], __uint_as_float((uint32_t)sa[i] << 23), wa);
 #pragma unroll
-                for (int j = 0; j < TN; ++j) fb[j] = frag(br[j]);
+            for (int q = 0; q < 4; ++q)
 #pragma unroll
-                for (int i = 0; i < TM; ++i) fa[i] = frag(ar[i]);
+                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wb[j][q], wa[q], acc[i][j], 0, 0, 0);
+        }
+    };
+    issue_scales(kb0, kb0 >> 2);
+    issue(kb0, kb0);
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    issue(kb0 + 1 < kb1 ? kb0 + 1 : kb0, kb0 + 1);
+    read_scales(kb0, sa, sb);
 #pragma unroll
-                for (int i = 0; i < TM; ++i)
+    for (int j = 0; j < TN; ++j) fb[0][j] = read(kb0, 0, brow + j * 4096);
+    fa[0] = read(kb0, 0, arow);
+    fa[1] = read(kb0, 0, arow + 4096);
+    // No branch in the body, or the compiler moves the multiplications behind the barrier: past the end the loads repeat the last block, into
+    // the stage that would have been its turn, and what is read of it is not used.
+    auto body = [&](int kb, bool scales) {
+        const int one = kb + 1, two = kb + 2 < kb1 ? kb + 2 : kb1 - 1;
 #pragma unroll
-                    for (int j = 0; j < TN; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[j], fa[i], acc[i][j], 0, 0, 0, (int)(sb[j] >> sh), 0, (int)(sa[i] >> sh));
-            } else {
-                bf16x8 wb[TN][4];
+        for (int step = 0; step < S; ++step) {
+            if (step == S - 2) {
+                // block kb + 1 has arrived, and every wavefront holds what it still needs of block kb
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                if (scales) issue_scales(two, (kb + 2) >> 2);
+                issue(two, kb);
+                read_scales(one, ta_, tb_);
 #pragma unroll
-                for (int j = 0; j < TN; ++j) f8_widen(frag(br[j]), __uint_as_float(((sb[j] >> sh) & 255u) << 23), wb[j]);
-#pragma unroll
-                for (int i = 0; i < TM; ++i) {
-                    bf16x8 wa[4];
-                    f8_widen(frag(ar[i]), __uint_as_float(((sa[i] >> sh) & 255u) << 23), wa);
-#pragma unroll
-                    for (int s = 0; s < 4; ++s)
-#pragma unroll
-                        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wb[j][s], wa[s], acc[i][j], 0, 0, 0);
-                }
+                for (int j = 0; j < TN; ++j) fb[0][j] = read(one, 0, brow + j * 4096);
             }
+            if (step + 2 < S) fa[(step + 2) & 3] = read(kb, (step + 2) / TM, arow + (step + 2) % TM * 4096);
+            else fa[(step + 2) & 3] = read(one, 0, arow + (step + 2 - S) * 4096);
+            if (step == TM - 2) {
+#pragma unroll
+                for (int j = 0; j < TN; ++j) fb[1][j] = read(kb, 1, brow + j * 4096);
+            }
+            if (step % TM == 0) widen_b(step / TM);
+            multiply(step);
+            __builtin_amdgcn_sched_barrier(0);
         }
+#pragma unroll
+        for (int i = 0; i < TM; ++i) sa[i] = ta_[i];
+#pragma unroll
+        for (int j = 0; j < TN; ++j) sb[j] = tb_[j];
+    };
+    int kb = kb0;
+    for (; kb + 4 <= kb1; kb += 4) {
+        body(kb, false);
+        body(kb + 1, false);
+        body(kb + 2, true);  // the next four blocks' scales, beside the first of them
+        body(kb + 3, false);
     }
+    for (; kb < kb1; ++kb) body(kb, false);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last repeated loads
     // acc[i][j][4 q + e] = C[m0 + .. + l31][n0 + .. + 8 q + 4 h + e]
     const int64_t slab = (int64_t)blockIdx.y * g.slab;
 #pragma unroll
@@ -317,57 +352,123 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_gemm_kernel(const F8Args 
         }
 }
 
-// Few rows of a (at most 16 MT): bound by reading b once.  A workgroup takes 16 rows of b; its wavefronts take the blocks of k in turn, each
+// 32 entries at x as 8-bit values and their scale's byte: the quantiser's own rule, the four lanes that share a block and a row agreeing on it
+template <typename T>
+__device__ __forceinline__ i32x8 f8_quantize32(const T* x, int left, uint32_t& scale) {
+    float v[32], a = 0.f;
+    if (left >= 32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float w[8];
+            lp_load8(x + 8 * i, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[8 * i + j] = w[j];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = i < left ? lp_float(x[i]) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 32; ++i) a = fmaxf(a, q_mag(v[i]));
+    a = fmaxf(a, __shfl_xor(a, 16));
+    a = fmaxf(a, __shfl_xor(a, 32));
+    const int e = q_exponent(a);
+    const float inv = q_pow2(-e);
+    scale = (uint32_t)(e + 127);
+    i32x8 r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = (int)q_pack4(v[4 * i] * inv, v[4 * i + 1] * inv, v[4 * i + 2] * inv, v[4 * i + 3] * inv);
+    return r;
+}
+struct f8_stored {};  // in place of an element type: a is in its 8-bit form
+
+// Few rows of a (at most 16 MT): bound by reading b once.  A workgroup takes 16 NB rows of b; its wavefronts take the blocks of k in turn, each
 // lane 32 bytes of a row straight into the registers that the 16 x 16 x 128 instruction reads, and the partial sums meet in LDS in a fixed order.
-template <int MT, bool WIDE>
-__global__ __launch_bounds__(1024) void fp8_rows_kernel(const F8Args g) {
+// X: the type of a where it is quantised on the way (at most 16 rows: the work is done again by every workgroup), or f8_stored.
+template <int MT, int NB, bool WIDE, typename X>
+__global__ __launch_bounds__(512) void fp8_rows_kernel(const F8Args g, const X* __restrict__ x, int64_t ldx, int K) {
+    constexpr bool STORED = std::is_same<X, f8_stored>::value;
     extern __shared__ __attribute__((aligned(16))) float part[];  // [waves][MT][256]
-    const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6, lane = threadIdx.x & 63, l15 = lane & 15, h = lane >> 4;
-    const int64_t n0 = (int64_t)blockIdx.x * 16;
-    const int64_t n = n0 + l15 < g.N ? n0 + l15 : g.N - 1;
-    const uint8_t *pb = g.b + n * g.ldb + h * 32, *psb = g.bs + n * g.ldbs;
-    const uint8_t *pa[MT], *psa[MT];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, lane = threadIdx.x & 63, l15 = lane & 15, h = lane >> 4;
+    const int64_t n0 = (int64_t)blockIdx.x * (16 * NB);
+    const uint8_t *pb[NB], *psb[NB], *pa[MT], *psa[MT];
+    const X* px[MT];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+        const int64_t n = n0 + 16 * j + l15 < g.N ? n0 + 16 * j + l15 : g.N - 1;
+        pb[j] = g.b + n * g.ldb + h * 32;
+        psb[j] = g.bs + n * g.ldbs;
+    }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         const int64_t m = 16 * i + l15 < g.M ? 16 * i + l15 : g.M - 1;
-        pa[i] = g.a + m * g.lda + h * 32;
-        psa[i] = g.as + m * g.ldas;
+        if constexpr (STORED) {
+            pa[i] = g.a + m * g.lda + h * 32;
+            psa[i] = g.as + m * g.ldas;
+        } else {
+            px[i] = x + m * ldx + h * 32;
+        }
     }
-    f32x4 acc[MT];
+    f32x4 acc[MT][NB];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int kb = wave; kb < g.kblocks; kb += waves) {
-        const i32x8 vb = *reinterpret_cast<const i32x8*>(pb + (int64_t)kb * 128);
-        const uint32_t sb = psb[kb];
-        bf16x8 wb[4];
-        if (WIDE) f8_widen(vb, __uint_as_float(sb << 23), wb);
+        i32x8 vb[NB], va[MT];
+        uint32_t sb[NB], sa[MT];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            vb[j] = *reinterpret_cast<const i32x8*>(pb[j] + (int64_t)kb * 128);
+            sb[j] = psb[j][kb];
+        }
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-            const i32x8 va = *reinterpret_cast<const i32x8*>(pa[i] + (int64_t)kb * 128);
-            const uint32_t sa = psa[i][kb];
-            if (!WIDE) {
-                acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vb, va, acc[i], 0, 0, 0, (int)sb, 0, (int)sa);
+            if constexpr (STORED) {
+                va[i] = *reinterpret_cast<const i32x8*>(pa[i] + (int64_t)kb * 128);
+                sa[i] = psa[i][kb];
             } else {
-                bf16x8 wa[4];
-                f8_widen(va, __uint_as_float(sa << 23), wa);
+                va[i] = f8_quantize32(px[i] + (int64_t)kb * 128, K - kb * 128 - h * 32, sa[i]);
+            }
+        }
+        if (!WIDE) {
 #pragma unroll
-                for (int s = 0; s < 4; ++s) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[s], wa[s], acc[i], 0, 0, 0);
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vb[j], va[i], acc[i][j], 0, 0, 0, (int)sb[j], 0, (int)sa[i]);
+        } else {
+            bf16x8 wa[MT][4];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) f8_widen(va[i], __uint_as_float(sa[i] << 23), wa[i]);
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+                bf16x8 wb[4];
+                f8_widen(vb[j], __uint_as_float(sb[j] << 23), wb);
+#pragma unroll
+                for (int s = 0; s < 4; ++s)
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[s], wa[i][s], acc[i][j], 0, 0, 0);
             }
         }
     }
-    // acc[i][e] = C[16 i + l15][n0 + 4 h + e]
+    // acc[i][j][e] = C[16 i + l15][n0 + 16 j + 4 h + e]
 #pragma unroll
-    for (int i = 0; i < MT; ++i) *reinterpret_cast<f32x4*>(&part[(wave * MT + i) * 256 + l15 * 16 + h * 4]) = acc[i];
-    __syncthreads();
-    for (int t = threadIdx.x; t < MT * 64; t += blockDim.x) {
-        f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        for (int w = 0; w < waves; ++w) v += *reinterpret_cast<const f32x4*>(&part[w * MT * 256 + t * 4]);
-        const int64_t m = t / 4, nn = n0 + (t & 3) * 4;
-        if (m >= g.M) continue;
-        if (g.bias)
-            for (int e = 0; e < 4; ++e)
-                if (nn + e < g.N) v[e] += g.bias[nn + e];
-        f8_store4(g, m, nn, v[0], v[1], v[2], v[3], 0);
+    for (int j = 0; j < NB; ++j) {
+        if (j) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < MT; ++i) *reinterpret_cast<f32x4*>(&part[(wave * MT + i) * 256 + l15 * 16 + h * 4]) = acc[i][j];
+        __syncthreads();
+        for (int t = threadIdx.x; t < MT * 64; t += blockDim.x) {
+            f32x4 v = {0.f, 0.f, 0.f, 0.f};
+            for (int w = 0; w < waves; ++w) v += *reinterpret_cast<const f32x4*>(&part[w * MT * 256 + t * 4]);
+            const int64_t m = t / 4, nn = n0 + 16 * j + (t & 3) * 4;
+            if (m >= g.M) continue;
+            if (g.bias)
+                for (int e = 0; e < 4; ++e)
+                    if (nn + e < g.N) v[e] += g.bias[nn + e];
+            f8_store4(g, m, nn, v[0], v[1], v[2], v[3], 0);
+        }
     }
 }
 
@@ -388,7 +489,9 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(const float* __restrict__
     f8_store4(g, m, n, v[0], v[1], v[2], v[3], 0);
 }
 
-constexpr int ROWS_MOST = 64;  // rows of a that the streaming kernel takes
+constexpr int64_t MOST_K = (1 << 24) - 128;  // a tile's rows lie within 32 bits of its first
+constexpr int ROWS_MOST = 64;   // rows of a that the streaming kernel takes
+constexpr int FUSED_MOST = 16;  // ... and quantises itself
 
 struct F8Plan {
     bool rows, big;
@@ -439,14 +542,26 @@ int32_t f8_launch_tiles(F8Args g, int slices, bool wide, hipStream_t s) {
     return MH_OK;
 }
 
-template <bool WIDE>
+template <int MT, int NB, typename X>
+void f8_launch_rows_nb(const F8Args& g, const X* x, int64_t ldx, int K, hipStream_t s) {
+    const int waves = g.kblocks >= 8 ? 8 : 4;
+    const dim3 grid((unsigned)mh_ceil_div(g.N, 16 * NB)), block(waves * 64);
+    if (g.kind != MH_BF16) MH_LAUNCH((fp8_rows_kernel<MT, NB, true, X>), grid, block, (size_t)waves * MT * 1024, s, g, x, ldx, K);
+    else MH_LAUNCH((fp8_rows_kernel<MT, NB, false, X>), grid, block, (size_t)waves * MT * 1024, s, g, x, ldx, K);
+}
+template <int MT>
 void f8_launch_rows(const F8Args& g, hipStream_t s) {
+    const f8_stored* none = nullptr;
+    // more rows of b a workgroup: a is read fewer times, as long as the workgroups still fill the chip
+    if (g.N >= 4 * 16 * 192) f8_launch_rows_nb<MT, 4>(g, none, 0, 0, s);
+    else if (g.N >= 2 * 16 * 192) f8_launch_rows_nb<MT, 2>(g, none, 0, 0, s);
+    else f8_launch_rows_nb<MT, 1>(g, none, 0, 0, s);
+}
+void f8_launch_rows_any(const F8Args& g, hipStream_t s) {
     const int mt = (int)mh_ceil_div(g.M, 16);
-    const int waves = g.kblocks >= 32 ? 16 : g.kblocks >= 8 ? 8 : 4;
-    const dim3 grid((unsigned)mh_ceil_div(g.N, 16)), block(waves * 64);
-    if (mt == 1) MH_LAUNCH((fp8_rows_kernel<1, WIDE>), grid, block, (size_t)waves * 1024, s, g);
-    else if (mt == 2) MH_LAUNCH((fp8_rows_kernel<2, WIDE>), grid, block, (size_t)waves * 2048, s, g);
-    else MH_LAUNCH((fp8_rows_kernel<4, WIDE>), grid, block, (size_t)waves * 4096, s, g);
+    if (mt == 1) f8_launch_rows<1>(g, s);
+    else if (mt == 2) f8_launch_rows<2>(g, s);
+    else f8_launch_rows<4>(g, s);
 }
 
 int32_t f8_check_matrix(const char* who, const char* name, const void* q, int64_t ld, const void* s, int64_t lds, int64_t rows, int64_t K) {
@@ -459,21 +574,26 @@ int32_t f8_check_matrix(const char* who, const char* name, const void* q, int64_
     return MH_OK;
 }
 
-int32_t f8_matmul(const char* who, const uint8_t* a, int64_t lda, const uint8_t* as, int64_t ldas, const uint8_t* b, int64_t ldb, const uint8_t* bs,
-                  int64_t ldbs, int64_t M, int64_t N, int64_t K, const float* bias, int32_t kind, void* out, int64_t ldo, void* ws, int64_t ws_bytes,
-                  hipStream_t s) {
+F8Args f8_args(const uint8_t* a, int64_t lda, const uint8_t* as, int64_t ldas, const uint8_t* b, int64_t ldb, const uint8_t* bs, int64_t ldbs, int64_t M,
+               int64_t N, int64_t K, const float* bias, int32_t kind, void* out, int64_t ldo) {
     F8Args g = {};
     g.a = a, g.as = as, g.b = b, g.bs = bs, g.lda = lda, g.ldas = ldas, g.ldb = ldb, g.ldbs = ldbs, g.M = M, g.N = N;
     g.kblocks = (int)mh_ceil_div(K, 128);
     g.bias = bias, g.kind = kind, g.out = out, g.ldo = ldo;
     const int64_t es = kind == MH_F32 ? 4 : 2;
     g.vec = ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) % (4 * es)) == 0;
+    return g;
+}
+
+int32_t f8_matmul(const char* who, const uint8_t* a, int64_t lda, const uint8_t* as, int64_t ldas, const uint8_t* b, int64_t ldb, const uint8_t* bs,
+                  int64_t ldbs, int64_t M, int64_t N, int64_t K, const float* bias, int32_t kind, void* out, int64_t ldo, void* ws, int64_t ws_bytes,
+                  hipStream_t s) {
+    F8Args g = f8_args(a, lda, as, ldas, b, ldb, bs, ldbs, M, N, K, bias, kind, out, ldo);
     const F8Plan p = f8_plan(M, N, K);
     const bool wide = kind != MH_BF16;
     g.kb_split = p.kb_split;
     if (p.rows) {
-        if (wide) f8_launch_rows<true>(g, s);
-        else f8_launch_rows<false>(g, s);
+        f8_launch_rows_any(g, s);
         MH_CHECK_LAUNCH(who);
         return MH_OK;
     }
@@ -517,7 +637,7 @@ int64_t f8_q_bytes(int64_t rows, int64_t K) { return mh_ceil_div(rows * mh_ceil_
 int64_t f8_s_bytes(int64_t rows, int64_t K) { return mh_ceil_div(rows * mh_ceil_div(mh_ceil_div(K, 128), 4) * 4, 256) * 256; }
 
 int32_t f8_check_out(const char* who, int64_t M, int64_t N, int64_t K, int32_t kind, const void* out, int64_t ldo) {
-    MH_REQUIRE(M >= 0 && N >= 0 && K >= 1 && K < (int64_t)1 << 31 && M < (int64_t)1 << 31 && N < (int64_t)1 << 31, "%s: sizes M=%lld N=%lld K=%lld", who,
+    MH_REQUIRE(M >= 0 && N >= 0 && K >= 1 && K <= MOST_K && M < (int64_t)1 << 31 && N < (int64_t)1 << 31, "%s: sizes M=%lld N=%lld K=%lld", who,
                (long long)M, (long long)N, (long long)K);
     MH_REQUIRE(kind == MH_F32 || kind == MH_BF16 || kind == MH_F16, "%s: unknown output type %d", who, (int)kind);
     MH_REQUIRE(ldo >= N && (out || M * N == 0), "%s: output rows of %lld entries cannot hold %lld", who, (long long)ldo, (long long)N);
@@ -567,12 +687,13 @@ int32_t mh_fp8_matmul(const void* a, int64_t lda, const void* a_scales, int64_t 
     if (M == 0 || N == 0) return MH_OK;
     if (int32_t rc = f8_check_matrix("mh_fp8_matmul", "a", a, lda, a_scales, ldas, M, K)) return rc;
     if (int32_t rc = f8_check_matrix("mh_fp8_matmul", "b", b, ldb, b_scales, ldbs, N, K)) return rc;
+    MH_REQUIRE(lda <= 1 << 24 && ldb <= 1 << 24, "mh_fp8_matmul: rows of %lld and %lld entries (at most 2^24)", (long long)lda, (long long)ldb);
     return f8_matmul("mh_fp8_matmul", static_cast<const uint8_t*>(a), lda, static_cast<const uint8_t*>(a_scales), ldas, static_cast<const uint8_t*>(b), ldb,
                      static_cast<const uint8_t*>(b_scales), ldbs, M, N, K, bias, out_dtype, out, ldo, workspace, workspace_bytes, mh_stream(stream));
 }
 
 int64_t mh_fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-    return M > 0 && N > 0 && K > 0 ? f8_q_bytes(M, K) + f8_s_bytes(M, K) + f8_part_bytes(M, N, K) : 0;
+    return M > FUSED_MOST && N > 0 && K > 0 ? f8_q_bytes(M, K) + f8_s_bytes(M, K) + f8_part_bytes(M, N, K) : 0;
 }
 
 int32_t mh_fp8_linear(const void* x, int32_t x_dtype, int64_t ldx, const void* w, int64_t ldw, const void* w_scales, int64_t ldws, int64_t M, int64_t N,
@@ -581,6 +702,19 @@ int32_t mh_fp8_linear(const void* x, int32_t x_dtype, int64_t ldx, const void* w
     if (int32_t rc = f8_check_out("mh_fp8_linear", M, N, K, out_dtype, out, ldo)) return rc;
     if (M == 0 || N == 0) return MH_OK;
     if (int32_t rc = f8_check_matrix("mh_fp8_linear", "w", w, ldw, w_scales, ldws, N, K)) return rc;
+    MH_REQUIRE(ldw <= 1 << 24, "mh_fp8_linear: rows of %lld entries (at most 2^24)", (long long)ldw);
+    if (M <= FUSED_MOST) {
+        MH_REQUIRE(x && ldx >= K, "mh_fp8_linear: x is NULL or its rows are shorter than %lld", (long long)K);
+        MH_REQUIRE(x_dtype == MH_F32 || x_dtype == MH_BF16 || x_dtype == MH_F16, "mh_fp8_linear: unknown type %d", (int)x_dtype);
+        const F8Args g = f8_args(nullptr, 0, nullptr, 0, static_cast<const uint8_t*>(w), ldw, static_cast<const uint8_t*>(w_scales), ldws, M, N, K, bias, out_dtype,
+                                 out, ldo);
+        hipStream_t s = mh_stream(stream);
+        if (x_dtype == MH_F32) f8_launch_rows_nb<1, 1>(g, static_cast<const float*>(x), ldx, (int)K, s);
+        else if (x_dtype == MH_BF16) f8_launch_rows_nb<1, 1>(g, static_cast<const lp_bf16*>(x), ldx, (int)K, s);
+        else f8_launch_rows_nb<1, 1>(g, static_cast<const lp_f16*>(x), ldx, (int)K, s);
+        MH_CHECK_LAUNCH("mh_fp8_linear");
+        return MH_OK;
+    }
     if (!workspace || workspace_bytes < mh_fp8_linear_workspace_bytes(M, N, K)) {
         mh_set_error("mh_fp8_linear: workspace too small (%lld bytes)", (long long)workspace_bytes);
         return MH_ERR_WORKSPACE;

@@ -2134,34 +2134,25 @@ _FLOATS = {torch.float32: _lib.MH_F32, torch.bfloat16: _lib.MH_BF16, torch.float
 _FP8_BLOCK = 128
 
 
-class _NoSwitch:
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        return False
-
-
-_NO_SWITCH = _NoSwitch()
-
-
-def _device_of(first: torch.Tensor, *others: Optional[torch.Tensor]):
-    """The context in which a call on ``first`` launches: its own device is made the current one where it is not (the stream is that device's
-    current stream), and every other tensor has to be on it."""
+def _elsewhere(first: torch.Tensor, *others: Optional[torch.Tensor]) -> bool:
+    """Whether ``first`` lies on another device than the current one (the call is then made again with that device current, so that it launches
+    on that device's current stream); every other tensor has to lie where ``first`` does."""
+    at = first.get_device()
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != at:
             raise ValueError(f"all tensors of a call must be on one device, got {first.device} and {t.device}")
-    return _NO_SWITCH if first.device.index == torch.cuda.current_device() else torch.cuda.device(first.device)
+    return at != torch.cuda.current_device()
 
 
 def _float_2d(t: torch.Tensor, name: str) -> int:
     """The type code of a 2-D fp32 / bf16 / fp16 tensor whose rows are contiguous (any distance between rows)."""
     _dev(t, name)
-    if t.dtype not in _FLOATS:
+    code = _FLOATS.get(t.dtype)
+    if code is None:
         raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
-    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+    if t.dim() != 2 or not (t.is_contiguous() or ((t.stride(1) == 1 or t.shape[1] <= 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]))):
         raise ValueError(f"{name} must be 2-D with contiguous rows that do not overlap, got shape {tuple(t.shape)}, strides {t.stride()}")
-    return _FLOATS[t.dtype]
+    return code
 
 
 def _ld(t: torch.Tensor) -> int:
@@ -2169,9 +2160,33 @@ def _ld(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
 
 
-def _scratch(nbytes: int, like: torch.Tensor) -> torch.Tensor:
+def _at(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def _here() -> int:
+    """The current device's current stream (what ``_stream`` gives, without the objects around it: these calls can be a few microseconds)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
+class _Untimed:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_UNTIMED = _Untimed()
+
+
+def _if_timed(name: str, nbytes: int = 0, flops: int = 0):
+    return _timed(name, nbytes, flops) if TIMER.enabled else _UNTIMED
+
+
+def _scratch(nbytes: int, like: torch.Tensor) -> Optional[torch.Tensor]:
     """Scratch of one call, from the caching allocator on the current stream: calls on two streams, and two captured graphs, never share it."""
-    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=like.device)
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
 
 
 class Fp8Matrix(NamedTuple):
@@ -2184,16 +2199,16 @@ class Fp8Matrix(NamedTuple):
 
 def _fp8_check(m: Fp8Matrix, name: str) -> Tuple[int, int]:
     v, s, K = m
-    _dev(v, f"{name}.values", torch.float8_e4m3fn)
-    _dev(s, f"{name}.scales", torch.uint8)
-    kp = -(-int(K) // _FP8_BLOCK) * _FP8_BLOCK
-    if K < 1 or v.dim() != 2 or s.dim() != 2 or v.shape[1] != kp or s.shape != (v.shape[0], -(-(kp // _FP8_BLOCK) // 4) * 4):
+    _dev(v, name, torch.float8_e4m3fn)
+    _dev(s, name, torch.uint8)
+    kb = -(-K // _FP8_BLOCK)
+    if K < 1 or v.dim() != 2 or s.dim() != 2 or v.shape[1] != kb * _FP8_BLOCK or s.shape[0] != v.shape[0] or s.shape[1] != -(-kb // 4) * 4:
         raise ValueError(f"{name}: values {tuple(v.shape)} and scales {tuple(s.shape)} are not the 8-bit form of a matrix of {K} columns")
     if not (v.is_contiguous() and s.is_contiguous()):
         raise ValueError(f"{name}: values and scales must be contiguous")
-    if s.device != v.device:
+    if s.get_device() != v.get_device():
         raise ValueError(f"{name}: values and scales must be on one device")
-    return v.shape[0], int(K)
+    return v.shape[0], K
 
 
 def fp8_quantize(x: torch.Tensor, transpose: bool = False, column_sums: bool = False):
@@ -2209,16 +2224,19 @@ def fp8_quantize(x: torch.Tensor, transpose: bool = False, column_sums: bool = F
     rows, cols = (K, R) if transpose else (R, K)
     if cols < 1:
         raise ValueError(f"fp8_quantize needs at least one entry along the blocks, got shape {tuple(x.shape)}")
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return fp8_quantize(x, transpose, column_sums)
     kb = -(-cols // _FP8_BLOCK)
-    with _device_of(x):
-        q = torch.empty((rows, kb * _FP8_BLOCK), dtype=torch.float8_e4m3fn, device=x.device)
-        s = torch.empty((rows, -(-kb // 4) * 4), dtype=torch.uint8, device=x.device)
-        sums = torch.empty((K,), dtype=torch.float32, device=x.device) if column_sums else None
-        if rows:
-            ws = _scratch(4 * kb * K, x) if column_sums else None
-            with _timed("fp8_quantize", nbytes=R * K * (x.element_size() + 1)):
-                check(lib.mh_fp8_quantize(_ptr(x), dt, _ld(x), R, K, int(transpose), _ptr(q), q.shape[1], _ptr(s), s.shape[1], _ptr(sums),
-                                          _ptr(ws), 0 if ws is None else ws.numel(), _stream()), "mh_fp8_quantize")
+    q = torch.empty((rows, kb * _FP8_BLOCK), dtype=torch.float8_e4m3fn, device=x.device)
+    s = torch.empty((rows, -(-kb // 4) * 4), dtype=torch.uint8, device=x.device)
+    sums = torch.empty((K,), dtype=torch.float32, device=x.device) if column_sums else None
+    if rows:
+        need = 4 * kb * K if column_sums else 0
+        ws = _scratch(need, x)
+        with _if_timed("fp8_quantize", R * K * (x.element_size() + 1)):
+            check(lib.mh_fp8_quantize(x.data_ptr(), dt, _ld(x), R, K, int(transpose), q.data_ptr(), q.shape[1], s.data_ptr(), s.shape[1],
+                                      _at(sums), _at(ws), need, _here()), "mh_fp8_quantize")
     m = Fp8Matrix(q, s, cols)
     return (m, sums) if column_sums else m
 
@@ -2234,12 +2252,11 @@ def _fp8_out(M: int, N: int, out: Optional[torch.Tensor], out_dtype, device) -> 
     return out
 
 
-def _fp8_bias(bias: Optional[torch.Tensor], N: int) -> Optional[torch.Tensor]:
+def _fp8_bias(bias: Optional[torch.Tensor], N: int) -> None:
     if bias is not None:
         _dev(bias, "bias", torch.float32)
         if bias.numel() != N or not bias.is_contiguous():
             raise ValueError(f"bias must be contiguous with {N} entries")
-    return bias
 
 
 def fp8_matmul(a: Fp8Matrix, b: Fp8Matrix, bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32,
@@ -2253,14 +2270,17 @@ def fp8_matmul(a: Fp8Matrix, b: Fp8Matrix, bias: Optional[torch.Tensor] = None, 
     if K != Kb:
         raise ValueError(f"a has {K} columns and b {Kb}")
     _fp8_bias(bias, N)
-    with _device_of(a.values, b.values, bias, out):
-        out = _fp8_out(M, N, out, out_dtype, a.values.device)
-        if M and N:
-            ws = _scratch(lib.mh_fp8_matmul_workspace_bytes(M, N, K), out)
-            with _timed("fp8_matmul", nbytes=(M + N) * K + M * N * out.element_size(), flops=2 * M * N * K):
-                check(lib.mh_fp8_matmul(_ptr(a.values), a.values.shape[1], _ptr(a.scales), a.scales.shape[1], _ptr(b.values),
-                                        b.values.shape[1], _ptr(b.scales), b.scales.shape[1], M, N, K, _ptr(bias), _FLOATS[out_dtype],
-                                        _ptr(out), _ld(out), _ptr(ws), ws.numel(), _stream()), "mh_fp8_matmul")
+    if _elsewhere(a.values, b.values, bias, out):
+        with torch.cuda.device(a.values.device):
+            return fp8_matmul(a, b, bias, out_dtype, out)
+    out = _fp8_out(M, N, out, out_dtype, a.values.device)
+    if M and N:
+        need = lib.mh_fp8_matmul_workspace_bytes(M, N, K)
+        ws = _scratch(need, out)
+        with _if_timed("fp8_matmul", (M + N) * K + M * N * out.element_size(), 2 * M * N * K):
+            check(lib.mh_fp8_matmul(a.values.data_ptr(), a.values.shape[1], a.scales.data_ptr(), a.scales.shape[1], b.values.data_ptr(),
+                                    b.values.shape[1], b.scales.data_ptr(), b.scales.shape[1], M, N, K, _at(bias), _FLOATS[out_dtype],
+                                    out.data_ptr(), _ld(out), _at(ws), need, _here()), "mh_fp8_matmul")
     return out
 
 
@@ -2275,14 +2295,16 @@ def fp8_linear(x: torch.Tensor, w: Fp8Matrix, bias: Optional[torch.Tensor] = Non
     if x.shape[1] != K:
         raise ValueError(f"x has {x.shape[1]} columns and w {K}")
     _fp8_bias(bias, N)
-    with _device_of(x, w.values, bias, out):
-        out = _fp8_out(M, N, out, out_dtype, x.device)
-        if M and N:
-            ws = _scratch(lib.mh_fp8_linear_workspace_bytes(M, N, K), x)
-            with _timed("fp8_linear", nbytes=M * K * x.element_size() + N * K + M * N * out.element_size(), flops=2 * M * N * K):
-                check(lib.mh_fp8_linear(_ptr(x), dt, _ld(x), _ptr(w.values), w.values.shape[1], _ptr(w.scales), w.scales.shape[1], M, N, K,
-                                        _ptr(bias), _FLOATS[out_dtype], _ptr(out), _ld(out), _ptr(ws), ws.numel(), _stream()),
-                      "mh_fp8_linear")
+    if _elsewhere(x, w.values, bias, out):
+        with torch.cuda.device(x.device):
+            return fp8_linear(x, w, bias, out_dtype, out)
+    out = _fp8_out(M, N, out, out_dtype, x.device)
+    if M and N:
+        need = lib.mh_fp8_linear_workspace_bytes(M, N, K)
+        ws = _scratch(need, x)
+        with _if_timed("fp8_linear", M * K * x.element_size() + N * K + M * N * out.element_size(), 2 * M * N * K):
+            check(lib.mh_fp8_linear(x.data_ptr(), dt, _ld(x), w.values.data_ptr(), w.values.shape[1], w.scales.data_ptr(), w.scales.shape[1], M, N,
+                                    K, _at(bias), _FLOATS[out_dtype], out.data_ptr(), _ld(out), _at(ws), need, _here()), "mh_fp8_linear")
     return out
 
 
@@ -2302,18 +2324,20 @@ def fp8_linear_backward(x: torch.Tensor, w: Fp8Matrix, dy: torch.Tensor, need_dx
         rows, cols = _fp8_check(w, "w")
         if (rows, cols) != (K, N):
             raise ValueError(f"w must be the 8-bit form of the [{K}, {N}] kernel, got [{rows}, {cols}]")
-    with _device_of(x, dy, w.values if need_dx else None):
-        if need_dx:
-            dx = fp8_matmul(fp8_quantize(dy), w)
-        if M == 0:
-            dw = torch.zeros((K, N), dtype=torch.float32, device=x.device) if need_dw else None
-            db = torch.zeros((N,), dtype=torch.float32, device=x.device) if need_db else None
-        elif need_dw or need_db:
-            dyt = fp8_quantize(dy, transpose=True, column_sums=need_db)
-            if need_db:
-                dyt, db = dyt
-            if need_dw:
-                dw = fp8_matmul(fp8_quantize(x, transpose=True), dyt)
+    if _elsewhere(x, dy, w.values if need_dx else None):
+        with torch.cuda.device(x.device):
+            return fp8_linear_backward(x, w, dy, need_dx, need_dw, need_db)
+    if need_dx:
+        dx = fp8_matmul(fp8_quantize(dy), w)
+    if M == 0:
+        dw = torch.zeros((K, N), dtype=torch.float32, device=x.device) if need_dw else None
+        db = torch.zeros((N,), dtype=torch.float32, device=x.device) if need_db else None
+    elif need_dw or need_db:
+        dyt = fp8_quantize(dy, transpose=True, column_sums=need_db)
+        if need_db:
+            dyt, db = dyt
+        if need_dw:
+            dw = fp8_matmul(fp8_quantize(x, transpose=True), dyt)
     return (dx, dw, db) if need_db else (dx, dw)
 
 
@@ -2383,19 +2407,20 @@ def token_logprobs(logits: torch.Tensor, ids: Optional[torch.Tensor] = None, k: 
     k = int(k)
     if not 0 <= k <= min(V, 256):
         raise ValueError(f"k must lie in [0, {min(V, 256)}], got {k}")
-    with _device_of(logits, ids):
-        f = torch.empty((5, N), dtype=torch.float32, device=logits.device)
-        logp, entropy, lse, stats = (f[0] if ids is not None else None), f[1], f[2], f[3:].view(N, 2)
-        top_logp = torch.empty((N, k), dtype=torch.float32, device=logits.device) if k else None
-        top_ids = torch.empty((N, k), dtype=torch.int32, device=logits.device) if k else None
-        if N:
-            need = lib.mh_token_logprobs_workspace_bytes(N, V, k)
-            ws = _scratch(need, logits) if need else None
-            with _timed("token_logprobs", nbytes=N * V * logits.element_size()):
-                check(lib.mh_token_logprobs(_ptr(logits), dt, _ld(logits), N, V, _ptr(ids), idt, k, float(temperature), _ptr(logp),
-                                            _ptr(entropy), _ptr(lse), _ptr(top_logp), _ptr(top_ids), _ptr(stats), _ptr(ws), need, _stream()),
-                      "mh_token_logprobs")
-    return TokenLogProbs(logp, entropy, lse, top_logp, top_ids, stats)
+    if _elsewhere(logits, ids):
+        with torch.cuda.device(logits.device):
+            return token_logprobs(logits, ids, k, temperature)
+    f = torch.empty(5 * N + N * k, dtype=torch.float32, device=logits.device)  # one allocation for all that is float32
+    stats, logp, entropy, lse, top_logp = f.split((2 * N, N, N, N, N * k))
+    top_ids = torch.empty((N, k), dtype=torch.int32, device=logits.device) if k else None
+    if N:
+        need = lib.mh_token_logprobs_workspace_bytes(N, V, k)
+        ws = _scratch(need, logits)
+        with _if_timed("token_logprobs", N * V * logits.element_size()):
+            check(lib.mh_token_logprobs(logits.data_ptr(), dt, _ld(logits), N, V, _at(ids), idt, k, temperature, logp.data_ptr(), entropy.data_ptr(),
+                                        lse.data_ptr(), top_logp.data_ptr(), _at(top_ids), stats.data_ptr(), _at(ws), need, _here()),
+                  "mh_token_logprobs")
+    return TokenLogProbs(None if ids is None else logp, entropy, lse, top_logp.view(N, k) if k else None, top_ids, stats.view(N, 2))
 
 
 def token_logprobs_backward(logits: torch.Tensor, ids: Optional[torch.Tensor], result: TokenLogProbs, dlogp: Optional[torch.Tensor] = None,
@@ -2412,13 +2437,15 @@ def token_logprobs_backward(logits: torch.Tensor, ids: Optional[torch.Tensor], r
     for t, n in ((dlogp, "dlogp"), (dentropy, "dentropy"), (dlse, "dlse"), (result.entropy, "result.entropy")):
         _row_floats(t, (N,), n)
     _row_floats(result.stats, (N, 2), "result.stats")
-    with _device_of(logits, ids, result.stats, dlogp, dentropy, dlse, out):
-        out = _dlogits(logits, out)
-        if N:
-            with _timed("token_logprobs_backward", nbytes=2 * N * V * logits.element_size()):
-                check(lib.mh_token_logprobs_bwd(_ptr(logits), dt, _ld(logits), N, V, _ptr(ids), idt, float(temperature), _ptr(result.stats),
-                                                _ptr(result.entropy), _ptr(dlogp), _ptr(dentropy), _ptr(dlse), _ptr(out), _ld(out), _stream()),
-                      "mh_token_logprobs_bwd")
+    if _elsewhere(logits, ids, result.stats, dlogp, dentropy, dlse, out):
+        with torch.cuda.device(logits.device):
+            return token_logprobs_backward(logits, ids, result, dlogp, dentropy, dlse, temperature, out)
+    out = _dlogits(logits, out)
+    if N:
+        with _if_timed("token_logprobs_backward", 2 * N * V * logits.element_size()):
+            check(lib.mh_token_logprobs_bwd(logits.data_ptr(), dt, _ld(logits), N, V, _at(ids), idt, temperature, result.stats.data_ptr(),
+                                            result.entropy.data_ptr(), _at(dlogp), _at(dentropy), _at(dlse), out.data_ptr(), _ld(out), _here()),
+                  "mh_token_logprobs_bwd")
     return out
 
 
@@ -2458,17 +2485,19 @@ def distill_topk(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logp: 
     if teacher_logp is None:
         raise ValueError("teacher_logp is needed")
     idt, K = _teacher(logits, teacher_ids, teacher_logp)
-    with _device_of(logits, teacher_ids, teacher_logp):
-        loss = torch.empty((N,), dtype=torch.float32, device=logits.device)
-        stats = torch.empty((N, 3), dtype=torch.float32, device=logits.device) if need_grad else None
-        top_grad = torch.empty((N, K), dtype=torch.float32, device=logits.device) if need_grad else None
-        if N:
-            need = lib.mh_distill_topk_workspace_bytes(N, V, int(tail))
-            ws = _scratch(need, logits) if need else None
-            with _timed("distill_topk", nbytes=N * V * logits.element_size()):
-                check(lib.mh_distill_topk(_ptr(logits), dt, _ld(logits), N, V, _ptr(teacher_ids), idt, _ld(teacher_ids),
-                                          _ptr(teacher_logp), _ld(teacher_logp), K, float(temperature), int(tail), _ptr(loss), _ptr(stats),
-                                          _ptr(top_grad), _ptr(ws), need, _stream()), "mh_distill_topk")
+    if _elsewhere(logits, teacher_ids, teacher_logp):
+        with torch.cuda.device(logits.device):
+            return distill_topk(logits, teacher_ids, teacher_logp, temperature, tail, need_grad)
+    loss = torch.empty((N,), dtype=torch.float32, device=logits.device)
+    stats = torch.empty((N, 3), dtype=torch.float32, device=logits.device) if need_grad else None
+    top_grad = torch.empty((N, K), dtype=torch.float32, device=logits.device) if need_grad else None
+    if N:
+        need = lib.mh_distill_topk_workspace_bytes(N, V, int(tail))
+        ws = _scratch(need, logits)
+        with _if_timed("distill_topk", N * V * logits.element_size()):
+            check(lib.mh_distill_topk(logits.data_ptr(), dt, _ld(logits), N, V, teacher_ids.data_ptr(), idt, _ld(teacher_ids), teacher_logp.data_ptr(),
+                                      _ld(teacher_logp), K, temperature, int(tail), loss.data_ptr(), _at(stats), _at(top_grad), _at(ws), need,
+                                      _here()), "mh_distill_topk")
     return DistillResult(loss, stats, top_grad)
 
 
@@ -2484,12 +2513,15 @@ def distill_topk_backward(logits: torch.Tensor, teacher_ids: torch.Tensor, resul
     _row_floats(result.stats, (N, 3), "result.stats")
     _row_floats(result.top_grad, (N, K), "result.top_grad")
     _row_floats(dloss, (N,), "dloss")
-    with _device_of(logits, teacher_ids, result.stats, result.top_grad, dloss, out):
-        out = _dlogits(logits, out)
-        if N:
-            with _timed("distill_topk_backward", nbytes=2 * N * V * logits.element_size()):
-                check(lib.mh_distill_topk_bwd(_ptr(logits), dt, _ld(logits), N, V, _ptr(teacher_ids), idt, _ld(teacher_ids), K,
-                                              float(temperature), _ptr(result.stats), _ptr(result.top_grad), _ptr(dloss), _ptr(out), _ld(out), _stream()), "mh_distill_topk_bwd")
+    if _elsewhere(logits, teacher_ids, result.stats, result.top_grad, dloss, out):
+        with torch.cuda.device(logits.device):
+            return distill_topk_backward(logits, teacher_ids, result, dloss, temperature, out)
+    out = _dlogits(logits, out)
+    if N:
+        with _if_timed("distill_topk_backward", 2 * N * V * logits.element_size()):
+            check(lib.mh_distill_topk_bwd(logits.data_ptr(), dt, _ld(logits), N, V, teacher_ids.data_ptr(), idt, _ld(teacher_ids), K, temperature,
+                                          result.stats.data_ptr(), result.top_grad.data_ptr(), _at(dloss), out.data_ptr(), _ld(out), _here()),
+                  "mh_distill_topk_bwd")
     return out
 
 
