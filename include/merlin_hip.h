@@ -754,6 +754,13 @@ int32_t mh_distill_topk(const void* logits, int32_t dtype, int64_t ld, int64_t N
 int32_t mh_distill_topk_bwd(const void* logits, int32_t dtype, int64_t ld, int64_t N, int64_t V, const void* teacher_ids, int32_t ids_dtype,
                             int64_t ld_ids, int32_t K, float temperature, const float* stats, const float* top_grad, const float* dloss, void* dlogits,
                             int64_t ldd, mh_stream_t stream);
+/* mh_distill_topk_train: mh_distill_topk and _bwd in one call, for row weights dloss that are known before; rows of up to 32768 entries of 16
+ * bits (16384 of 32) are read once, in one launch. */
+int64_t mh_distill_topk_train_workspace_bytes(int64_t N, int64_t V, int32_t K, int32_t dtype, int32_t tail);
+int32_t mh_distill_topk_train(const void* logits, int32_t dtype, int64_t ld, int64_t N, int64_t V, const void* teacher_ids, int32_t ids_dtype,
+                              int64_t ld_ids, const float* teacher_logp, int64_t ld_logp, int32_t K, float temperature, int32_t tail,
+                              const float* dloss, float* loss, void* dlogits, int64_t ldd, void* workspace, int64_t workspace_bytes,
+                              mh_stream_t stream);
 
 /* ---- launch recorder: a train step traced once, replayed without re-entering the host language ----------------------------
  * Replaces the role of Keras' traced `train_function` (BaseModel.fit -> make_train_function, models/base.py:1361-1421): between

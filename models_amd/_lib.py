@@ -125,6 +125,8 @@ SIGNATURES = {
     "mh_distill_topk_workspace_bytes": (_i64, [_i64, _i64, _i32]),
     "mh_distill_topk": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _i32, _i64, _p, _i64, _i32, _f32, _i32, _p, _p, _p, _p, _i64, _p]),
     "mh_distill_topk_bwd": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _i32, _i64, _i32, _f32, _p, _p, _p, _p, _i64, _p]),
+    "mh_distill_topk_train_workspace_bytes": (_i64, [_i64, _i64, _i32, _i32, _i32]),
+    "mh_distill_topk_train": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _i32, _i64, _p, _i64, _i32, _f32, _i32, _p, _p, _p, _i64, _p, _i64, _p]),
     "mh_record_begin": (_i32, []),
     "mh_record_end": (_i32, [C.POINTER(_p)]),
     "mh_record_abort": (_i32, []),

@@ -10,6 +10,8 @@
 // Masked entries (-inf) have p = 0.  A row with nothing left has log p = -inf, entropy 0 and no gradient.  NaN or +inf makes a row's values NaN.
 #include "mh_lowp.h"
 
+#include <type_traits>
+
 namespace {
 
 constexpr float LN2 = 0.693147180559945309f;
@@ -42,10 +44,14 @@ __device__ __forceinline__ Sum sum_join(Sum a, Sum b, float c) {
     sum_to(b, m, c);
     return Sum{m, a.s + b.s, a.u + b.u};
 }
-template <int NT>
-__device__ __forceinline__ Sum sum_block(Sum a, float c, Sum* red) {
+__device__ __forceinline__ Sum sum_wave(Sum a, float c) {
 #pragma unroll
     for (int o = 32; o; o >>= 1) a = sum_join(a, Sum{__shfl_xor(a.m, o), __shfl_xor(a.s, o), __shfl_xor(a.u, o)}, c);
+    return a;
+}
+template <int NT>
+__device__ __forceinline__ Sum sum_block(Sum a, float c, Sum* red) {
+    a = sum_wave(a, c);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
     __syncthreads();
@@ -64,18 +70,6 @@ __device__ __forceinline__ float max_block(float v, float* red) {
     v = red[0];
 #pragma unroll
     for (int w = 1; w < NT / 64; ++w) v = fmaxf(v, red[w]);
-    return v;
-}
-template <int NT>
-__device__ __forceinline__ double add_block(double v, double* red) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = red[0];
-#pragma unroll
-    for (int w = 1; w < NT / 64; ++w) v += red[w];
     return v;
 }
 template <int NT>
@@ -145,6 +139,17 @@ __device__ __forceinline__ void each_entry(const T* x, int n, F f) {
     }
 }
 
+// masks the entries of vector v whose bit is set
+template <int VE>
+__device__ __forceinline__ void mask_values(float (&a)[VE], const uint32_t* bits, int v) {
+    const uint32_t w = VE == 8 ? (bits[v >> 2] >> (8 * (v & 3))) & 255u : (bits[v >> 3] >> (4 * (v & 7))) & 15u;
+    if (w) {
+#pragma unroll
+        for (int i = 0; i < VE; ++i)
+            if (w >> i & 1) a[i] = -INF;
+    }
+}
+
 // The sums over the n entries at x.  `most` receives the thread's own largest entry (NaN left out).  SKIP: entries whose bit is set in `skip` do
 // not count.
 template <int NT, bool ENT, bool SKIP, typename T>
@@ -153,14 +158,6 @@ __device__ __forceinline__ Sum read_sums(const T* x, int n, float c, const uint3
     Run r(c);
     most = -INF;
     const int nv = n / VE;
-    auto masked = [&](float (&a)[VE], int v) {
-        const uint32_t w = VE == 8 ? (skip[v >> 2] >> (8 * (v & 3))) & 255u : (skip[v >> 3] >> (4 * (v & 7))) & 15u;
-        if (w) {
-#pragma unroll
-            for (int i = 0; i < VE; ++i)
-                if (w >> i & 1) a[i] = -INF;
-        }
-    };
     int v = threadIdx.x;
     for (; v + (U - 1) * NT < nv; v += U * NT) {
         uint4 w[U];
@@ -171,7 +168,7 @@ __device__ __forceinline__ Sum read_sums(const T* x, int n, float c, const uint3
         for (int j = 0; j < U; ++j) {
             float b[VE];
             lp_unpack(w[j], b, x);
-            if (SKIP) masked(b, v + j * NT);
+            if (SKIP) mask_values(b, skip, v + j * NT);
 #pragma unroll
             for (int i = 0; i < VE; ++i) a[j * VE + i] = b[i];
         }
@@ -182,7 +179,7 @@ __device__ __forceinline__ Sum read_sums(const T* x, int n, float c, const uint3
     for (; v < nv; v += NT) {
         float a[VE];
         lp_unpack(lp_load16(x + (int64_t)v * VE), a, x);
-        if (SKIP) masked(a, v);
+        if (SKIP) mask_values(a, skip, v);
         const float b = most_of(a);
         most = fmaxf(most, b);
         r.template take<ENT>(a, b, c);
@@ -565,94 +562,176 @@ struct DsArgs {
     float4* part;
 };
 
-template <int NT>
+// One wavefront does a row's entries, E of them a lane (entry lane + 64 i), by shuffles alone.
+constexpr int SEEN = 2 * TOP_MOST;
 struct DsLds {
-    double red[NT / 64], q[TOP_MOST];
-    float fred[NT / 64];
-    int id[TOP_MOST];
+    double q[TOP_MOST];
+    int id[TOP_MOST], seen[SEEN];
 };
+template <int E>
+struct DsTeacher {
+    int id[E];         // -1: none
+    bool first[E];     // no entry before has the same id
+    float l[E];        // the student's logit
+    double q[E], lq[E];  // the teacher's mass, and its logarithm
+    double of_id[E];   // all entries' mass on this id
+    double Q;          // the entries' mass
+    bool any;          // the row has a teacher
+};
+__device__ __forceinline__ float max_wave(float v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    return v;
+}
+__device__ __forceinline__ double add_wave(double v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+// LDS written before is read after, by the same wavefront
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
 
-// t: the sums over the row (tail: over the row without the teacher's entries).  Returns the row's weight, with t what it belongs to.
-template <int NT, typename T>
-__device__ __forceinline__ float ds_finish(const DsArgs& g, int64_t row, Sum& t, DsLds<NT>& s, float* my_grad) {
-    static_assert(NT >= TOP_MOST, "a thread for each entry");
-    const int j = threadIdx.x;
-    int id = -1;
-    float l = -INF, tl = -INF;
-    if (j < g.K) {
-        const int64_t v = id_at(g.ids, g.ids_dtype, row * g.ld_ids + j);
-        if (v >= 0 && v < g.V) {
-            id = (int)v;
-            tl = g.tlp[row * g.ld_tlp + j];
-            l = lp_float(static_cast<const T*>(g.x)[row * g.ld + id]);
+template <int E, typename T>
+__device__ __forceinline__ void ds_teacher(const DsArgs& g, int64_t row, DsLds& s, DsTeacher<E>& e) {
+    const int lane = threadIdx.x & 63;
+    float tl[E], tm = -INF;
+    bool some = false;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const int j = lane + 64 * i;
+        e.id[i] = -1, tl[i] = -INF;
+        if (j < g.K) {
+            const int64_t v = id_at(g.ids, g.ids_dtype, row * g.ld_ids + j);
+            if (v >= 0 && v < g.V) e.id[i] = (int)v, tl[i] = g.tlp[row * g.ld_tlp + j];
         }
-        s.id[j] = id;
     }
-    const bool ok = id >= 0;
-    const float tm = max_block<NT>(tl, s.fred);  // its barriers publish s.id
-    bool first = ok;
-    for (int i = 0; i < j && first; ++i)
-        if (i < g.K && s.id[i] == id) first = false;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        e.l[i] = e.id[i] >= 0 ? lp_float(static_cast<const T*>(g.x)[row * g.ld + e.id[i]]) : -INF;
+        tm = fmaxf(tm, tl[i]);
+        some |= e.id[i] >= 0 && (g.tail || !(tl[i] == -INF));  // NaN counts: it has to show
+    }
+    e.any = __any(some);
+    tm = g.tail ? 0.f : max_wave(tm);
+    e.Q = 0.0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        e.lq[i] = e.any ? (double)tl[i] - tm : 0.0;
+        e.q[i] = e.id[i] >= 0 && e.any ? exp(e.lq[i]) : 0.0;
+        e.Q += e.q[i];
+    }
+    e.Q = add_wave(e.Q);
+    if (!g.tail && e.any) {
+        const double lQ = log(e.Q);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            e.q[i] /= e.Q;
+            e.lq[i] -= lQ;
+        }
+        e.Q = 1.0;
+    }
+    // Does the row give an id twice?  A table of twice as many places as entries tells; only then are the entries compared with each other.
+    for (int i = lane; i < SEEN; i += 64) s.seen[i] = -1;
+    wave_fence();
+    bool twice = false;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        e.first[i] = e.id[i] >= 0;
+        e.of_id[i] = e.q[i];
+        if (e.id[i] >= 0) {
+            uint32_t h = ((uint32_t)e.id[i] * 2654435761u) / (0x80000000u / (SEEN / 2));
+            for (int was; (was = atomicCAS(&s.seen[h], -1, e.id[i])) != -1; h = (h + 1) & (SEEN - 1))
+                if (was == e.id[i]) {
+                    twice = true;
+                    break;
+                }
+        }
+    }
+    if (__any(twice)) {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (lane + 64 * i < g.K) s.id[lane + 64 * i] = e.id[i], s.q[lane + 64 * i] = e.q[i];
+        wave_fence();
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            if (e.id[i] < 0) continue;
+            e.of_id[i] = 0.0;
+            for (int j = 0; j < g.K; ++j)
+                if (s.id[j] == e.id[i]) {
+                    e.of_id[i] += s.q[j];
+                    if (j < lane + 64 * i) e.first[i] = false;
+                }
+        }
+    }
+}
+
+// The row's loss, the entries' gradients and the weight of the other columns, from t: the sums over the row (tail: over the row without the
+// teacher's entries).
+template <int E>
+__device__ __forceinline__ float ds_loss(const DsArgs& g, const Sum& t, const DsTeacher<E>& e, float& loss, float (&grad)[E]) {
     float m = t.m;
     double sum = t.s;
     if (g.tail) {
-        m = fmaxf(m, max_block<NT>(l, s.fred));
-        const double e = first && l > -INF ? exp((double)(l - m) * g.inv_t) : first && l != l ? (double)l : 0.0;
-        sum = add_block<NT>(e, s.red) + (t.m == -INF ? 0.0 : (double)t.s * exp((double)(t.m - m) * g.inv_t));
+        float lm = -INF;
+#pragma unroll
+        for (int i = 0; i < E; ++i) lm = fmaxf(lm, e.l[i]);
+        m = fmaxf(m, max_wave(lm));
+        sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (e.first[i] && !(e.l[i] == -INF)) sum += exp((double)(e.l[i] - m) * g.inv_t);
+        sum = add_wave(sum) + (t.m == -INF ? 0.0 : (double)t.s * exp((double)(t.m - m) * g.inv_t));
     }
-    const bool any = __syncthreads_or(ok && (g.tail || !(tl == -INF)));  // the row has a teacher; NaN counts: it has to show
     const double ln_s = log(sum);
-    double q, lq, r = 0.0;
-    if (g.tail) {
-        lq = tl;
-        q = ok ? exp(lq) : 0.0;
-    } else {
-        lq = any ? (double)tl - tm : 0.0;
-        q = ok && any ? exp(lq) : 0.0;
-    }
-    double Q = add_block<NT>(q, s.red);
-    if (!g.tail) {
-        if (any) {
-            q /= Q;
-            lq -= log(Q);
-            Q = 1.0;
-        }
-    } else if (any && t.m > -INF && t.s != 0.f) {
-        r = 1.0 - Q;
-        if (r < 0.0) r = 0.0;
-    }
-    if (j < g.K) s.q[j] = q;
     const bool none = m == -INF;  // the student's row is masked throughout
-    const double lp = none ? -(double)INF : (double)(l - m) * g.inv_t - ln_s;
-    double term = q > 0.0 || q != q ? q * (lq - lp) : 0.0;
-    double loss = add_block<NT>(term, s.red);  // its barriers publish s.q
-    double pr = 1.0;
-    if (g.tail && r > 0.0) {
-        const double lpr = (double)(t.m - m) * g.inv_t + log((double)t.s) - ln_s;
-        pr = exp(lpr);
-        loss += r * (log(r) - lpr);
+    double lp[E], total = 0.0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        lp[i] = none ? -(double)INF : (double)(e.l[i] - m) * g.inv_t - ln_s;
+        if (e.q[i] > 0.0 || e.q[i] != e.q[i]) total += e.q[i] * (e.lq[i] - lp[i]);
     }
-    const bool live = any && !none;
-    if (j == 0) g.loss[row] = any ? (float)loss : 0.f;
-    const double c = Q + r;
-    if (j < g.K && ok) {
-        double mine = 0.0;
-        for (int i = 0; i < g.K; ++i) mine += s.id[i] == id ? s.q[i] : 0.0;
-        *my_grad = live ? (float)(c * exp(lp) - mine) : 0.f;
-    }
+    total = add_wave(total);
+    const bool others = g.tail && !(t.m == -INF) && t.s != 0.f;
+    const double left = others && e.any && e.Q < 1.0 ? 1.0 - e.Q : 0.0, c = e.Q + left;
+    const double lpr = others ? (double)(t.m - m) * g.inv_t + log((double)t.s) - ln_s : 0.0;
+    if (left > 0.0) total += left * (log(left) - lpr);
+    loss = e.any ? (float)total : 0.f;
+    const bool live = e.any && !none;
+#pragma unroll
+    for (int i = 0; i < E; ++i) grad[i] = live && e.id[i] >= 0 ? (float)(c * exp(lp[i]) - e.of_id[i]) : 0.f;
     if (!live) return 0.f;
     if (!g.tail) return 1.f;
-    if (t.m == -INF || t.s == 0.f) return 0.f;  // no column besides the entries
-    return (float)(c * (r > 0.0 ? pr : exp((double)(t.m - m) * g.inv_t + log((double)t.s) - ln_s)) - r);
+    return others ? (float)(c * exp(lpr) - left) : 0.f;
 }
 
-template <int NT, typename T>
-__device__ __forceinline__ void ds_store(const DsArgs& g, int64_t row, Sum t, DsLds<NT>& s) {
-    float grad = 0.f;
-    const float w = ds_finish<NT, T>(g, row, t, s, &grad);
+// A row's parts joined, and its loss: a wavefront a row.
+template <int E, typename T>
+__global__ __launch_bounds__(256) void distill_topk_finish_kernel(const DsArgs g) {
+    __shared__ DsLds lds[4];
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= g.N) return;
+    const float4* part = g.part + row * g.parts;
+    Sum t = {-3.402823466e38f, 0.f, 0.f};
+    for (int i = lane; i < g.parts; i += 64) {
+        const float4 v = part[i];
+        if (v.x != -INF) t = sum_join(t, Sum{v.x, v.y, v.z}, g.c);
+    }
+    DsTeacher<E> e;
+    ds_teacher<E, T>(g, row, lds[threadIdx.x >> 6], e);
+    t = sum_wave(t, g.c);
+    if (t.s == 0.f) t.m = -INF;
+    float loss, grad[E];
+    const float w = ds_loss<E>(g, t, e, loss, grad);
+    if (lane == 0) g.loss[row] = loss;
     if (g.stats) {
-        if (threadIdx.x < g.K) g.top_grad[row * g.K + threadIdx.x] = grad;
-        if (threadIdx.x == 0) {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (lane + 64 * i < g.K) g.top_grad[row * g.K + lane + 64 * i] = grad[i];
+        if (lane == 0) {
             g.stats[3 * row] = t.m;
             g.stats[3 * row + 1] = t.s > 0.f || t.s != t.s ? log2f(t.s) : 0.f;
             g.stats[3 * row + 2] = w;
@@ -672,27 +751,17 @@ __device__ __forceinline__ void ds_bits(const DsArgs& g, int64_t row, int c0, in
     __syncthreads();
 }
 
+// The sums of a row, or a part of one, with a tail without the teacher's entries.
 template <int NT, typename T, bool TAIL>
-__global__ __launch_bounds__(NT) void distill_topk_kernel(const DsArgs g) {
+__global__ __launch_bounds__(NT) void distill_topk_sums_kernel(const DsArgs g) {
     extern __shared__ uint32_t bits[];
     __shared__ Sum red[NT / 64];
-    __shared__ DsLds<NT> lds;
     const int64_t row = blockIdx.x / (uint32_t)g.parts;
     const int part = (int)(blockIdx.x % (uint32_t)g.parts), c0 = part * g.chunk, n = g.V - c0 < g.chunk ? g.V - c0 : g.chunk;
-    const T* x = static_cast<const T*>(g.x) + row * g.ld + c0;
     if (TAIL) ds_bits<NT>(g, row, c0, n, bits);
     float most;
-    const Sum t = read_sums<NT, false, TAIL>(x, n, g.c, bits, most, red);
-    if (g.parts == 1) ds_store<NT, T>(g, row, t, lds);
-    else if (threadIdx.x == 0) g.part[row * g.parts + part] = make_float4(t.m, t.s, t.u, 0.f);
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void distill_topk_join_kernel(const DsArgs g) {
-    __shared__ DsLds<256> lds;
-    __shared__ Sum sums[4];
-    const int64_t row = blockIdx.x;
-    ds_store<256, T>(g, row, join_parts<256>(g.part + row * g.parts, g.parts, g.c, sums), lds);
+    const Sum t = read_sums<NT, false, TAIL>(static_cast<const T*>(g.x) + row * g.ld + c0, n, g.c, bits, most, red);
+    if (threadIdx.x == 0) g.part[row * g.parts + part] = make_float4(t.m, t.s, t.u, 0.f);
 }
 
 template <int NT, typename T>
@@ -708,6 +777,128 @@ __global__ __launch_bounds__(NT) void distill_topk_bwd_kernel(const GradArgs g) 
     for (int j = threadIdx.x; j < g.K; j += NT) {
         const int64_t v = id_at(g.ids, g.ids_dtype, row * g.ld_ids + j);
         if (v >= c0 && v < c0 + n) lp_store(d + (v - c0), f == 0.f ? 0.f : g.top_grad[row * g.K + j] * f);  // an id given twice has one value
+    }
+}
+
+// A row's loss and gradient from one read: the row stays in registers, R 16-byte vectors a thread, between its sums and its gradient.
+__device__ __forceinline__ uint4 all_masked(const float*) { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+__device__ __forceinline__ uint4 all_masked(const lp_bf16*) { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+__device__ __forceinline__ uint4 all_masked(const lp_f16*) { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
+
+// Hides from the compiler that a vector is what it was: it would unpack the whole row beforehand and keep the values of one use for the next, at two to
+// four times the registers.
+__device__ __forceinline__ void forget(uint4& w) { asm volatile("" : "+v"(w.x), "+v"(w.y), "+v"(w.z), "+v"(w.w)); }
+
+// p, the same for all threads, and a thread's offset in bytes: one address register instead of two for every access
+template <typename T>
+__device__ __forceinline__ T* at_offset(T* p, uint32_t bytes) {
+    typedef typename std::conditional<std::is_const<T>::value, const char, char>::type byte;
+    return reinterpret_cast<T*>(reinterpret_cast<byte*>(p) + bytes);
+}
+
+template <int NT, int R, int E, typename T, bool TAIL>
+__global__ __launch_bounds__(NT) void distill_topk_train_kernel(const DsArgs g, const float* __restrict__ dloss, T* __restrict__ dall, int64_t ldd) {
+    constexpr int VE = lp_vec<T>::N;
+    extern __shared__ uint32_t bits[];
+    __shared__ Sum red[NT / 64];
+    __shared__ DsLds lds;
+    __shared__ float weight;
+    const int64_t row = blockIdx.x;
+    const T* x = static_cast<const T*>(g.x) + row * g.ld;
+    T* d = dall + row * ldd;
+    const int nv = g.V / VE, rest = g.V - nv * VE;
+    const float f = (dloss ? dloss[row] : 1.f) * g.inv_t;
+    uint4 w[R];
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+        const int v = threadIdx.x + j * NT;
+        w[j] = v < nv ? lp_load16(at_offset(x + j * NT * VE, threadIdx.x * 16)) : all_masked(x);
+    }
+    const int last = nv * VE + threadIdx.x;  // this thread's entry behind the vectors
+    const float one = threadIdx.x < rest ? lp_float(x[last]) : -INF;
+    if (TAIL) ds_bits<NT>(g, row, 0, g.V, bits);
+    DsTeacher<E> e;
+    if (threadIdx.x < 64) ds_teacher<E, T>(g, row, lds, e);  // the first wavefront, while the others add
+    auto values = [&](int j, float (&a)[VE]) {
+        forget(w[j]);
+        lp_unpack(w[j], a, x);
+        if (TAIL) {
+            const int v = threadIdx.x + j * NT;
+            if (v < nv) mask_values(a, bits, v);
+        }
+    };
+    const bool skip_one = TAIL && threadIdx.x < rest && (bits[last >> 5] >> (last & 31) & 1);
+    Run run(g.c);
+    float most = -INF;
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+        float a[VE];
+        values(j, a);
+        const float b = most_of(a);
+        most = fmaxf(most, b);
+        run.template take<false>(a, b, g.c);
+        asm volatile("" : "+v"(run.s));  // added up here, not behind the barrier that follows: one vector's values live at a time
+    }
+    {
+        const float a[1] = {skip_one ? -INF : one};
+        most = fmaxf(most, a[0]);
+        run.template take<false>(a, a[0], g.c);
+    }
+    const bool beyond = __syncthreads_or(!(run.B < 2.f * FAR));
+    Sum t = sum_block<NT>(run.sum(g.c), g.c, red);
+    if (t.s == 0.f || beyond) {  // as in read_sums
+        t = Sum{max_block<NT>(most, reinterpret_cast<float*>(red)), 0.f, 0.f};
+        if (t.m != -INF) {
+            Sum a = {t.m, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                float l[VE];
+                values(j, l);
+#pragma unroll
+                for (int i = 0; i < VE; ++i) a.s += ex2((l[i] - t.m) * g.c);
+                asm volatile("" : "+v"(a.s));
+            }
+            a.s += ex2(((skip_one ? -INF : one) - t.m) * g.c);
+            t = sum_block<NT>(a, g.c, red);
+        }
+    }
+    float loss, grad[E];
+    if (threadIdx.x < 64) {
+        const float wt = ds_loss<E>(g, t, e, loss, grad);
+        if (threadIdx.x == 0) {
+            g.loss[row] = loss;
+            weight = wt;
+        }
+    }
+    __syncthreads();
+    const float A = weight * f;
+    if (A == 0.f) {
+        zero_row<NT>(d, g.V);
+    } else {
+        const float L = log2f(t.s);
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            const int v = threadIdx.x + j * NT;
+            if (v < nv) {
+                float l[VE], o[VE];
+                forget(w[j]);
+                lp_unpack(w[j], l, x);
+                grad_values<T>(l, o, t.m, g.c, L, A, 0.f, false);
+                lp_store16(at_offset(d + j * NT * VE, threadIdx.x * 16), o);
+            }
+        }
+        if (threadIdx.x < rest) {
+            const float l[1] = {one};
+            float o[1];
+            grad_values<T>(l, o, t.m, g.c, L, A, 0.f, false);
+            lp_store(d + last, o[0]);
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < 64) {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (e.id[i] >= 0) lp_store(d + e.id[i], f == 0.f ? 0.f : grad[i] * f);
     }
 }
 
@@ -748,6 +939,10 @@ int32_t ts_workspace(const char* who, const void* ws, int64_t bytes, int64_t nee
 
 // threads of a row's (or part's) workgroup
 constexpr int64_t SHORT_ROW = 4096;
+// What a workgroup of a gradient reads and writes: workgroups run in order, so short ones keep the chip's accesses in one stretch of memory, and the
+// lines a workgroup wrote are still in L2 when the teacher's entries are put in.  4096 x 131072 in bf16, 128 entries: 424 / 348 / 419 us at 8 / 16 / 32
+// KB, 442 with a workgroup a row.
+constexpr int64_t GRAD_BYTES = 16384;
 
 template <typename T>
 void lp_launch(const LpArgs& g, hipStream_t s) {
@@ -766,17 +961,47 @@ void ds_launch(const DsArgs& g, hipStream_t s) {
     const dim3 grid((unsigned)(g.N * g.parts));
     const size_t lds = g.tail ? (size_t)(g.chunk + 31) / 32 * 4 : 0;
     if (g.chunk <= SHORT_ROW) {
-        if (g.tail) MH_LAUNCH((distill_topk_kernel<256, T, true>), grid, dim3(256), lds, s, g);
-        else MH_LAUNCH((distill_topk_kernel<256, T, false>), grid, dim3(256), lds, s, g);
+        if (g.tail) MH_LAUNCH((distill_topk_sums_kernel<256, T, true>), grid, dim3(256), lds, s, g);
+        else MH_LAUNCH((distill_topk_sums_kernel<256, T, false>), grid, dim3(256), lds, s, g);
     } else {
-        if (g.tail) MH_LAUNCH((distill_topk_kernel<512, T, true>), grid, dim3(512), lds, s, g);
-        else MH_LAUNCH((distill_topk_kernel<512, T, false>), grid, dim3(512), lds, s, g);
+        if (g.tail) MH_LAUNCH((distill_topk_sums_kernel<512, T, true>), grid, dim3(512), lds, s, g);
+        else MH_LAUNCH((distill_topk_sums_kernel<512, T, false>), grid, dim3(512), lds, s, g);
     }
-    if (g.parts > 1) MH_LAUNCH(distill_topk_join_kernel<T>, dim3((unsigned)g.N), dim3(256), 0, s, g);
+    const dim3 rows((unsigned)mh_ceil_div(g.N, 4));
+    if (g.K <= 64) MH_LAUNCH((distill_topk_finish_kernel<1, T>), rows, dim3(256), 0, s, g);
+    else if (g.K <= 128) MH_LAUNCH((distill_topk_finish_kernel<2, T>), rows, dim3(256), 0, s, g);
+    else MH_LAUNCH((distill_topk_finish_kernel<4, T>), rows, dim3(256), 0, s, g);
+}
+// Whether the rows are short enough to stay in registers: the loss and the gradient are one launch then, and one read.
+template <typename T>
+constexpr int64_t ds_train_most() {
+    return 512 * 8 * lp_vec<T>::N;
+}
+template <int E, typename T>
+void ds_train_launch(const DsArgs& g, const float* dloss, T* out, int64_t ldd, hipStream_t s) {
+    constexpr int VE = lp_vec<T>::N;
+    const dim3 grid((unsigned)g.N);
+    const size_t lds = g.tail ? (size_t)(g.V + 31) / 32 * 4 : 0;
+#define DS_TRAIN(NT, R)                                                                                                           \
+    do {                                                                                                                          \
+        if (g.tail) MH_LAUNCH((distill_topk_train_kernel<NT, R, E, T, true>), grid, dim3(NT), lds, s, g, dloss, out, ldd);         \
+        else MH_LAUNCH((distill_topk_train_kernel<NT, R, E, T, false>), grid, dim3(NT), lds, s, g, dloss, out, ldd);               \
+    } while (0)
+    if (g.V <= 256 * 2 * VE) DS_TRAIN(256, 2);
+    else if (g.V <= 512 * 4 * VE) DS_TRAIN(512, 4);
+    else DS_TRAIN(512, 8);
+#undef DS_TRAIN
+}
+template <typename T>
+void ds_train(const DsArgs& g, const float* dloss, void* d, int64_t ldd, hipStream_t s) {
+    T* out = static_cast<T*>(d);
+    if (g.K <= 64) ds_train_launch<1, T>(g, dloss, out, ldd, s);
+    else if (g.K <= 128) ds_train_launch<2, T>(g, dloss, out, ldd, s);
+    else ds_train_launch<4, T>(g, dloss, out, ldd, s);
 }
 template <typename T>
 void grad_launch(GradArgs g, bool distill, hipStream_t s) {
-    plan_parts(g.N, g.V, 1 << 20, 1, g.parts, g.chunk);
+    plan_parts(g.N, g.V, 1 << 20, mh_ceil_div(g.V * (int64_t)sizeof(T), GRAD_BYTES), g.parts, g.chunk);
     const dim3 grid((unsigned)(g.N * g.parts));
     if (distill) MH_LAUNCH((distill_topk_bwd_kernel<512, T>), grid, dim3(512), 0, s, g);
     else MH_LAUNCH((token_logprobs_bwd_kernel<512, T>), grid, dim3(512), 0, s, g);
@@ -842,7 +1067,7 @@ int64_t mh_distill_topk_workspace_bytes(int64_t N, int64_t V, int32_t tail) {
     if (N <= 0 || V <= 0 || V >= (int64_t)1 << 31) return 0;
     int parts, chunk;
     ds_plan(N, V, tail != 0, parts, chunk);
-    return parts == 1 ? 0 : N * parts * 16;
+    return N * parts * 16;
 }
 
 int32_t mh_distill_topk(const void* logits, int32_t dtype, int64_t ld, int64_t N, int64_t V, const void* teacher_ids, int32_t ids_dtype,
@@ -866,6 +1091,43 @@ int32_t mh_distill_topk(const void* logits, int32_t dtype, int64_t ld, int64_t N
     else if (dtype == MH_BF16) ds_launch<lp_bf16>(g, s);
     else ds_launch<lp_f16>(g, s);
     MH_CHECK_LAUNCH("mh_distill_topk");
+    return MH_OK;
+}
+
+int64_t mh_distill_topk_train_workspace_bytes(int64_t N, int64_t V, int32_t K, int32_t dtype, int32_t tail) {
+    if (N <= 0 || V <= 0 || V >= (int64_t)1 << 31 || K < 1 || K > TOP_MOST) return 0;
+    if (V <= (dtype == MH_F32 ? ds_train_most<float>() : ds_train_most<lp_bf16>())) return 0;
+    return mh_distill_topk_workspace_bytes(N, V, tail) + N * (3 + (int64_t)K) * 4;
+}
+
+int32_t mh_distill_topk_train(const void* logits, int32_t dtype, int64_t ld, int64_t N, int64_t V, const void* teacher_ids, int32_t ids_dtype, int64_t ld_ids,
+                              const float* teacher_logp, int64_t ld_logp, int32_t K, float temperature, int32_t tail, const float* dloss, float* loss,
+                              void* dlogits, int64_t ldd, void* workspace, int64_t workspace_bytes, mh_stream_t stream) {
+    if (int32_t rc = ts_check("mh_distill_topk_train", logits, dtype, ld, N, V, ids_dtype, temperature)) return rc;
+    MH_REQUIRE(K >= 1 && K <= TOP_MOST, "mh_distill_topk_train: %d teacher entries a row (1 to %d)", (int)K, TOP_MOST);
+    if (N == 0) return MH_OK;
+    MH_REQUIRE(teacher_ids && teacher_logp && loss && dlogits && ld_ids >= K && ld_logp >= K && ldd >= V,
+               "mh_distill_topk_train: an argument is NULL, or rows are too short");
+    const int64_t need = mh_distill_topk_train_workspace_bytes(N, V, K, dtype, tail);
+    if (int32_t rc = ts_workspace("mh_distill_topk_train", workspace, workspace_bytes, need)) return rc;
+    if (need) {
+        char* ws = static_cast<char*>(workspace);
+        const int64_t parts = mh_distill_topk_workspace_bytes(N, V, tail);
+        float *stats = reinterpret_cast<float*>(ws + parts), *top_grad = stats + 3 * N;
+        if (int32_t rc = mh_distill_topk(logits, dtype, ld, N, V, teacher_ids, ids_dtype, ld_ids, teacher_logp, ld_logp, K, temperature, tail, loss, stats,
+                                         top_grad, ws, parts, stream))
+            return rc;
+        return mh_distill_topk_bwd(logits, dtype, ld, N, V, teacher_ids, ids_dtype, ld_ids, K, temperature, stats, top_grad, dloss, dlogits, ldd, stream);
+    }
+    DsArgs g = {};
+    g.x = logits, g.ld = ld, g.N = N, g.V = (int)V, g.K = K, g.tail = tail != 0, g.ids = teacher_ids, g.ids_dtype = ids_dtype, g.ld_ids = ld_ids;
+    g.tlp = teacher_logp, g.ld_tlp = ld_logp, g.inv_t = 1.f / temperature, g.c = (float)(1.4426950408889634074 / (double)temperature);
+    g.loss = loss;
+    hipStream_t s = mh_stream(stream);
+    if (dtype == MH_F32) ds_train<float>(g, dloss, dlogits, ldd, s);
+    else if (dtype == MH_BF16) ds_train<lp_bf16>(g, dloss, dlogits, ldd, s);
+    else ds_train<lp_f16>(g, dloss, dlogits, ldd, s);
+    MH_CHECK_LAUNCH("mh_distill_topk_train");
     return MH_OK;
 }
 

@@ -2388,7 +2388,7 @@ def _catalogue(logits: torch.Tensor, temperature: float):
 def _dlogits(logits: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
     """The gradient's buffer: ``out`` (``logits`` itself is allowed), or a new contiguous one."""
     if out is None:
-        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        return torch.empty_like(logits, memory_format=torch.contiguous_format)
     _float_2d(out, "out")
     if out.shape != logits.shape or out.dtype != logits.dtype:
         raise ValueError(f"out must be {list(logits.shape)} of {logits.dtype}, got {list(out.shape)} of {out.dtype}")
@@ -2411,7 +2411,7 @@ def token_logprobs(logits: torch.Tensor, ids: Optional[torch.Tensor] = None, k: 
         with torch.cuda.device(logits.device):
             return token_logprobs(logits, ids, k, temperature)
     f = torch.empty(5 * N + N * k, dtype=torch.float32, device=logits.device)  # one allocation for all that is float32
-    stats, logp, entropy, lse, top_logp = f.split((2 * N, N, N, N, N * k))
+    stats, logp, entropy, lse, top_logp = torch.split_with_sizes(f, (2 * N, N, N, N, N * k))
     top_ids = torch.empty((N, k), dtype=torch.int32, device=logits.device) if k else None
     if N:
         need = lib.mh_token_logprobs_workspace_bytes(N, V, k)
@@ -2464,13 +2464,13 @@ def _teacher(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logp: Opti
     idt = _ids_dtype(teacher_ids, "teacher_ids")
     if teacher_logp is not None:
         _dev(teacher_logp, "teacher_logp", torch.float32)
-    for t, n in ((teacher_ids, "teacher_ids"), (teacher_logp, "teacher_logp")):
-        if t is None:
-            continue
-        if t.dim() != 2 or t.shape[0] != N or not 1 <= t.shape[1] <= 256 or t.shape[1] != teacher_ids.shape[1]:
-            raise ValueError(f"{n} must be [{N}, K] with 1 to 256 entries a row, got {list(t.shape)}")
-        if (t.shape[1] > 1 and t.stride(1) != 1) or (N > 1 and t.stride(0) < t.shape[1]):
-            raise ValueError(f"{n} must have contiguous rows that do not overlap, got strides {t.stride()}")
+    if teacher_ids.dim() != 2 or teacher_ids.shape[0] != N or not 1 <= teacher_ids.shape[1] <= 256:
+        raise ValueError(f"teacher_ids must be [{N}, K] with 1 to 256 entries a row, got {list(teacher_ids.shape)}")
+    if teacher_logp is not None and teacher_logp.shape != teacher_ids.shape:
+        raise ValueError(f"teacher_logp must be {list(teacher_ids.shape)}, as teacher_ids, got {list(teacher_logp.shape)}")
+    for t in (teacher_ids, teacher_logp):
+        if t is not None and not t.is_contiguous() and ((t.shape[1] > 1 and t.stride(1) != 1) or (N > 1 and t.stride(0) < t.shape[1])):
+            raise ValueError(f"a teacher's entries must have contiguous rows that do not overlap, got strides {t.stride()}")
     return idt, teacher_ids.shape[1]
 
 
@@ -2527,6 +2527,25 @@ def distill_topk_backward(logits: torch.Tensor, teacher_ids: torch.Tensor, resul
 
 def distill_topk_train(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logp: torch.Tensor, dloss: Optional[torch.Tensor] = None,
                        temperature: float = 1.0, tail: bool = False, out: Optional[torch.Tensor] = None) -> Tuple[DistillResult, torch.Tensor]:
-    """A training step's ``(distill_topk(...), distill_topk_backward(..., dloss))`` where the row weights ``dloss`` [N] are known beforehand."""
-    result = distill_topk(logits, teacher_ids, teacher_logp, temperature, tail)
-    return result, distill_topk_backward(logits, teacher_ids, result, dloss, temperature, out)
+    """A training step's loss and gradient where the row weights ``dloss`` [N] (None: ones) are known beforehand: ``distill_topk`` and
+    ``distill_topk_backward`` in one call, which is one launch and one read for rows of up to 32768 entries of 16 bits (16384 of 32).  The
+    result holds the loss alone.  ``out`` may be ``logits`` itself."""
+    lib = _lib.load()
+    dt, N, V = _catalogue(logits, temperature)
+    if teacher_logp is None:
+        raise ValueError("teacher_logp is needed")
+    idt, K = _teacher(logits, teacher_ids, teacher_logp)
+    _row_floats(dloss, (N,), "dloss")
+    if _elsewhere(logits, teacher_ids, teacher_logp, dloss, out):
+        with torch.cuda.device(logits.device):
+            return distill_topk_train(logits, teacher_ids, teacher_logp, dloss, temperature, tail, out)
+    out = _dlogits(logits, out)
+    loss = torch.empty((N,), dtype=torch.float32, device=logits.device)
+    if N:
+        need = lib.mh_distill_topk_train_workspace_bytes(N, V, K, dt, int(tail))
+        ws = _scratch(need, logits)
+        with _if_timed("distill_topk_train", 2 * N * V * logits.element_size()):
+            check(lib.mh_distill_topk_train(logits.data_ptr(), dt, _ld(logits), N, V, teacher_ids.data_ptr(), idt, _ld(teacher_ids),
+                                            teacher_logp.data_ptr(), _ld(teacher_logp), K, temperature, int(tail), _at(dloss), loss.data_ptr(),
+                                            out.data_ptr(), _ld(out), _at(ws), need, _here()), "mh_distill_topk_train")
+    return DistillResult(loss, None, None), out

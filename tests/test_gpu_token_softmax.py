@@ -296,7 +296,8 @@ def check_distill(x, ids, tlp, T, tail, rng):
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("tail", [False, True])
 @pytest.mark.parametrize("N,V,K,T,pad,off", [(1, 1, 1, 1.0, 0, 0), (3, 4, 4, 2.0, 0, 1), (5, 63, 7, 1.0, 3, 0), (9, 1009, 256, 0.5, 0, 0), (4, 4100, 33, 1.0, 7, 5),
-                                             (1030, 600, 5, 1.0, 0, 0), (2, 70001, 128, 1.0, 0, 0), (3, 300007, 64, 3.0, 1, 0), (1040, 8300, 16, 1.0, 0, 0)])
+                                             (1030, 600, 5, 1.0, 0, 0), (2, 70001, 128, 1.0, 0, 0), (3, 300007, 64, 3.0, 1, 0), (1040, 8300, 16, 1.0, 0, 0),
+                                             (2, 4096, 9, 1.0, 0, 0), (2, 16385, 64, 1.0, 0, 3), (66, 65543, 40, 1.0, 3, 0), (65, 131072, 128, 2.0, 0, 0)])
 def test_distill(device, dtype, tail, N, V, K, T, pad, off):
     rng = np.random.default_rng(N + V + K)
     x = make(rng, N, V, dtype, device, pad, off, masked=0.0)

@@ -52,7 +52,7 @@ def test_workspaces():
     for kw in (dict(nws=need - 1), dict(ws=None), dict(ws=A + 8)):
         assert call("mh_token_logprobs", LP, LP, **dict(dict(V=100000, ld=100000, nws=need), **kw)) == -4
     need = lib.mh_distill_topk_workspace_bytes(2, 100000, 1)
-    assert need > 0 and lib.mh_distill_topk_workspace_bytes(5000, 100000, 1) == 0 and lib.mh_distill_topk_workspace_bytes(5000, 1000000, 1) > 0
+    assert need > 0 and lib.mh_distill_topk_workspace_bytes(5000, 100000, 1) == 5000 * 16 < lib.mh_distill_topk_workspace_bytes(5000, 1000000, 1)
     for kw in (dict(nws=need - 1), dict(ws=None), dict(ws=A + 8)):
         assert call("mh_distill_topk", DS, DS, **dict(dict(V=100000, ld=100000, nws=need), **kw)) == -4
 
@@ -68,3 +68,21 @@ def test_host_tensors_are_refused():
         ops.token_logprobs(x)
     with pytest.raises(_lib.MerlinHipError):
         ops.distill_topk(x, torch.zeros(2, 1, dtype=torch.int64), torch.zeros(2, 1))
+
+
+DST = dict(x=A, dt=0, ld=1000, N=2, V=1000, ids=A, idt=1, ldi=5, tlp=A, ldt=5, K=5, T=1.0, tail=1, w=A, loss=A, d=A, ldd=1000, ws=A, nws=1 << 20, stream=0)
+
+
+@pytest.mark.parametrize("kw", COMMON[:-1] + [dict(K=0), dict(K=257), dict(ids=None), dict(tlp=None), dict(loss=None), dict(d=None), dict(ldi=4), dict(ldt=4), dict(ldd=999)])
+def test_distill_train_refuses(kw):
+    assert call("mh_distill_topk_train", DST, DST, **kw) == -1
+
+
+def test_distill_train_workspace():
+    lib = _lib.load()
+    assert lib.mh_distill_topk_train_workspace_bytes(4096, 32768, 128, 1, 1) == 0 == lib.mh_distill_topk_train_workspace_bytes(16, 1009, 5, 0, 0)
+    need = lib.mh_distill_topk_train_workspace_bytes(2, 200000, 5, 0, 1)
+    assert need > 0
+    for kw in (dict(nws=need - 1), dict(ws=None), dict(ws=A + 8)):
+        assert call("mh_distill_topk_train", DST, DST, **dict(dict(V=200000, ld=200000, ldd=200000, nws=need), **kw)) == -4
+    assert call("mh_distill_topk_train", DST, DST, N=0, x=None) == 0
