@@ -44,46 +44,83 @@ __device__ __forceinline__ Sum sum_join(Sum a, Sum b, float c) {
     sum_to(b, m, c);
     return Sum{m, a.s + b.s, a.u + b.u};
 }
-__device__ __forceinline__ Sum sum_wave(Sum a, float c) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) a = sum_join(a, Sum{__shfl_xor(a.m, o), __shfl_xor(a.s, o), __shfl_xor(a.u, o)}, c);
-    return a;
+// Reductions over a wavefront by data-parallel moves (a few cycles each, where a shuffle goes through LDS): within rows of 16 lanes, row 0 into 1 and 2
+// into 3, rows 0-1 into 3; lane 63 has it.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float moved(float other, float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(other), __float_as_int(v), CTRL, ROWS, 0xf, false));
 }
+__device__ __forceinline__ float of_last(float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63)); }
+__device__ __forceinline__ float max_wave(float v) {
+    v = fmaxf(v, moved<0x111, 0xf>(v, v));
+    v = fmaxf(v, moved<0x112, 0xf>(v, v));
+    v = fmaxf(v, moved<0x114, 0xf>(v, v));
+    v = fmaxf(v, moved<0x118, 0xf>(v, v));
+    v = fmaxf(v, moved<0x142, 0xa>(v, v));
+    v = fmaxf(v, moved<0x143, 0xc>(v, v));
+    return of_last(v);
+}
+__device__ __forceinline__ float add_wave(float v) {
+    v += moved<0x111, 0xf>(0.f, v);
+    v += moved<0x112, 0xf>(0.f, v);
+    v += moved<0x114, 0xf>(0.f, v);
+    v += moved<0x118, 0xf>(0.f, v);
+    v += moved<0x142, 0xa>(0.f, v);
+    v += moved<0x143, 0xc>(0.f, v);
+    return of_last(v);
+}
+__device__ __forceinline__ double add_wave(double v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+__device__ __forceinline__ Sum sum_wave(Sum a, float c) {
+    sum_to(a, max_wave(a.m), c);
+    return Sum{a.m, add_wave(a.s), add_wave(a.u)};
+}
+// Over the first NT threads of a workgroup; every thread of it takes part in the barriers and has the result.
 template <int NT>
 __device__ __forceinline__ Sum sum_block(Sum a, float c, Sum* red) {
     a = sum_wave(a, c);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
+    if ((threadIdx.x & 63) == 0 && threadIdx.x < NT) red[threadIdx.x >> 6] = a;
     __syncthreads();
-    a = red[0];
+    float m = red[0].m;
 #pragma unroll
-    for (int w = 1; w < NT / 64; ++w) a = sum_join(a, red[w], c);
-    return a;
+    for (int w = 1; w < NT / 64; ++w) m = fmaxf(m, red[w].m);
+    Sum t = {m, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) {
+        Sum b = red[w];
+        sum_to(b, m, c);
+        t.s += b.s;
+        t.u += b.u;
+    }
+    return t;
 }
 template <int NT>
 __device__ __forceinline__ float max_block(float v, float* red) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    v = max_wave(v);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0 && threadIdx.x < NT) red[threadIdx.x >> 6] = v;
     __syncthreads();
     v = red[0];
 #pragma unroll
     for (int w = 1; w < NT / 64; ++w) v = fmaxf(v, red[w]);
     return v;
 }
+// the sum over the wavefronts of a number that each knows; two sets of places in turn: one barrier a count
 template <int NT>
-__device__ __forceinline__ int count_block(int mine, int* red, int& phase) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) mine += __shfl_xor(mine, o);
-    int* r = red + (phase ^= 1) * (NT / 64);  // two sets in turn: one barrier a count
-    if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = mine;
+__device__ __forceinline__ int count_block(int of_wave, int* red, int& phase) {
+    int* r = red + (phase ^= 1) * (NT / 64);
+    if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = of_wave;
     __syncthreads();
     int n = 0;
 #pragma unroll
     for (int w = 0; w < NT / 64; ++w) n += r[w];
     return n;
 }
+__device__ __forceinline__ int lanes(bool p) { return __popcll(__ballot(p)); }
 
 // The sums of a thread while it reads: t = l c - B in one fused operation, B the rounded product m c.  What B lacks of m c -- 16 at most below 2^29 --
 // is put right once, at the end, exactly: fma(m, c, -B) is what the rounding took.
@@ -112,6 +149,11 @@ struct Run {
     }
 };
 
+// a vector of -inf
+__device__ __forceinline__ uint4 all_masked(const float*) { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+__device__ __forceinline__ uint4 all_masked(const lp_bf16*) { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+__device__ __forceinline__ uint4 all_masked(const lp_f16*) { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
+
 template <int N>
 __device__ __forceinline__ float most_of(const float (&v)[N]) {
     float a = v[0];
@@ -125,6 +167,7 @@ template <int NT, typename T, typename F>
 __device__ __forceinline__ void each_entry(const T* x, int n, F f) {
     constexpr int VE = lp_vec<T>::N;
     const int nv = n / VE;
+    if (threadIdx.x >= NT) return;
     for (int v = threadIdx.x; v < nv; v += NT) {
         float a[VE];
         lp_unpack(lp_load16(x + (int64_t)v * VE), a, x);
@@ -150,7 +193,7 @@ __device__ __forceinline__ void mask_values(float (&a)[VE], const uint32_t* bits
     }
 }
 
-// The sums over the n entries at x.  `most` receives the thread's own largest entry (NaN left out).  SKIP: entries whose bit is set in `skip` do
+// The sums over the n entries at x, read by the first NT threads.  `most` receives the thread's own largest entry (NaN left out).  SKIP: entries whose bit is set in `skip` do
 // not count.
 template <int NT, bool ENT, bool SKIP, typename T>
 __device__ __forceinline__ Sum read_sums(const T* x, int n, float c, const uint32_t* skip, float& most, Sum* red) {
@@ -158,7 +201,7 @@ __device__ __forceinline__ Sum read_sums(const T* x, int n, float c, const uint3
     Run r(c);
     most = -INF;
     const int nv = n / VE;
-    int v = threadIdx.x;
+    int v = threadIdx.x < NT ? threadIdx.x : nv;
     for (; v + (U - 1) * NT < nv; v += U * NT) {
         uint4 w[U];
 #pragma unroll
@@ -184,7 +227,7 @@ __device__ __forceinline__ Sum read_sums(const T* x, int n, float c, const uint3
         most = fmaxf(most, b);
         r.template take<ENT>(a, b, c);
     }
-    if (threadIdx.x < n - nv * VE) {
+    if (threadIdx.x < n - nv * VE) {  // fewer than a vector: never the extra wavefront
         const int i = nv * VE + threadIdx.x;
         float a[1] = {lp_float(x[i])};
         if (SKIP && (skip[i >> 5] >> (i & 31) & 1)) a[0] = -INF;
@@ -256,7 +299,7 @@ __device__ __forceinline__ void top_entries(const T* x, int n, int first, int k,
     uint32_t low = 0;
     for (int b = 31; b >= 16; --b) {
         const uint32_t next = low | 1u << b;
-        if (count_block<NT>(mine >= next ? 1 : 0, s.red, phase) >= k) low = next;
+        if (count_block<NT>(lanes(mine >= next), s.red, phase) >= k) low = next;
     }
     if (low <= KEY_NONE) low = KEY_NONE + 1;
     if (threadIdx.x == 0) s.n = s.nq = 0;
@@ -268,14 +311,22 @@ __device__ __forceinline__ void top_entries(const T* x, int n, int first, int k,
         const int at = atomicAdd(&s.n, 1);
         if (at < CAND) s.cand[at] = key;
     };
-    for (int p = threadIdx.x; p < nq * sweeps; p += NT) {
-        const int v = s.list[p % nq] + p / nq * NT;
-        if (v < nv) {
+    for (int p = threadIdx.x; p < nq * sweeps; p += 4 * NT) {
+        uint4 w[4];
+        int v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int q = p + j * NT;
+            v[j] = q < nq * sweeps ? s.list[q % nq] + q / nq * NT : nv;
+            w[j] = v[j] < nv ? lp_load16(x + (int64_t)v[j] * VE) : all_masked(x);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
             float a[VE];
-            lp_unpack(lp_load16(x + (int64_t)v * VE), a, x);
+            lp_unpack(w[j], a, x);
 #pragma unroll
             for (int i = 0; i < VE; ++i)
-                if (a[i] > -INF && key_of(a[i] + 0.f) >= low) put(key_at(a[i], first + v * VE + i));
+                if (a[i] > -INF && key_of(a[i] + 0.f) >= low) put(key_at(a[i], first + v[j] * VE + i));
         }
     }
     if (threadIdx.x < n - nv * VE) {
@@ -291,6 +342,8 @@ __device__ __forceinline__ void top_entries(const T* x, int n, int first, int k,
 #pragma unroll
                 for (int i = 0; i < VE; ++i) c += key_at(l[i], first + at + i) >= next ? 1 : 0;
             });
+#pragma unroll
+            for (int o = 32; o; o >>= 1) c += __shfl_xor(c, o);
             return count_block<NT>(c, s.red, phase);
         });
         if (threadIdx.x == 0) s.n = 0;
@@ -308,7 +361,7 @@ __device__ __forceinline__ void top_entries(const T* x, int n, int first, int k,
     if (have > NT) {
         const uint64_t t = key_threshold(k, NT, [&](uint64_t next) {
             int c = 0;
-            for (int i = threadIdx.x; i < have; i += NT) c += s.cand[i] >= next ? 1 : 0;
+            for (int i = 0; i < CAND; i += NT) c += lanes(i + (int)threadIdx.x < have && s.cand[i + threadIdx.x] >= next);
             return count_block<NT>(c, s.red, phase);
         });
         uint64_t keep[CAND / NT];
@@ -329,6 +382,7 @@ __device__ __forceinline__ void top_entries(const T* x, int n, int first, int k,
     if (threadIdx.x < have) {
         const uint64_t key = s.cand[threadIdx.x];
         int place = 0;
+#pragma unroll 8
         for (int i = 0; i < have; ++i) place += s.cand[i] > key ? 1 : 0;
         if (place < k) emit(place, key);
     }
@@ -358,14 +412,17 @@ __device__ __forceinline__ float lp_value(float l, const Sum& t, float inv_t) {
     return t.m == -INF ? -INF : fmaf(l - t.m, inv_t, -logf(t.s));
 }
 
+// the row's given id's logit, asked for before the row is read
 template <typename T>
-__device__ __forceinline__ void lp_finish(const LpArgs& g, int64_t row, const Sum& t) {
+__device__ __forceinline__ float lp_given(const LpArgs& g, int64_t row, bool& has) {
+    const int64_t id = g.ids ? id_at(g.ids, g.ids_dtype, row) : -1;
+    has = id >= 0 && id < g.V;
+    return has ? lp_float(static_cast<const T*>(g.x)[row * g.ld + id]) : 0.f;
+}
+__device__ __forceinline__ void lp_finish(const LpArgs& g, int64_t row, const Sum& t, bool has, float given) {
     const float ls = log2f(t.s);
     const bool none = t.m == -INF;
-    if (g.ids) {
-        const int64_t id = id_at(g.ids, g.ids_dtype, row);
-        g.logp[row] = id >= 0 && id < g.V ? lp_value(lp_float(static_cast<const T*>(g.x)[row * g.ld + id]), t, g.inv_t) : 0.f;
-    }
+    if (g.ids) g.logp[row] = has ? lp_value(given, t, g.inv_t) : 0.f;
     g.entropy[row] = none ? 0.f : LN2 * (ls - t.u / t.s);
     g.lse[row] = none ? -INF : fmaf(t.m, g.inv_t, logf(t.s));
     g.stats[2 * row] = t.m;
@@ -384,10 +441,12 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(const LpArgs g) {
     const int64_t row = blockIdx.x / (uint32_t)g.parts;
     const int part = (int)(blockIdx.x % (uint32_t)g.parts), c0 = part * g.chunk, n = g.V - c0 < g.chunk ? g.V - c0 : g.chunk;
     const T* x = static_cast<const T*>(g.x) + row * g.ld + c0;
-    float most;
+    float most, given = 0.f;
+    bool has = false;
+    if (threadIdx.x == 0 && g.parts == 1) given = lp_given<T>(g, row, has);
     const Sum t = read_sums<NT, true, false>(x, n, g.c, nullptr, most, red);
     if (threadIdx.x == 0) {
-        if (g.parts == 1) lp_finish<T>(g, row, t);
+        if (g.parts == 1) lp_finish(g, row, t, has, given);
         else g.part[row * g.parts + part] = make_float4(t.m, t.s, t.u, 0.f);
     }
     if constexpr (TOP) {
@@ -417,21 +476,23 @@ __global__ __launch_bounds__(512) void token_logprobs_join_kernel(const LpArgs g
     __shared__ Sum sums[8];
     __shared__ int red[16], have;
     const int64_t row = blockIdx.x;
-    const Sum t = join_parts<512>(g.part + row * g.parts, g.parts, g.c, sums);
-    if (threadIdx.x == 0) lp_finish<T>(g, row, t);
-    if (!g.k) return;
     const int n = g.parts * g.k;
     const uint64_t* in = g.tops + row * n;
     uint64_t key[JOIN_MOST / 512];
 #pragma unroll
     for (int j = 0; j < JOIN_MOST / 512; ++j) key[j] = (int)threadIdx.x + 512 * j < n ? in[threadIdx.x + 512 * j] : 0;
+    bool has = false;
+    const float given = threadIdx.x == 0 ? lp_given<T>(g, row, has) : 0.f;
+    const Sum t = join_parts<512>(g.part + row * g.parts, g.parts, g.c, sums);
+    if (threadIdx.x == 0) lp_finish(g, row, t, has, given);
+    if (!g.k) return;
     int phase = 0;
     uint64_t th = 1;
     if (n > 512)
         th = key_threshold(g.k, 512, [&](uint64_t next) {
             int c = 0;
 #pragma unroll
-            for (int j = 0; j < JOIN_MOST / 512; ++j) c += key[j] >= next ? 1 : 0;
+            for (int j = 0; j < JOIN_MOST / 512; ++j) c += lanes(key[j] >= next);
             return count_block<512>(c, red, phase);
         });
     if (th == 0) th = 1;  // fewer than k keys in all
@@ -444,6 +505,7 @@ __global__ __launch_bounds__(512) void token_logprobs_join_kernel(const LpArgs g
     if (threadIdx.x < have) {
         const uint64_t mine = cand[threadIdx.x];
         int place = 0;
+#pragma unroll 8
         for (int i = 0; i < have; ++i) place += cand[i] > mine ? 1 : 0;
         if (place < g.k) lp_emit(g, row, t, place, mine);
     }
@@ -578,16 +640,6 @@ struct DsTeacher {
     double Q;          // the entries' mass
     bool any;          // the row has a teacher
 };
-__device__ __forceinline__ float max_wave(float v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
-}
-__device__ __forceinline__ double add_wave(double v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
 // LDS written before is read after, by the same wavefront
 __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -656,14 +708,17 @@ __device__ __forceinline__ void ds_teacher(const DsArgs& g, int64_t row, DsLds& 
             if (lane + 64 * i < g.K) s.id[lane + 64 * i] = e.id[i], s.q[lane + 64 * i] = e.q[i];
         wave_fence();
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            if (e.id[i] < 0) continue;
-            e.of_id[i] = 0.0;
-            for (int j = 0; j < g.K; ++j)
-                if (s.id[j] == e.id[i]) {
-                    e.of_id[i] += s.q[j];
-                    if (j < lane + 64 * i) e.first[i] = false;
-                }
+        for (int i = 0; i < E; ++i) e.of_id[i] = 0.0;
+#pragma unroll 4
+        for (int j = 0; j < g.K; ++j) {
+            const int id = s.id[j];
+            const double q = s.q[j];
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const bool same = id == e.id[i];
+                e.of_id[i] += same ? q : 0.0;
+                if (same && j < lane + 64 * i) e.first[i] = false;
+            }
         }
     }
 }
@@ -707,6 +762,24 @@ __device__ __forceinline__ float ds_loss(const DsArgs& g, const Sum& t, const Ds
     return others ? (float)(c * exp(lpr) - left) : 0.f;
 }
 
+template <int E>
+__device__ __forceinline__ void ds_store(const DsArgs& g, int64_t row, const Sum& t, const DsTeacher<E>& e) {
+    const int lane = threadIdx.x & 63;
+    float loss, grad[E];
+    const float w = ds_loss<E>(g, t, e, loss, grad);
+    if (lane == 0) g.loss[row] = loss;
+    if (g.stats) {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (lane + 64 * i < g.K) g.top_grad[row * g.K + lane + 64 * i] = grad[i];
+        if (lane == 0) {
+            g.stats[3 * row] = t.m;
+            g.stats[3 * row + 1] = t.s > 0.f || t.s != t.s ? log2f(t.s) : 0.f;
+            g.stats[3 * row + 2] = w;
+        }
+    }
+}
+
 // A row's parts joined, and its loss: a wavefront a row.
 template <int E, typename T>
 __global__ __launch_bounds__(256) void distill_topk_finish_kernel(const DsArgs g) {
@@ -724,44 +797,41 @@ __global__ __launch_bounds__(256) void distill_topk_finish_kernel(const DsArgs g
     ds_teacher<E, T>(g, row, lds[threadIdx.x >> 6], e);
     t = sum_wave(t, g.c);
     if (t.s == 0.f) t.m = -INF;
-    float loss, grad[E];
-    const float w = ds_loss<E>(g, t, e, loss, grad);
-    if (lane == 0) g.loss[row] = loss;
-    if (g.stats) {
-#pragma unroll
-        for (int i = 0; i < E; ++i)
-            if (lane + 64 * i < g.K) g.top_grad[row * g.K + lane + 64 * i] = grad[i];
-        if (lane == 0) {
-            g.stats[3 * row] = t.m;
-            g.stats[3 * row + 1] = t.s > 0.f || t.s != t.s ? log2f(t.s) : 0.f;
-            g.stats[3 * row + 2] = w;
-        }
-    }
+    ds_store<E>(g, row, t, e);
 }
 
 // bit i of `bits`: column c0 + i is one of the row's teacher entries
-template <int NT>
 __device__ __forceinline__ void ds_bits(const DsArgs& g, int64_t row, int c0, int n, uint32_t* bits) {
-    for (int i = threadIdx.x; i < (n + 31) / 32; i += NT) bits[i] = 0;
+    for (int i = threadIdx.x; i < (n + 31) / 32; i += blockDim.x) bits[i] = 0;
     __syncthreads();
-    for (int j = threadIdx.x; j < g.K; j += NT) {
+    for (int j = threadIdx.x; j < g.K; j += blockDim.x) {
         const int64_t v = id_at(g.ids, g.ids_dtype, row * g.ld_ids + j);
         if (v >= c0 && v < c0 + n) atomicOr(&bits[(v - c0) >> 5], 1u << ((v - c0) & 31));
     }
     __syncthreads();
 }
 
-// The sums of a row, or a part of one, with a tail without the teacher's entries.
-template <int NT, typename T, bool TAIL>
-__global__ __launch_bounds__(NT) void distill_topk_sums_kernel(const DsArgs g) {
+// The sums of a row, or a part of one, with a tail without the teacher's entries.  E != 0: a row a workgroup, which has one wavefront more for the
+// teacher's entries, done while the others read.
+template <int NT, int E, typename T, bool TAIL>
+__global__ __launch_bounds__(NT + (E ? 64 : 0)) void distill_topk_sums_kernel(const DsArgs g) {
     extern __shared__ uint32_t bits[];
     __shared__ Sum red[NT / 64];
-    const int64_t row = blockIdx.x / (uint32_t)g.parts;
-    const int part = (int)(blockIdx.x % (uint32_t)g.parts), c0 = part * g.chunk, n = g.V - c0 < g.chunk ? g.V - c0 : g.chunk;
-    if (TAIL) ds_bits<NT>(g, row, c0, n, bits);
+    const int64_t row = E ? blockIdx.x : blockIdx.x / (uint32_t)g.parts;
+    const int part = E ? 0 : (int)(blockIdx.x % (uint32_t)g.parts), c0 = part * g.chunk, n = g.V - c0 < g.chunk ? g.V - c0 : g.chunk;
+    if (TAIL) ds_bits(g, row, c0, n, bits);
+    const T* x = static_cast<const T*>(g.x) + row * g.ld + c0;
     float most;
-    const Sum t = read_sums<NT, false, TAIL>(static_cast<const T*>(g.x) + row * g.ld + c0, n, g.c, bits, most, red);
-    if (threadIdx.x == 0) g.part[row * g.parts + part] = make_float4(t.m, t.s, t.u, 0.f);
+    if constexpr (E != 0) {
+        __shared__ DsLds lds;
+        DsTeacher<E> e;
+        if (threadIdx.x >= NT) ds_teacher<E, T>(g, row, lds, e);
+        const Sum t = read_sums<NT, false, TAIL>(x, n, g.c, bits, most, red);
+        if (threadIdx.x >= NT) ds_store<E>(g, row, t, e);
+    } else {
+        const Sum t = read_sums<NT, false, TAIL>(x, n, g.c, bits, most, red);
+        if (threadIdx.x == 0) g.part[row * g.parts + part] = make_float4(t.m, t.s, t.u, 0.f);
+    }
 }
 
 template <int NT, typename T>
@@ -781,10 +851,6 @@ __global__ __launch_bounds__(NT) void distill_topk_bwd_kernel(const GradArgs g) 
 }
 
 // A row's loss and gradient from one read: the row stays in registers, R 16-byte vectors a thread, between its sums and its gradient.
-__device__ __forceinline__ uint4 all_masked(const float*) { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
-__device__ __forceinline__ uint4 all_masked(const lp_bf16*) { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
-__device__ __forceinline__ uint4 all_masked(const lp_f16*) { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
-
 // Hides from the compiler that a vector is what it was: it would unpack the whole row beforehand and keep the values of one use for the next, at two to
 // four times the registers.
 __device__ __forceinline__ void forget(uint4& w) { asm volatile("" : "+v"(w.x), "+v"(w.y), "+v"(w.z), "+v"(w.w)); }
@@ -816,7 +882,7 @@ __global__ __launch_bounds__(NT) void distill_topk_train_kernel(const DsArgs g, 
     }
     const int last = nv * VE + threadIdx.x;  // this thread's entry behind the vectors
     const float one = threadIdx.x < rest ? lp_float(x[last]) : -INF;
-    if (TAIL) ds_bits<NT>(g, row, 0, g.V, bits);
+    if (TAIL) ds_bits(g, row, 0, g.V, bits);
     DsTeacher<E> e;
     if (threadIdx.x < 64) ds_teacher<E, T>(g, row, lds, e);  // the first wavefront, while the others add
     auto values = [&](int j, float (&a)[VE]) {
@@ -956,26 +1022,38 @@ void lp_launch(const LpArgs& g, hipStream_t s) {
     }
     if (g.parts > 1) MH_LAUNCH(token_logprobs_join_kernel<T>, dim3((unsigned)g.N), dim3(512), 0, s, g);
 }
-template <typename T>
-void ds_launch(const DsArgs& g, hipStream_t s) {
+template <int E, typename T>
+void ds_launch_sums(const DsArgs& g, hipStream_t s) {
     const dim3 grid((unsigned)(g.N * g.parts));
     const size_t lds = g.tail ? (size_t)(g.chunk + 31) / 32 * 4 : 0;
     if (g.chunk <= SHORT_ROW) {
-        if (g.tail) MH_LAUNCH((distill_topk_sums_kernel<256, T, true>), grid, dim3(256), lds, s, g);
-        else MH_LAUNCH((distill_topk_sums_kernel<256, T, false>), grid, dim3(256), lds, s, g);
+        if (g.tail) MH_LAUNCH((distill_topk_sums_kernel<256, E, T, true>), grid, dim3(256 + (E ? 64 : 0)), lds, s, g);
+        else MH_LAUNCH((distill_topk_sums_kernel<256, E, T, false>), grid, dim3(256 + (E ? 64 : 0)), lds, s, g);
     } else {
-        if (g.tail) MH_LAUNCH((distill_topk_sums_kernel<512, T, true>), grid, dim3(512), lds, s, g);
-        else MH_LAUNCH((distill_topk_sums_kernel<512, T, false>), grid, dim3(512), lds, s, g);
+        if (g.tail) MH_LAUNCH((distill_topk_sums_kernel<512, E, T, true>), grid, dim3(512 + (E ? 64 : 0)), lds, s, g);
+        else MH_LAUNCH((distill_topk_sums_kernel<512, E, T, false>), grid, dim3(512 + (E ? 64 : 0)), lds, s, g);
     }
+}
+template <typename T>
+void ds_launch(const DsArgs& g, hipStream_t s) {
+    if (g.parts == 1) {
+        if (g.K <= 64) ds_launch_sums<1, T>(g, s);
+        else if (g.K <= 128) ds_launch_sums<2, T>(g, s);
+        else ds_launch_sums<4, T>(g, s);
+        return;
+    }
+    ds_launch_sums<0, T>(g, s);
     const dim3 rows((unsigned)mh_ceil_div(g.N, 4));
     if (g.K <= 64) MH_LAUNCH((distill_topk_finish_kernel<1, T>), rows, dim3(256), 0, s, g);
     else if (g.K <= 128) MH_LAUNCH((distill_topk_finish_kernel<2, T>), rows, dim3(256), 0, s, g);
     else MH_LAUNCH((distill_topk_finish_kernel<4, T>), rows, dim3(256), 0, s, g);
 }
-// Whether the rows are short enough to stay in registers: the loss and the gradient are one launch then, and one read.
+// Whether loss and gradient are one launch and one read: the row has to stay in registers, and the one wavefront that does the teacher's entries must
+// not be what the workgroup waits for, unless the rows are few and the launches are what counts.  In bf16, one launch against three: 16 x 1009, 5
+// entries 14 / 20 us; 2048 x 32768, 64 entries 68 / 79; 8192 x 32768, 64 entries 278 / 320; 256 entries: 512 rows 45 / 60, 2048 rows 155 / 123.
 template <typename T>
-constexpr int64_t ds_train_most() {
-    return 512 * 8 * lp_vec<T>::N;
+bool ds_train_once(int64_t N, int64_t V, int K) {
+    return V <= 512 * 8 * lp_vec<T>::N && (K <= 64 || N <= 1024);
 }
 template <int E, typename T>
 void ds_train_launch(const DsArgs& g, const float* dloss, T* out, int64_t ldd, hipStream_t s) {
@@ -1067,7 +1145,7 @@ int64_t mh_distill_topk_workspace_bytes(int64_t N, int64_t V, int32_t tail) {
     if (N <= 0 || V <= 0 || V >= (int64_t)1 << 31) return 0;
     int parts, chunk;
     ds_plan(N, V, tail != 0, parts, chunk);
-    return N * parts * 16;
+    return parts == 1 ? 0 : N * parts * 16;
 }
 
 int32_t mh_distill_topk(const void* logits, int32_t dtype, int64_t ld, int64_t N, int64_t V, const void* teacher_ids, int32_t ids_dtype,
@@ -1096,7 +1174,7 @@ int32_t mh_distill_topk(const void* logits, int32_t dtype, int64_t ld, int64_t N
 
 int64_t mh_distill_topk_train_workspace_bytes(int64_t N, int64_t V, int32_t K, int32_t dtype, int32_t tail) {
     if (N <= 0 || V <= 0 || V >= (int64_t)1 << 31 || K < 1 || K > TOP_MOST) return 0;
-    if (V <= (dtype == MH_F32 ? ds_train_most<float>() : ds_train_most<lp_bf16>())) return 0;
+    if (dtype == MH_F32 ? ds_train_once<float>(N, V, K) : ds_train_once<lp_bf16>(N, V, K)) return 0;
     return mh_distill_topk_workspace_bytes(N, V, tail) + N * (3 + (int64_t)K) * 4;
 }
 
