@@ -202,30 +202,31 @@ __device__ __forceinline__ Sum read_sums(const T* x, int n, float c, const uint3
     most = -INF;
     const int nv = n / VE;
     int v = threadIdx.x < NT ? threadIdx.x : nv;
-    for (; v + (U - 1) * NT < nv; v += U * NT) {
-        uint4 w[U];
-#pragma unroll
-        for (int j = 0; j < U; ++j) w[j] = lp_load16(x + (int64_t)(v + j * NT) * VE);
+    auto batch = [&](const uint4 (&w)[U]) {
         float a[U * VE];
 #pragma unroll
         for (int j = 0; j < U; ++j) {
             float b[VE];
             lp_unpack(w[j], b, x);
-            if (SKIP) mask_values(b, skip, v + j * NT);
+            if (SKIP && v + j * NT < nv) mask_values(b, skip, v + j * NT);
 #pragma unroll
             for (int i = 0; i < VE; ++i) a[j * VE + i] = b[i];
         }
         const float b = most_of(a);
         most = fmaxf(most, b);
         r.template take<ENT>(a, b, c);
+    };
+    for (; v + (U - 1) * NT < nv; v += U * NT) {
+        uint4 w[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) w[j] = lp_load16(x + (int64_t)(v + j * NT) * VE);
+        batch(w);
     }
-    for (; v < nv; v += NT) {
-        float a[VE];
-        lp_unpack(lp_load16(x + (int64_t)v * VE), a, x);
-        if (SKIP) mask_values(a, skip, v);
-        const float b = most_of(a);
-        most = fmaxf(most, b);
-        r.template take<ENT>(a, b, c);
+    if (v < nv) {  // the last vectors together as well
+        uint4 w[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) w[j] = v + j * NT < nv ? lp_load16(x + (int64_t)(v + j * NT) * VE) : all_masked(x);
+        batch(w);
     }
     if (threadIdx.x < n - nv * VE) {  // fewer than a vector: never the extra wavefront
         const int i = nv * VE + threadIdx.x;
@@ -536,24 +537,14 @@ __device__ __forceinline__ void grad_values(const float (&l)[N], float (&o)[N], 
     }
 }
 
+// A vector at a time: what hides the loads here is the number of wavefronts, and more vectors a thread cost more of those than they bring
+// (4096 x 131003 bf16 with entropy: 360 us, 513 with four vectors in flight a thread at 81 registers).
 template <int NT, typename T, bool ENT>
 __device__ __forceinline__ void grad_row(const T* x, T* d, int n, float m, float c, float L, float A, float B) {
-    constexpr int VE = lp_vec<T>::N, U = 4;
+    constexpr int VE = lp_vec<T>::N;
     const int nv = n / VE;
-    int v = threadIdx.x;
-    for (; v + (U - 1) * NT < nv; v += U * NT) {
-        uint4 w[U];
-#pragma unroll
-        for (int j = 0; j < U; ++j) w[j] = lp_load16(x + (int64_t)(v + j * NT) * VE);
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-            float l[VE], o[VE];
-            lp_unpack(w[j], l, x);
-            grad_values<T>(l, o, m, c, L, A, B, ENT);
-            lp_store16(d + (int64_t)(v + j * NT) * VE, o);
-        }
-    }
-    for (; v < nv; v += NT) {
+#pragma unroll 1
+    for (int v = threadIdx.x; v < nv; v += NT) {
         float l[VE], o[VE];
         lp_unpack(lp_load16(x + (int64_t)v * VE), l, x);
         grad_values<T>(l, o, m, c, L, A, B, ENT);
@@ -814,7 +805,7 @@ __device__ __forceinline__ void ds_bits(const DsArgs& g, int64_t row, int c0, in
 // The sums of a row, or a part of one, with a tail without the teacher's entries.  E != 0: a row a workgroup, which has one wavefront more for the
 // teacher's entries, done while the others read.
 template <int NT, int E, typename T, bool TAIL>
-__global__ __launch_bounds__(NT + (E ? 64 : 0)) void distill_topk_sums_kernel(const DsArgs g) {
+__global__ __launch_bounds__(NT + (E ? 64 : 0), E == 1 || E == 2 ? 8 : 1) void distill_topk_sums_kernel(const DsArgs g) {
     extern __shared__ uint32_t bits[];
     __shared__ Sum red[NT / 64];
     const int64_t row = E ? blockIdx.x : blockIdx.x / (uint32_t)g.parts;
@@ -1005,10 +996,11 @@ int32_t ts_workspace(const char* who, const void* ws, int64_t bytes, int64_t nee
 
 // threads of a row's (or part's) workgroup
 constexpr int64_t SHORT_ROW = 4096;
-// What a workgroup of a gradient reads and writes: workgroups run in order, so short ones keep the chip's accesses in one stretch of memory, and the
-// lines a workgroup wrote are still in L2 when the teacher's entries are put in.  4096 x 131072 in bf16, 128 entries: 424 / 348 / 419 us at 8 / 16 / 32
-// KB, 442 with a workgroup a row.
-constexpr int64_t GRAD_BYTES = 16384;
+// What a workgroup of a gradient (512 threads) reads, and writes as much: workgroups start in order, so short ones keep the chip's accesses in one stretch
+// of memory, and the lines a workgroup wrote are still in L2 when the teacher's entries are put in; shorter than two vectors a thread, starting them
+// is what takes the time.  4096 x 131072 in bf16: distillation with 128 entries 399 / 353 / 373 / 404 us at 8 / 16 / 24 / 32 KB (442 with a workgroup
+// a row), log probabilities and entropy 465 / 372 / 355 / 368.
+constexpr int64_t GRAD_BYTES_LOGPROBS = 24576, GRAD_BYTES_DISTILL = 16384;
 
 template <typename T>
 void lp_launch(const LpArgs& g, hipStream_t s) {
@@ -1026,12 +1018,13 @@ template <int E, typename T>
 void ds_launch_sums(const DsArgs& g, hipStream_t s) {
     const dim3 grid((unsigned)(g.N * g.parts));
     const size_t lds = g.tail ? (size_t)(g.chunk + 31) / 32 * 4 : 0;
+    constexpr int NT = E ? 448 : 512;  // eight wavefronts in all: four workgroups fill a compute unit
     if (g.chunk <= SHORT_ROW) {
         if (g.tail) MH_LAUNCH((distill_topk_sums_kernel<256, E, T, true>), grid, dim3(256 + (E ? 64 : 0)), lds, s, g);
         else MH_LAUNCH((distill_topk_sums_kernel<256, E, T, false>), grid, dim3(256 + (E ? 64 : 0)), lds, s, g);
     } else {
-        if (g.tail) MH_LAUNCH((distill_topk_sums_kernel<512, E, T, true>), grid, dim3(512 + (E ? 64 : 0)), lds, s, g);
-        else MH_LAUNCH((distill_topk_sums_kernel<512, E, T, false>), grid, dim3(512 + (E ? 64 : 0)), lds, s, g);
+        if (g.tail) MH_LAUNCH((distill_topk_sums_kernel<NT, E, T, true>), grid, dim3(512), lds, s, g);
+        else MH_LAUNCH((distill_topk_sums_kernel<NT, E, T, false>), grid, dim3(512), lds, s, g);
     }
 }
 template <typename T>
@@ -1079,7 +1072,7 @@ void ds_train(const DsArgs& g, const float* dloss, void* d, int64_t ldd, hipStre
 }
 template <typename T>
 void grad_launch(GradArgs g, bool distill, hipStream_t s) {
-    plan_parts(g.N, g.V, 1 << 20, mh_ceil_div(g.V * (int64_t)sizeof(T), GRAD_BYTES), g.parts, g.chunk);
+    plan_parts(g.N, g.V, 1 << 20, mh_ceil_div(g.V * (int64_t)sizeof(T), distill ? GRAD_BYTES_DISTILL : GRAD_BYTES_LOGPROBS), g.parts, g.chunk);
     const dim3 grid((unsigned)(g.N * g.parts));
     if (distill) MH_LAUNCH((distill_topk_bwd_kernel<512, T>), grid, dim3(512), 0, s, g);
     else MH_LAUNCH((token_logprobs_bwd_kernel<512, T>), grid, dim3(512), 0, s, g);
