@@ -21,6 +21,11 @@ constexpr float LN2 = 0.693147180559945309f;
 constexpr float FAR = 0x1p28f;
 constexpr float INF = __builtin_inff();
 constexpr int TOP_MOST = 256;        // most alternatives, and teacher entries, of a row
+// stretches of a row (or part) whose largest entry LDS holds, in a workgroup of NT threads
+template <int NT>
+constexpr int buckets() {
+    return NT == 256 ? 1024 : 4096;
+}
 constexpr int CAND = 2048;           // candidates of a row (or part of one) that LDS holds
 constexpr int JOIN_MOST = 16 * 512;  // candidates of all parts of a row that the joining kernel holds in registers
 constexpr int TAIL_CHUNK = 1 << 18;  // columns of a part whose membership bits lie in LDS (32 KB)
@@ -193,15 +198,16 @@ __device__ __forceinline__ void mask_values(float (&a)[VE], const uint32_t* bits
     }
 }
 
-// The sums over the n entries at x, read by the first NT threads.  `most` receives the thread's own largest entry (NaN left out).  SKIP: entries whose bit is set in `skip` do
-// not count.
-template <int NT, bool ENT, bool SKIP, typename T>
-__device__ __forceinline__ Sum read_sums(const T* x, int n, float c, const uint32_t* skip, float& most, Sum* red) {
+// The sums over the n entries at x, read by the first NT threads.  SKIP: entries whose bit is set in `skip` do
+// not count.  TOP: bucket[v >> shift] receives the largest entry of each vector (shift = 0) or of eight neighbouring ones, 128 bytes (shift = 3); past
+// the last bucket they start over at the first, and the same threads come by: their number is a multiple of a round's.
+template <int NT, bool ENT, bool SKIP, bool TOP, typename T>
+__device__ __forceinline__ Sum read_sums(const T* x, int n, float c, const uint32_t* skip, float* bucket, int shift, Sum* red) {
     constexpr int VE = lp_vec<T>::N, U = 4;
     Run r(c);
-    most = -INF;
+    float most = -INF;
     const int nv = n / VE;
-    int v = threadIdx.x < NT ? threadIdx.x : nv;
+    int v = threadIdx.x < NT ? threadIdx.x : (nv | 7) + 1;
     auto batch = [&](const uint4 (&w)[U]) {
         float a[U * VE];
 #pragma unroll
@@ -209,6 +215,19 @@ __device__ __forceinline__ Sum read_sums(const T* x, int n, float c, const uint3
             float b[VE];
             lp_unpack(w[j], b, x);
             if (SKIP && v + j * NT < nv) mask_values(b, skip, v + j * NT);
+            if (TOP) {
+                float q = most_of(b);
+                if (shift) {
+                    q = fmaxf(q, moved<0xb1, 0xf>(q, q));   // lanes 1 0 3 2
+                    q = fmaxf(q, moved<0x4e, 0xf>(q, q));   // 2 3 0 1
+                    q = fmaxf(q, moved<0x141, 0xf>(q, q));  // 7 6 .. 0
+                }
+                if (v + j * NT < nv && (!shift || (threadIdx.x & 7) == 0)) {
+                    const int at = (v + j * NT) >> shift;
+                    float* b = bucket + (at & (buckets<NT>() - 1));
+                    *b = at < buckets<NT>() ? q : fmaxf(q, *b);
+                }
+            }
 #pragma unroll
             for (int i = 0; i < VE; ++i) a[j * VE + i] = b[i];
         }
@@ -216,13 +235,14 @@ __device__ __forceinline__ Sum read_sums(const T* x, int n, float c, const uint3
         most = fmaxf(most, b);
         r.template take<ENT>(a, b, c);
     };
-    for (; v + (U - 1) * NT < nv; v += U * NT) {
+    // eight lanes go together, so that one of them can speak for a bucket
+    for (; (v | 7) + (U - 1) * NT < nv; v += U * NT) {
         uint4 w[U];
 #pragma unroll
         for (int j = 0; j < U; ++j) w[j] = lp_load16(x + (int64_t)(v + j * NT) * VE);
         batch(w);
     }
-    if (v < nv) {  // the last vectors together as well
+    if ((v & ~7) < nv) {  // the last vectors, together as well
         uint4 w[U];
 #pragma unroll
         for (int j = 0; j < U; ++j) w[j] = v + j * NT < nv ? lp_load16(x + (int64_t)(v + j * NT) * VE) : all_masked(x);
@@ -285,40 +305,53 @@ __device__ __forceinline__ uint64_t key_threshold(int k, int most, C count) {
 template <int NT>
 struct TopLds {
     uint64_t cand[CAND];
+    union {
+        float most[buckets<NT>()];     // while the row is read
+        uint16_t list[buckets<NT>()];  // the buckets to read again
+    };
     int n, nq, red[2 * (NT / 64)];
-    uint16_t list[NT];
 };
 
-// The k largest keys of the n entries at x, in order, to emit(place, key).  `most` is the thread's own largest entry: the k-th largest of those
-// bounds the row's k-th largest from below, so only the entries of about k threads are read again -- k / NT of the row.
+// The k largest keys of the n entries at x, in order, to emit(place, key).  The k-th largest among largest entries of parts of the row bounds the row's
+// k-th largest from below, so only about k buckets are read again, as whole lines.  (With one bucket a thread, its vectors NT apart, 100 of 512 buckets
+// touched nearly every line of the row: 64 x 1000000, k = 100 took 84 us, 43 without alternatives.)
 template <int NT, typename T, typename E>
-__device__ __forceinline__ void top_entries(const T* x, int n, int first, int k, float most, TopLds<NT>& s, E emit) {
-    constexpr int VE = lp_vec<T>::N;
-    const int nv = n / VE, sweeps = (nv + NT - 1) / NT;
+__device__ __forceinline__ void top_entries(const T* x, int n, int first, int k, int shift, TopLds<NT>& s, E emit) {
+    constexpr int VE = lp_vec<T>::N, B = buckets<NT>(), PER = B / NT;
+    const int nv = n / VE, all = (nv + (1 << shift) - 1) >> shift, nb = all < B ? all : B;
     int phase = 0;
-    const uint32_t mine = key_of(most + 0.f);
-    uint32_t low = 0;
-    for (int b = 31; b >= 16; --b) {
-        const uint32_t next = low | 1u << b;
-        if (count_block<NT>(lanes(mine >= next), s.red, phase) >= k) low = next;
-    }
-    if (low <= KEY_NONE) low = KEY_NONE + 1;
     if (threadIdx.x == 0) s.n = s.nq = 0;
     __syncthreads();
-    if (mine >= low) s.list[atomicAdd(&s.nq, 1)] = (uint16_t)threadIdx.x;
+    uint32_t mine[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) mine[i] = i * NT + (int)threadIdx.x < nb ? key_of(s.most[i * NT + threadIdx.x] + 0.f) : 0;
+    // the k-th largest of the threads' largest, to 16 bits: a little below the buckets' own, and one comparison a round
+    uint32_t largest = 0, low = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) largest = mine[i] > largest ? mine[i] : largest;
+    if (nb >= k)
+        for (int b = 31; b >= 16; --b) {
+            const uint32_t next = low | 1u << b;
+            if (count_block<NT>(lanes(largest >= next), s.red, phase) >= k) low = next;
+        }
+    if (low <= KEY_NONE) low = KEY_NONE + 1;
     __syncthreads();
-    const int nq = s.nq;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+        if (mine[i] >= low) s.list[atomicAdd(&s.nq, 1)] = (uint16_t)(i * NT + threadIdx.x);
+    __syncthreads();
+    const int lap = s.nq << shift, nq = lap * ((all + B - 1) / B);  // vectors to read again: of each round of the buckets
     auto put = [&](uint64_t key) {
         const int at = atomicAdd(&s.n, 1);
         if (at < CAND) s.cand[at] = key;
     };
-    for (int p = threadIdx.x; p < nq * sweeps; p += 4 * NT) {
+    for (int p = threadIdx.x; p < nq; p += 4 * NT) {
         uint4 w[4];
         int v[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int q = p + j * NT;
-            v[j] = q < nq * sweeps ? s.list[q % nq] + q / nq * NT : nv;
+            v[j] = q < nq ? ((q / lap * B + s.list[q % lap >> shift]) << shift) + (q & ((1 << shift) - 1)) : nv;
             w[j] = v[j] < nv ? lp_load16(x + (int64_t)v[j] * VE) : all_masked(x);
         }
 #pragma unroll
@@ -442,16 +475,17 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(const LpArgs g) {
     const int64_t row = blockIdx.x / (uint32_t)g.parts;
     const int part = (int)(blockIdx.x % (uint32_t)g.parts), c0 = part * g.chunk, n = g.V - c0 < g.chunk ? g.V - c0 : g.chunk;
     const T* x = static_cast<const T*>(g.x) + row * g.ld + c0;
-    float most, given = 0.f;
+    float given = 0.f;
     bool has = false;
     if (threadIdx.x == 0 && g.parts == 1) given = lp_given<T>(g, row, has);
-    const Sum t = read_sums<NT, true, false>(x, n, g.c, nullptr, most, red);
+    const int shift = n / lp_vec<T>::N <= buckets<NT>() ? 0 : 3;
+    const Sum t = read_sums<NT, true, false, TOP>(x, n, g.c, nullptr, TOP ? lds.most : nullptr, shift, red);
     if (threadIdx.x == 0) {
         if (g.parts == 1) lp_finish(g, row, t, has, given);
         else g.part[row * g.parts + part] = make_float4(t.m, t.s, t.u, 0.f);
     }
     if constexpr (TOP) {
-        top_entries<NT>(x, n, c0, g.k, most, lds, [&](int place, uint64_t key) {
+        top_entries<NT>(x, n, c0, g.k, shift, lds, [&](int place, uint64_t key) {
             if (g.parts == 1) lp_emit(g, row, t, place, key);
             else g.tops[(row * g.parts + part) * g.k + place] = key;
         });
@@ -812,15 +846,14 @@ __global__ __launch_bounds__(NT + (E ? 64 : 0), E == 1 || E == 2 ? 8 : 1) void d
     const int part = E ? 0 : (int)(blockIdx.x % (uint32_t)g.parts), c0 = part * g.chunk, n = g.V - c0 < g.chunk ? g.V - c0 : g.chunk;
     if (TAIL) ds_bits(g, row, c0, n, bits);
     const T* x = static_cast<const T*>(g.x) + row * g.ld + c0;
-    float most;
     if constexpr (E != 0) {
         __shared__ DsLds lds;
         DsTeacher<E> e;
         if (threadIdx.x >= NT) ds_teacher<E, T>(g, row, lds, e);
-        const Sum t = read_sums<NT, false, TAIL>(x, n, g.c, bits, most, red);
+        const Sum t = read_sums<NT, false, TAIL, false>(x, n, g.c, bits, nullptr, 0, red);
         if (threadIdx.x >= NT) ds_store<E>(g, row, t, e);
     } else {
-        const Sum t = read_sums<NT, false, TAIL>(x, n, g.c, bits, most, red);
+        const Sum t = read_sums<NT, false, TAIL, false>(x, n, g.c, bits, nullptr, 0, red);
         if (threadIdx.x == 0) g.part[row * g.parts + part] = make_float4(t.m, t.s, t.u, 0.f);
     }
 }

@@ -126,7 +126,8 @@ def check_grad(x, ids, r, z, lp, ent, T, g, h, c, inplace=False):
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("N,V,k,T,pad,off", [(1, 1, 1, 1.0, 0, 0), (3, 2, 2, 0.5, 1, 0), (5, 63, 5, 2.0, 0, 1), (4, 500, 256, 1.0, 13, 3), (7, 4096, 1, 0.05, 0, 0),
                                              (2, 4097, 20, 1.0, 0, 0), (1030, 777, 7, 1.0, 0, 0), (6, 8200, 100, 1.3, 5, 7), (1, 70001, 256, 1.0, 0, 0),
-                                             (3, 262147, 33, 0.7, 2, 1), (1100, 9001, 0, 1.0, 0, 0)])
+                                             (3, 262147, 33, 0.7, 2, 1), (1100, 9001, 0, 1.0, 0, 0),
+                                             (1025, 33001, 9, 1.0, 6, 2)])
 def test_logprobs_and_gradient(device, dtype, N, V, k, T, pad, off):
     rng = np.random.default_rng(N + V + k)
     x = make(rng, N, V, dtype, device, pad, off, masked=0.02 if V > 4 else 0.0)
@@ -143,6 +144,32 @@ def test_logprobs_and_gradient(device, dtype, N, V, k, T, pad, off):
     wide = torch.full((N, V + 9), 5.0, dtype=TYPES[dtype], device=device)
     ops.token_logprobs_backward(x, ids, r, g, h, c, temperature=T, out=wide[:, 2:2 + V])
     assert torch.equal(wide[:, 2:2 + V], d) and (wide[:, :2] == 5).all() and (wide[:, 2 + V:] == 5).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("N,V,k", [(1030, 300011, 40), (1030, 66001, 256), (1, 3000017, 256), (2, 5000, 200)])
+def test_alternatives_of_long_rows(device, dtype, N, V, k):
+    """Rows longer than the stretches whose largest entries are kept, large entries placed at the ends of rows and of stretches; against a sort of
+    (value, place) pairs on the device."""
+    g = torch.Generator(device=device).manual_seed(V)
+    x = torch.empty(N, V, dtype=TYPES[dtype], device=device)
+    for n in range(0, N, 64):
+        x[n:n + 64] = torch.randn(min(64, N - n), V, generator=g, device=device).to(x.dtype)
+    for at in (0, 1, 31, 32, 4095 * 8, 32767, V // 2, V - 1, V - 2, V - 9, V - 33):
+        if 0 <= at < V:
+            x[::3, at] = 9.0 + at % 3
+    r = ops.token_logprobs(x, None, k=k)
+    lse = torch.empty(N, device=device, dtype=torch.float64)
+    for n in range(0, N, 64):
+        part = x[n:n + 64]
+        bits = part.float().view(torch.int32).long()
+        key = torch.where(bits < 0, -(bits & 0x7FFFFFFF), bits) * 2 ** 31 + (2 ** 31 - 1 - torch.arange(V, device=device))
+        top = key.topk(k, 1).indices
+        assert torch.equal(r.top_ids[n:n + 64].long(), top)
+        lse[n:n + 64] = torch.logsumexp(part.double(), 1)
+        want = part.gather(1, top).double() - lse[n:n + 64, None]
+        assert ((r.top_logp[n:n + 64].double() - want).abs() <= eps(V) + 2.0 ** -22 * (want.abs() + math.log(V))).all()
+    assert ((r.lse.double() - lse).abs() <= eps(V) + 2.0 ** -22 * (12 + math.log(V))).all()
 
 
 def awkward(dtype, V, rng):
