@@ -145,7 +145,7 @@ struct F8Args {
     int kind;  // MH_F32 / MH_BF16 / MH_F16
     void* out;
     int64_t ldo, slab;  // slab: entries between the slices' partial outputs
-    int vec;            // four entries of an output row can be stored together
+    int vec;            // entries of an output row that can be stored together: 1: four, 2: eight of 16 bits as well, 0: each alone
 };
 
 __device__ __forceinline__ void f8_dma16(const void* g, void* l) {
@@ -185,6 +185,28 @@ __device__ __forceinline__ void f8_store4(const F8Args& g, int64_t m, int64_t n,
             if (g.kind == MH_F32) static_cast<float*>(g.out)[at + i] = v[i];
             else static_cast<uint16_t*>(g.out)[at + i] = (uint16_t)(g.kind == MH_BF16 ? lp_pack_bf16(v[i], 0.f) : lp_pack_f16(v[i], 0.f));
         }
+}
+
+// eight entries of a row in 16 bits
+__device__ __forceinline__ void f8_store8(const F8Args& g, int64_t m, int64_t n, const f32x4& lo, const f32x4& hi, const float (&b)[8], int64_t slab) {
+    const int64_t at = slab + m * g.ldo + n;
+    uint16_t* o = static_cast<uint16_t*>(g.out) + at;
+    const float v[8] = {lo[0] + b[0], lo[1] + b[1], lo[2] + b[2], lo[3] + b[3], hi[0] + b[4], hi[1] + b[5], hi[2] + b[6], hi[3] + b[7]};
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = g.kind == MH_BF16 ? lp_pack_bf16(v[2 * i], v[2 * i + 1]) : lp_pack_f16(v[2 * i], v[2 * i + 1]);
+    if (g.vec > 1 && n + 8 <= g.N) {
+        *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (n + i < g.N) o[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+}
+// LDS written before is read after, by the same wavefront
+__device__ __forceinline__ void f8_wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
 // Tiled product.  WIDE: operands widened to bf16 on the way from LDS, for outputs of fp32 and fp16.  The 8-bit matrix instruction takes its
@@ -333,23 +355,41 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_gemm_kernel(const F8Args 
         body(kb + 3, false);
     }
     for (; kb < kb1; ++kb) body(kb, false);
+    // Output: acc[i][j][4 q + e] = C[m0 + .. + 32 i + l31][n0 + .. + 32 j + 8 q + 4 h + e].  A wavefront turns 32 rows round in LDS and stores whole
+    // stretches of rows (stored from the accumulators, eight or sixteen bytes of 32 rows at a time, 1000 x 50000 x 128 took 62 us).
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last repeated loads
-    // acc[i][j][4 q + e] = C[m0 + .. + l31][n0 + .. + 8 q + 4 h + e]
-    const int64_t slab = (int64_t)blockIdx.y * g.slab;
+    __syncthreads();
+    constexpr int CW = BN / WN, PITCH = CW + 4;
+    static_assert(WM * WN * 32 * PITCH * 4 <= 2 * STAGE, "the turned rows fit the stages");
+    float* const buf = reinterpret_cast<float*>(smem) + wave * 32 * PITCH;
+    const int64_t nw = n0 + wn * CW, mw = m0 + wm * (BM / WM), slab = (int64_t)blockIdx.y * g.slab;
+    const bool wide_out = g.kind == MH_F32;
+    const int per = wide_out ? 4 : 8, lpr = CW / per, c = lane % lpr * per;  // entries a lane stores, lanes a row, this lane's column
+    float bias[8];
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
+    for (int e = 0; e < 8; ++e) bias[e] = g.bias && e < per && nw + c + e < g.N ? g.bias[nw + c + e] : 0.f;
 #pragma unroll
-        for (int qd = 0; qd < 4; ++qd) {
-            const int64_t n = n0 + wn * (BN / WN) + j * 32 + 8 * qd + 4 * h;
-            float b[4];
+    for (int i = 0; i < TM; ++i) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) b[e] = g.bias && n + e < g.N ? g.bias[n + e] : 0.f;
+        for (int j = 0; j < TN; ++j)
 #pragma unroll
-            for (int i = 0; i < TM; ++i) {
-                const int64_t m = m0 + wm * (BM / WM) + i * 32 + l31;
-                if (m < g.M) f8_store4(g, m, n, acc[i][j][4 * qd] + b[0], acc[i][j][4 * qd + 1] + b[1], acc[i][j][4 * qd + 2] + b[2], acc[i][j][4 * qd + 3] + b[3], slab);
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<f32x4*>(buf + l31 * PITCH + j * 32 + 8 * q + 4 * h) =
+                    f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        f8_wave_fence();
+        for (int r = lane / lpr; r < 32; r += 64 / lpr) {
+            const int64_t m = mw + i * 32 + r;
+            if (m >= g.M) break;
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(buf + r * PITCH + c);
+            if (wide_out) {
+                f8_store4(g, m, nw + c, lo[0] + bias[0], lo[1] + bias[1], lo[2] + bias[2], lo[3] + bias[3], slab);
+            } else {
+                const f32x4 hi = *reinterpret_cast<const f32x4*>(buf + r * PITCH + c + 4);
+                f8_store8(g, m, nw + c, lo, hi, bias, slab);
             }
         }
+        f8_wave_fence();
+    }
 }
 
 // 32 entries at x as 8-bit values and their scale's byte: the quantiser's own rule, the four lanes that share a block and a row agreeing on it
@@ -507,7 +547,10 @@ F8Plan f8_plan(int64_t M, int64_t N, int64_t K) {
         p.rows = true;
         return p;
     }
-    p.big = mh_ceil_div(M, 256) * mh_ceil_div(N, 256) >= 256;
+    // Large tiles read less and small ones wait less at their ends: large where the sum is long and the chip has two rounds of them.  Large / small,
+    // fp32 and bf16 outputs: 8192 x 8192 x 8192 868 / 945, 486 / 583 us; 65536 x 512 x 3341 268 / 264, 165 / 179; 16384 x 1024 x 2048 81 / 74,
+    // 58 / 52; 65536 x 256 x 512 46 / 31, 48 / 25.
+    p.big = kb >= 16 && mh_ceil_div(M, 256) * mh_ceil_div(N, 256) >= 512;
     if (!p.big) {
         // too few tiles for the chip: slices of the summed axis, each long enough to be worth its partial output
         const int64_t tiles = mh_ceil_div(M, 128) * mh_ceil_div(N, 128);
@@ -581,7 +624,8 @@ F8Args f8_args(const uint8_t* a, int64_t lda, const uint8_t* as, int64_t ldas, c
     g.kblocks = (int)mh_ceil_div(K, 128);
     g.bias = bias, g.kind = kind, g.out = out, g.ldo = ldo;
     const int64_t es = kind == MH_F32 ? 4 : 2;
-    g.vec = ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) % (4 * es)) == 0;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(out);
+    g.vec = ldo % 4 || at % (4 * es) ? 0 : ldo % 8 || at % (8 * es) ? 1 : 2;
     return g;
 }
 
