@@ -422,15 +422,19 @@ __device__ __forceinline__ i32x8 f8_quantize32(const T* x, int left, uint32_t& s
 }
 struct f8_stored {};  // in place of an element type: a is in its 8-bit form
 
-// Few rows of a (at most 16 MT): bound by reading b once.  A workgroup takes 16 NB rows of b; its wavefronts take the blocks of k in turn, each
-// lane 32 bytes of a row straight into the registers that the 16 x 16 x 128 instruction reads, and the partial sums meet in LDS in a fixed order.
-// X: the type of a where it is quantised on the way (at most 16 rows: the work is done again by every workgroup), or f8_stored.
+// Few rows of a (at most 16 MT): bound by reading b once.  A wavefront takes 16 NB rows of b, each lane 32 bytes of a row straight into the registers
+// that the 16 x 16 x 128 instruction reads; of a workgroup's eight wavefronts WK share the blocks of k and the others have rows of their own.  The
+// next block is asked for while one is multiplied; partial sums meet in LDS in a fixed order and leave as whole stretches of output rows.
+// X: the type of a where it is quantised on the way (at most 16 rows: the work is done again for every 16 NB rows of b), or f8_stored.
+constexpr int RW = 8;  // wavefronts
 template <int MT, int NB, bool WIDE, typename X>
-__global__ __launch_bounds__(512) void fp8_rows_kernel(const F8Args g, const X* __restrict__ x, int64_t ldx, int K) {
-    constexpr bool STORED = std::is_same<X, f8_stored>::value;
-    extern __shared__ __attribute__((aligned(16))) float part[];  // [waves][MT][256]
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, lane = threadIdx.x & 63, l15 = lane & 15, h = lane >> 4;
-    const int64_t n0 = (int64_t)blockIdx.x * (16 * NB);
+__global__ __launch_bounds__(64 * RW, 2) void fp8_rows_kernel(const F8Args g, const X* __restrict__ x, int64_t ldx, int K, int wk) {
+    constexpr bool STORED = std::is_same<X, f8_stored>::value, AHEAD = !(WIDE && MT * NB > 8);
+    constexpr int PITCH = NB * 16 + 4;
+    __shared__ __attribute__((aligned(16))) float part[RW][16 * PITCH];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l15 = lane & 15, h = lane >> 4;
+    const int kw = wave % wk, wn = RW / wk;  // this wavefront's share of k, and the number of row groups
+    const int64_t nblock = (int64_t)blockIdx.x * wn * (16 * NB), n0 = nblock + wave / wk * (16 * NB);
     const uint8_t *pb[NB], *psb[NB], *pa[MT], *psa[MT];
     const X* px[MT];
 #pragma unroll
@@ -454,60 +458,90 @@ __global__ __launch_bounds__(512) void fp8_rows_kernel(const F8Args g, const X* 
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int kb = wave; kb < g.kblocks; kb += waves) {
-        i32x8 vb[NB], va[MT];
+    struct Block {
+        i32x8 b[NB], a[MT];
         uint32_t sb[NB], sa[MT];
+    };
+    auto load = [&](int kb, Block& v) {
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            vb[j] = *reinterpret_cast<const i32x8*>(pb[j] + (int64_t)kb * 128);
-            sb[j] = psb[j][kb];
+            v.b[j] = *reinterpret_cast<const i32x8*>(pb[j] + (int64_t)kb * 128);
+            v.sb[j] = psb[j][kb];
         }
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             if constexpr (STORED) {
-                va[i] = *reinterpret_cast<const i32x8*>(pa[i] + (int64_t)kb * 128);
-                sa[i] = psa[i][kb];
+                v.a[i] = *reinterpret_cast<const i32x8*>(pa[i] + (int64_t)kb * 128);
+                v.sa[i] = psa[i][kb];
             } else {
-                va[i] = f8_quantize32(px[i] + (int64_t)kb * 128, K - kb * 128 - h * 32, sa[i]);
+                v.a[i] = f8_quantize32(px[i] + (int64_t)kb * 128, K - kb * 128 - h * 32, v.sa[i]);
             }
         }
+    };
+    auto multiply = [&](const Block& v) {
         if (!WIDE) {
 #pragma unroll
             for (int j = 0; j < NB; ++j)
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
-                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vb[j], va[i], acc[i][j], 0, 0, 0, (int)sb[j], 0, (int)sa[i]);
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(v.b[j], v.a[i], acc[i][j], 0, 0, 0, (int)v.sb[j], 0, (int)v.sa[i]);
         } else {
             bf16x8 wa[MT][4];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) f8_widen(va[i], __uint_as_float(sa[i] << 23), wa[i]);
+            for (int i = 0; i < MT; ++i) f8_widen(v.a[i], __uint_as_float(v.sa[i] << 23), wa[i]);
 #pragma unroll
             for (int j = 0; j < NB; ++j) {
                 bf16x8 wb[4];
-                f8_widen(vb[j], __uint_as_float(sb[j] << 23), wb);
+                f8_widen(v.b[j], __uint_as_float(v.sb[j] << 23), wb);
 #pragma unroll
                 for (int s = 0; s < 4; ++s)
 #pragma unroll
                     for (int i = 0; i < MT; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[s], wa[i][s], acc[i][j], 0, 0, 0);
             }
         }
+    };
+    if (AHEAD) {
+        Block u, v;
+        if (kw < g.kblocks) load(kw, u);
+        for (int kb = kw; kb < g.kblocks; kb += 2 * wk) {
+            if (kb + wk < g.kblocks) load(kb + wk, v);
+            multiply(u);
+            if (kb + wk < g.kblocks) {
+                if (kb + 2 * wk < g.kblocks) load(kb + 2 * wk, u);
+                multiply(v);
+            }
+        }
+    } else {
+        for (int kb = kw; kb < g.kblocks; kb += wk) {
+            Block u;
+            load(kb, u);
+            multiply(u);
+        }
     }
     // acc[i][j][e] = C[16 i + l15][n0 + 16 j + 4 h + e]
+    const bool wide_out = g.kind == MH_F32;
+    const int per = wide_out ? 4 : 8, lpr = NB * 16 / per;  // entries a thread stores, threads a row
 #pragma unroll
-    for (int j = 0; j < NB; ++j) {
-        if (j) __syncthreads();
+    for (int i = 0; i < MT; ++i) {
+        if (i) __syncthreads();
 #pragma unroll
-        for (int i = 0; i < MT; ++i) *reinterpret_cast<f32x4*>(&part[(wave * MT + i) * 256 + l15 * 16 + h * 4]) = acc[i][j];
+        for (int j = 0; j < NB; ++j) *reinterpret_cast<f32x4*>(&part[wave][l15 * PITCH + j * 16 + h * 4]) = acc[i][j];
         __syncthreads();
-        for (int t = threadIdx.x; t < MT * 64; t += blockDim.x) {
-            f32x4 v = {0.f, 0.f, 0.f, 0.f};
-            for (int w = 0; w < waves; ++w) v += *reinterpret_cast<const f32x4*>(&part[w * MT * 256 + t * 4]);
-            const int64_t m = t / 4, nn = n0 + 16 * j + (t & 3) * 4;
-            if (m >= g.M) continue;
-            if (g.bias)
-                for (int e = 0; e < 4; ++e)
-                    if (nn + e < g.N) v[e] += g.bias[nn + e];
-            f8_store4(g, m, nn, v[0], v[1], v[2], v[3], 0);
+        for (int t = threadIdx.x; t < wn * 16 * lpr; t += 64 * RW) {
+            const int gr = t / (16 * lpr), r = t / lpr % 16, c = t % lpr * per;
+            const int64_t m = 16 * i + r, n = nblock + gr * (16 * NB) + c;
+            if (m >= g.M || n >= g.N) continue;
+            f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+            for (int w = 0; w < wk; ++w) {
+                const float* p = &part[gr * wk + w][r * PITCH + c];
+                lo += *reinterpret_cast<const f32x4*>(p);
+                if (!wide_out) hi += *reinterpret_cast<const f32x4*>(p + 4);
+            }
+            float bias[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) bias[e] = g.bias && e < per && n + e < g.N ? g.bias[n + e] : 0.f;
+            if (wide_out) f8_store4(g, m, n, lo[0] + bias[0], lo[1] + bias[1], lo[2] + bias[2], lo[3] + bias[3], 0);
+            else f8_store8(g, m, n, lo, hi, bias, 0);
         }
     }
 }
@@ -517,14 +551,21 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(const float* __restrict__
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, quads = (g.N + 3) / 4;
     if (i >= g.M * quads) return;
     const int64_t m = i / quads, n = (i % quads) * 4;
-    float v[4];
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    const float* p = part + m * g.N + n;
+    if (g.N % 4 == 0) {
+#pragma unroll 4
+        for (int s = 0; s < slices; ++s) v += *reinterpret_cast<const f32x4*>(p + (int64_t)s * g.slab);
+    } else {
+        for (int s = 0; s < slices; ++s)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        v[e] = 0.f;
-        if (n + e < g.N) {
-            for (int s = 0; s < slices; ++s) v[e] += part[(int64_t)s * g.slab + m * g.N + n + e];
-            if (g.bias) v[e] += g.bias[n + e];
-        }
+            for (int e = 0; e < 4; ++e)
+                if (n + e < g.N) v[e] += p[(int64_t)s * g.slab + e];
+    }
+    if (g.bias) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (n + e < g.N) v[e] += g.bias[n + e];
     }
     f8_store4(g, m, n, v[0], v[1], v[2], v[3], 0);
 }
@@ -552,10 +593,14 @@ F8Plan f8_plan(int64_t M, int64_t N, int64_t K) {
     // 58 / 52; 65536 x 256 x 512 46 / 31, 48 / 25.
     p.big = kb >= 16 && mh_ceil_div(M, 256) * mh_ceil_div(N, 256) >= 512;
     if (!p.big) {
-        // too few tiles for the chip: slices of the summed axis, each long enough to be worth its partial output
+        // Too few tiles for the chip: slices of the summed axis, each long enough to be worth its partial output (eight blocks: 1024^3 in one slice
+        // 14 us, two 17), and not more than the join reads well (128 x 415 x 65536: 64 slices 75 us, 32 50).  A tile for each of the 256 compute
+        // units is enough (2048^3 bf16: 17 us, 28 in two slices); below that two workgroups a unit are better than one (1024 x 2048 x 16384: 58,
+        // 64).
         const int64_t tiles = mh_ceil_div(M, 128) * mh_ceil_div(N, 128);
-        int64_t s = 512 / tiles;
+        int64_t s = tiles >= 256 ? 1 : 512 / tiles;
         if (s > kb / 8) s = kb / 8;
+        if (s > 32) s = 32;
         if (s > 1) {
             p.kb_split = (int)mh_ceil_div(mh_ceil_div(kb, s), 4) * 4;
             p.slices = (int)mh_ceil_div(kb, p.kb_split);
@@ -586,25 +631,27 @@ int32_t f8_launch_tiles(F8Args g, int slices, bool wide, hipStream_t s) {
 }
 
 template <int MT, int NB, typename X>
-void f8_launch_rows_nb(const F8Args& g, const X* x, int64_t ldx, int K, hipStream_t s) {
-    const int waves = g.kblocks >= 8 ? 8 : 4;
-    const dim3 grid((unsigned)mh_ceil_div(g.N, 16 * NB)), block(waves * 64);
-    if (g.kind != MH_BF16) MH_LAUNCH((fp8_rows_kernel<MT, NB, true, X>), grid, block, (size_t)waves * MT * 1024, s, g, x, ldx, K);
-    else MH_LAUNCH((fp8_rows_kernel<MT, NB, false, X>), grid, block, (size_t)waves * MT * 1024, s, g, x, ldx, K);
+void f8_launch_rows_nb(const F8Args& g, const X* x, int64_t ldx, int K, int wk, hipStream_t s) {
+    const dim3 grid((unsigned)mh_ceil_div(g.N, RW / wk * 16 * NB)), block(64 * RW);
+    if (g.kind != MH_BF16) MH_LAUNCH((fp8_rows_kernel<MT, NB, true, X>), grid, block, 0, s, g, x, ldx, K, wk);
+    else MH_LAUNCH((fp8_rows_kernel<MT, NB, false, X>), grid, block, 0, s, g, x, ldx, K, wk);
 }
-template <int MT>
-void f8_launch_rows(const F8Args& g, hipStream_t s) {
-    const f8_stored* none = nullptr;
-    // more rows of b a workgroup: a is read fewer times, as long as the workgroups still fill the chip
-    if (g.N >= 4 * 16 * 192) f8_launch_rows_nb<MT, 4>(g, none, 0, 0, s);
-    else if (g.N >= 2 * 16 * 192) f8_launch_rows_nb<MT, 2>(g, none, 0, 0, s);
-    else f8_launch_rows_nb<MT, 1>(g, none, 0, 0, s);
+template <int MT, typename X>
+void f8_launch_rows(const F8Args& g, const X* x, int64_t ldx, int K, hipStream_t s) {
+    const int wk = g.kblocks >= 8 ? 8 : g.kblocks >= 4 ? 4 : g.kblocks >= 2 ? 2 : 1;
+    // more rows of b a wavefront: a is read, or quantised, fewer times, as long as the workgroups still fill the chip
+    auto groups = [&](int nb) { return mh_ceil_div(g.N, RW / wk * 16 * nb); };
+    if (groups(4) >= 192) f8_launch_rows_nb<MT, 4>(g, x, ldx, K, wk, s);
+    else if (groups(2) >= 192) f8_launch_rows_nb<MT, 2>(g, x, ldx, K, wk, s);
+    else f8_launch_rows_nb<MT, 1>(g, x, ldx, K, wk, s);
 }
 void f8_launch_rows_any(const F8Args& g, hipStream_t s) {
+    const f8_stored* none = nullptr;
     const int mt = (int)mh_ceil_div(g.M, 16);
-    if (mt == 1) f8_launch_rows<1>(g, s);
-    else if (mt == 2) f8_launch_rows<2>(g, s);
-    else f8_launch_rows<4>(g, s);
+    if (mt == 1) f8_launch_rows<1>(g, none, 0, 0, s);
+    else if (mt == 2) f8_launch_rows<2>(g, none, 0, 0, s);
+    else if (mt == 3) f8_launch_rows<3>(g, none, 0, 0, s);
+    else f8_launch_rows<4>(g, none, 0, 0, s);
 }
 
 int32_t f8_check_matrix(const char* who, const char* name, const void* q, int64_t ld, const void* s, int64_t lds, int64_t rows, int64_t K) {
@@ -753,9 +800,9 @@ int32_t mh_fp8_linear(const void* x, int32_t x_dtype, int64_t ldx, const void* w
         const F8Args g = f8_args(nullptr, 0, nullptr, 0, static_cast<const uint8_t*>(w), ldw, static_cast<const uint8_t*>(w_scales), ldws, M, N, K, bias, out_dtype,
                                  out, ldo);
         hipStream_t s = mh_stream(stream);
-        if (x_dtype == MH_F32) f8_launch_rows_nb<1, 1>(g, static_cast<const float*>(x), ldx, (int)K, s);
-        else if (x_dtype == MH_BF16) f8_launch_rows_nb<1, 1>(g, static_cast<const lp_bf16*>(x), ldx, (int)K, s);
-        else f8_launch_rows_nb<1, 1>(g, static_cast<const lp_f16*>(x), ldx, (int)K, s);
+        if (x_dtype == MH_F32) f8_launch_rows<1>(g, static_cast<const float*>(x), ldx, (int)K, s);
+        else if (x_dtype == MH_BF16) f8_launch_rows<1>(g, static_cast<const lp_bf16*>(x), ldx, (int)K, s);
+        else f8_launch_rows<1>(g, static_cast<const lp_f16*>(x), ldx, (int)K, s);
         MH_CHECK_LAUNCH("mh_fp8_linear");
         return MH_OK;
     }
