@@ -392,22 +392,9 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_gemm_kernel(const F8Args 
     }
 }
 
-// 32 entries at x as 8-bit values and their scale's byte: the quantiser's own rule, the four lanes that share a block and a row agreeing on it
-template <typename T>
-__device__ __forceinline__ i32x8 f8_quantize32(const T* x, int left, uint32_t& scale) {
-    float v[32], a = 0.f;
-    if (left >= 32) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float w[8];
-            lp_load8(x + 8 * i, w);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[8 * i + j] = w[j];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = i < left ? lp_float(x[i]) : 0.f;
-    }
+// 32 entries as 8-bit values and their scale's byte: the quantiser's own rule, the four lanes that share a block and a row agreeing on it
+__device__ __forceinline__ i32x8 f8_quantize32(const float (&v)[32], uint32_t& scale) {
+    float a = 0.f;
 #pragma unroll
     for (int i = 0; i < 32; ++i) a = fmaxf(a, q_mag(v[i]));
     a = fmaxf(a, __shfl_xor(a, 16));
@@ -422,27 +409,101 @@ __device__ __forceinline__ i32x8 f8_quantize32(const T* x, int left, uint32_t& s
 }
 struct f8_stored {};  // in place of an element type: a is in its 8-bit form
 
-// Few rows of a (at most 16 MT): bound by reading b once.  A wavefront takes 16 NB rows of b, each lane 32 bytes of a row straight into the registers
-// that the 16 x 16 x 128 instruction reads; of a workgroup's eight wavefronts WK share the blocks of k and the others have rows of their own.  The
-// next block is asked for while one is multiplied; partial sums meet in LDS in a fixed order and leave as whole stretches of output rows.
-// X: the type of a where it is quantised on the way (at most 16 rows: the work is done again for every 16 NB rows of b), or f8_stored.
+// What a lane holds of a row of a for one block of k: its 32 entries in the 8-bit form, or as they come.
+template <typename X>
+struct F8Lane {
+    static constexpr int N = sizeof(X) * 2;  // 16-byte vectors
+    uint4 w[N];
+    __device__ __forceinline__ void load(const X* p, int left) {
+        if (left >= 32) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) w[i] = lp_load16(p + i * lp_vec<X>::N);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                X v[lp_vec<X>::N] = {};
+#pragma unroll
+                for (int j = 0; j < lp_vec<X>::N; ++j)
+                    if (i * lp_vec<X>::N + j < left) v[j] = p[i * lp_vec<X>::N + j];
+                __builtin_memcpy(&w[i], v, 16);
+            }
+        }
+    }
+    __device__ __forceinline__ void arrived() {
+#pragma unroll
+        for (int i = 0; i < N; ++i) asm volatile("" : "+v"(w[i].x), "+v"(w[i].y), "+v"(w[i].z), "+v"(w[i].w));
+    }
+    __device__ __forceinline__ i32x8 values(uint32_t& scale) const {
+        float v[32];
+        const X* type = nullptr;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float u[lp_vec<X>::N];
+            lp_unpack(w[i], u, type);
+#pragma unroll
+            for (int j = 0; j < lp_vec<X>::N; ++j) v[i * lp_vec<X>::N + j] = u[j];
+        }
+        return f8_quantize32(v, scale);
+    }
+};
+template <>
+struct F8Lane<f8_stored> {
+    i32x4 lo, hi;
+    uint32_t s;
+    __device__ __forceinline__ void load(const uint8_t* p, const uint8_t* ps) {
+        lo = *reinterpret_cast<const i32x4*>(p);
+        hi = *reinterpret_cast<const i32x4*>(p + 16);
+        s = *ps;
+    }
+    __device__ __forceinline__ void arrived() { asm volatile("" : "+v"(lo), "+v"(hi), "+v"(s)); }
+    __device__ __forceinline__ i32x8 values(uint32_t& scale) const {
+        scale = s;
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+};
+
+// Few rows of a (at most 16 MT): bound by reading b once.  A wavefront takes 16 NB rows of b for the 16 x 16 x 128 instruction; of a workgroup's eight,
+// WK share the blocks of k and the others have rows of their own.  The instruction wants 16 rows in neighbouring lanes, which as loads would ask the
+// cache for a line 16 bytes at a time (48 x 4096 -> 14341 took 28 us so): b comes by direct-to-LDS loads of whole lines into two stages of the
+// wavefront's own, the next block's while one is multiplied, and no barrier is needed.  Partial sums meet in LDS in a fixed order and leave as
+// whole stretches of output rows.  X: the type of a where it is quantised on the way (at most 16 rows: the work is done again for every 16 NB
+// rows of b), or f8_stored.
 constexpr int RW = 8;  // wavefronts
+template <int NB>
+constexpr int f8_rows_stage() {
+    return NB * 16 * 128;
+}
 template <int MT, int NB, bool WIDE, typename X>
 __global__ __launch_bounds__(64 * RW, 2) void fp8_rows_kernel(const F8Args g, const X* __restrict__ x, int64_t ldx, int K, int wk) {
-    constexpr bool STORED = std::is_same<X, f8_stored>::value, AHEAD = !(WIDE && MT * NB > 8);
-    constexpr int PITCH = NB * 16 + 4;
-    __shared__ __attribute__((aligned(16))) float part[RW][16 * PITCH];
+    constexpr bool STORED = std::is_same<X, f8_stored>::value;
+    constexpr int PITCH = NB * 16 + 4, STAGE = f8_rows_stage<NB>();
+    static_assert(16 * PITCH * 4 <= 2 * STAGE, "a wavefront's partial sums fit its stages");
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l15 = lane & 15, h = lane >> 4;
-    const int kw = wave % wk, wn = RW / wk;  // this wavefront's share of k, and the number of row groups
+    const int wn = RW / wk;  // row groups of the workgroup
     const int64_t nblock = (int64_t)blockIdx.x * wn * (16 * NB), n0 = nblock + wave / wk * (16 * NB);
-    const uint8_t *pb[NB], *psb[NB], *pa[MT], *psa[MT];
-    const X* px[MT];
+    // this wavefront's blocks of k: whole words of scales where there are enough
+    int share = (g.kblocks + wk - 1) / wk;
+    if (share >= 4) share = (share + 3) & ~3;
+    const int kb0 = wave % wk * share, kb1 = kb0 + share < g.kblocks ? kb0 + share : g.kblocks;
+    uint8_t* const stage = smem + wave * 2 * STAGE;
+    const int64_t nf = n0 < g.N ? n0 : g.N - 1;  // a group past the end reads the last row and stores nothing
+    const uint8_t *const tb = g.b + nf * g.ldb, *const tbs = g.bs + nf * g.ldbs;
+    const int last = g.N - nf < 16 * NB ? (int)(g.N - nf) - 1 : 16 * NB - 1;
+    uint32_t src[2 * NB], ssrc[NB];
 #pragma unroll
-    for (int j = 0; j < NB; ++j) {
-        const int64_t n = n0 + 16 * j + l15 < g.N ? n0 + 16 * j + l15 : g.N - 1;
-        pb[j] = g.b + n * g.ldb + h * 32;
-        psb[j] = g.bs + n * g.ldbs;
+    for (int j = 0; j < 2 * NB; ++j) {
+        const int r = 8 * j + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
+        src[j] = (uint32_t)((r < last ? r : last) * g.ldb) + c * 16;
     }
+#pragma unroll
+    for (int j = 0; j < NB; ++j) ssrc[j] = (uint32_t)((16 * j + l15 < last ? 16 * j + l15 : last) * g.ldbs);
+    auto issue = [&](int kb) {
+#pragma unroll
+        for (int j = 0; j < 2 * NB; ++j) f8_dma16(tb + (int64_t)kb * 128 + src[j], stage + (kb & 1) * STAGE + j * 1024);
+    };
+    const uint8_t *pa[MT], *psa[MT];
+    const X* px[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         const int64_t m = 16 * i + l15 < g.M ? 16 * i + l15 : g.M - 1;
@@ -458,74 +519,86 @@ __global__ __launch_bounds__(64 * RW, 2) void fp8_rows_kernel(const F8Args g, co
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    uint32_t sb[NB];
     struct Block {
-        i32x8 b[NB], a[MT];
-        uint32_t sb[NB], sa[MT];
+        F8Lane<X> a[MT];
     };
     auto load = [&](int kb, Block& v) {
 #pragma unroll
-        for (int j = 0; j < NB; ++j) {
-            v.b[j] = *reinterpret_cast<const i32x8*>(pb[j] + (int64_t)kb * 128);
-            v.sb[j] = psb[j][kb];
-        }
-#pragma unroll
         for (int i = 0; i < MT; ++i) {
-            if constexpr (STORED) {
-                v.a[i] = *reinterpret_cast<const i32x8*>(pa[i] + (int64_t)kb * 128);
-                v.sa[i] = psa[i][kb];
-            } else {
-                v.a[i] = f8_quantize32(px[i] + (int64_t)kb * 128, K - kb * 128 - h * 32, v.sa[i]);
-            }
+            if constexpr (STORED) v.a[i].load(pa[i] + (int64_t)kb * 128, psa[i] + kb);
+            else v.a[i].load(px[i] + (int64_t)kb * 128, K - kb * 128 - h * 32);
         }
     };
-    auto multiply = [&](const Block& v) {
-        if (!WIDE) {
+    // Block kb: b's lines were asked for before a's, and loads arrive in order: where a is there, b is.
+    auto multiply = [&](int kb, Block& v) {
+        if (kb == kb0 || (kb & 3) == 0) {
 #pragma unroll
-            for (int j = 0; j < NB; ++j)
+            for (int j = 0; j < NB; ++j) sb[j] = *reinterpret_cast<const uint32_t*>(tbs + (kb & ~3) + ssrc[j]);
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) v.a[i].arrived();
+        asm volatile("" ::: "memory");
+        const uint8_t* st = stage + (kb & 1) * STAGE;
+        const int sw = (l15 >> 1) & 7, sh = (kb & 3) * 8;
+        i32x8 va[MT];
+        uint32_t sa[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) va[i] = v.a[i].values(sa[i]);
+        bf16x8 wa[MT][4];
+        if (WIDE) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) f8_widen(va[i], __uint_as_float(sa[i] << 23), wa[i]);
+        }
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            const i32x4 lo = *reinterpret_cast<const i32x4*>(st + (16 * j + l15) * 128 + (((2 * h) ^ sw) << 4));
+            const i32x4 hi = *reinterpret_cast<const i32x4*>(st + (16 * j + l15) * 128 + (((2 * h + 1) ^ sw) << 4));
+            const i32x8 vb = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            const uint32_t s = sb[j] >> sh;
+            if (!WIDE) {
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
-                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(v.b[j], v.a[i], acc[i][j], 0, 0, 0, (int)v.sb[j], 0, (int)v.sa[i]);
-        } else {
-            bf16x8 wa[MT][4];
-#pragma unroll
-            for (int i = 0; i < MT; ++i) f8_widen(v.a[i], __uint_as_float(v.sa[i] << 23), wa[i]);
-#pragma unroll
-            for (int j = 0; j < NB; ++j) {
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vb, va[i], acc[i][j], 0, 0, 0, (int)s, 0, (int)sa[i]);
+            } else {
                 bf16x8 wb[4];
-                f8_widen(v.b[j], __uint_as_float(v.sb[j] << 23), wb);
+                f8_widen(vb, __uint_as_float((s & 255u) << 23), wb);
 #pragma unroll
-                for (int s = 0; s < 4; ++s)
+                for (int q = 0; q < 4; ++q)
 #pragma unroll
-                    for (int i = 0; i < MT; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[s], wa[i][s], acc[i][j], 0, 0, 0);
+                    for (int i = 0; i < MT; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[q], wa[i][q], acc[i][j], 0, 0, 0);
             }
         }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage has been read: the block after the next may take it
     };
-    if (AHEAD) {
+    if (kb0 < kb1) {
         Block u, v;
-        if (kw < g.kblocks) load(kw, u);
-        for (int kb = kw; kb < g.kblocks; kb += 2 * wk) {
-            if (kb + wk < g.kblocks) load(kb + wk, v);
-            multiply(u);
-            if (kb + wk < g.kblocks) {
-                if (kb + 2 * wk < g.kblocks) load(kb + 2 * wk, u);
-                multiply(v);
+        issue(kb0);
+        load(kb0, u);
+        for (int kb = kb0; kb < kb1; kb += 2) {
+            if (kb + 1 < kb1) {
+                issue(kb + 1);
+                load(kb + 1, v);
             }
-        }
-    } else {
-        for (int kb = kw; kb < g.kblocks; kb += wk) {
-            Block u;
-            load(kb, u);
-            multiply(u);
+            multiply(kb, u);
+            if (kb + 1 < kb1) {
+                if (kb + 2 < kb1) {
+                    issue(kb + 2);
+                    load(kb + 2, u);
+                }
+                multiply(kb + 1, v);
+            }
         }
     }
     // acc[i][j][e] = C[16 i + l15][n0 + 16 j + 4 h + e]
+    auto part = [&](int w) { return reinterpret_cast<float*>(smem + w * 2 * STAGE); };
     const bool wide_out = g.kind == MH_F32;
     const int per = wide_out ? 4 : 8, lpr = NB * 16 / per;  // entries a thread stores, threads a row
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         if (i) __syncthreads();
 #pragma unroll
-        for (int j = 0; j < NB; ++j) *reinterpret_cast<f32x4*>(&part[wave][l15 * PITCH + j * 16 + h * 4]) = acc[i][j];
+        for (int j = 0; j < NB; ++j) *reinterpret_cast<f32x4*>(part(wave) + l15 * PITCH + j * 16 + h * 4) = acc[i][j];
         __syncthreads();
         for (int t = threadIdx.x; t < wn * 16 * lpr; t += 64 * RW) {
             const int gr = t / (16 * lpr), r = t / lpr % 16, c = t % lpr * per;
@@ -533,7 +606,7 @@ __global__ __launch_bounds__(64 * RW, 2) void fp8_rows_kernel(const F8Args g, co
             if (m >= g.M || n >= g.N) continue;
             f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
             for (int w = 0; w < wk; ++w) {
-                const float* p = &part[gr * wk + w][r * PITCH + c];
+                const float* p = part(gr * wk + w) + r * PITCH + c;
                 lo += *reinterpret_cast<const f32x4*>(p);
                 if (!wide_out) hi += *reinterpret_cast<const f32x4*>(p + 4);
             }
@@ -614,6 +687,17 @@ int64_t f8_part_bytes(int64_t M, int64_t N, int64_t K) {
     return p.slices > 1 ? (int64_t)p.slices * M * N * 4 : 0;
 }
 
+template <typename K, typename... A>
+int32_t f8_launch(K kern, dim3 grid, dim3 block, int lds, hipStream_t s, A... args) {
+    if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
+        (void)hipGetLastError();
+        mh_set_error("mh_fp8_matmul: %d bytes of LDS refused", lds);
+        return MH_ERR_LAUNCH;
+    }
+    MH_LAUNCH(kern, grid, block, lds, s, args...);
+    return MH_OK;
+}
+
 template <int BM, int BN, int WM, int WN>
 int32_t f8_launch_tiles(F8Args g, int slices, bool wide, hipStream_t s) {
     g.mt = (int)mh_ceil_div(g.M, BM);
@@ -622,36 +706,31 @@ int32_t f8_launch_tiles(F8Args g, int slices, bool wide, hipStream_t s) {
     const dim3 grid(8 * g.per_xcd, slices), block(WM * WN * 64);
     constexpr int lds = 2 * ((BM + BN) * 128 + (BM + BN) * 4);
     const auto kern = wide ? fp8_gemm_kernel<BM, BN, WM, WN, true> : fp8_gemm_kernel<BM, BN, WM, WN, false>;
-    if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
-        mh_set_error("mh_fp8_matmul: %d bytes of LDS refused", lds);
-        return MH_ERR_LAUNCH;
-    }
-    MH_LAUNCH(kern, grid, block, lds, s, g);
-    return MH_OK;
+    return f8_launch(kern, grid, block, lds, s, g);
 }
 
 template <int MT, int NB, typename X>
-void f8_launch_rows_nb(const F8Args& g, const X* x, int64_t ldx, int K, int wk, hipStream_t s) {
+int32_t f8_launch_rows_nb(const F8Args& g, const X* x, int64_t ldx, int K, int wk, hipStream_t s) {
     const dim3 grid((unsigned)mh_ceil_div(g.N, RW / wk * 16 * NB)), block(64 * RW);
-    if (g.kind != MH_BF16) MH_LAUNCH((fp8_rows_kernel<MT, NB, true, X>), grid, block, 0, s, g, x, ldx, K, wk);
-    else MH_LAUNCH((fp8_rows_kernel<MT, NB, false, X>), grid, block, 0, s, g, x, ldx, K, wk);
+    const auto kern = g.kind != MH_BF16 ? fp8_rows_kernel<MT, NB, true, X> : fp8_rows_kernel<MT, NB, false, X>;
+    return f8_launch(kern, grid, block, RW * 2 * f8_rows_stage<NB>(), s, g, x, ldx, K, wk);
 }
 template <int MT, typename X>
-void f8_launch_rows(const F8Args& g, const X* x, int64_t ldx, int K, hipStream_t s) {
+int32_t f8_launch_rows(const F8Args& g, const X* x, int64_t ldx, int K, hipStream_t s) {
     const int wk = g.kblocks >= 8 ? 8 : g.kblocks >= 4 ? 4 : g.kblocks >= 2 ? 2 : 1;
     // more rows of b a wavefront: a is read, or quantised, fewer times, as long as the workgroups still fill the chip
     auto groups = [&](int nb) { return mh_ceil_div(g.N, RW / wk * 16 * nb); };
-    if (groups(4) >= 192) f8_launch_rows_nb<MT, 4>(g, x, ldx, K, wk, s);
-    else if (groups(2) >= 192) f8_launch_rows_nb<MT, 2>(g, x, ldx, K, wk, s);
-    else f8_launch_rows_nb<MT, 1>(g, x, ldx, K, wk, s);
+    if (groups(4) >= 192) return f8_launch_rows_nb<MT, 4>(g, x, ldx, K, wk, s);
+    if (groups(2) >= 192) return f8_launch_rows_nb<MT, 2>(g, x, ldx, K, wk, s);
+    return f8_launch_rows_nb<MT, 1>(g, x, ldx, K, wk, s);
 }
-void f8_launch_rows_any(const F8Args& g, hipStream_t s) {
+int32_t f8_launch_rows_any(const F8Args& g, hipStream_t s) {
     const f8_stored* none = nullptr;
     const int mt = (int)mh_ceil_div(g.M, 16);
-    if (mt == 1) f8_launch_rows<1>(g, none, 0, 0, s);
-    else if (mt == 2) f8_launch_rows<2>(g, none, 0, 0, s);
-    else if (mt == 3) f8_launch_rows<3>(g, none, 0, 0, s);
-    else f8_launch_rows<4>(g, none, 0, 0, s);
+    if (mt == 1) return f8_launch_rows<1>(g, none, 0, 0, s);
+    if (mt == 2) return f8_launch_rows<2>(g, none, 0, 0, s);
+    if (mt == 3) return f8_launch_rows<3>(g, none, 0, 0, s);
+    return f8_launch_rows<4>(g, none, 0, 0, s);
 }
 
 int32_t f8_check_matrix(const char* who, const char* name, const void* q, int64_t ld, const void* s, int64_t lds, int64_t rows, int64_t K) {
@@ -684,7 +763,7 @@ int32_t f8_matmul(const char* who, const uint8_t* a, int64_t lda, const uint8_t*
     const bool wide = kind != MH_BF16;
     g.kb_split = p.kb_split;
     if (p.rows) {
-        f8_launch_rows_any(g, s);
+        if (int32_t rc = f8_launch_rows_any(g, s)) return rc;
         MH_CHECK_LAUNCH(who);
         return MH_OK;
     }
@@ -800,9 +879,10 @@ int32_t mh_fp8_linear(const void* x, int32_t x_dtype, int64_t ldx, const void* w
         const F8Args g = f8_args(nullptr, 0, nullptr, 0, static_cast<const uint8_t*>(w), ldw, static_cast<const uint8_t*>(w_scales), ldws, M, N, K, bias, out_dtype,
                                  out, ldo);
         hipStream_t s = mh_stream(stream);
-        if (x_dtype == MH_F32) f8_launch_rows<1>(g, static_cast<const float*>(x), ldx, (int)K, s);
-        else if (x_dtype == MH_BF16) f8_launch_rows<1>(g, static_cast<const lp_bf16*>(x), ldx, (int)K, s);
-        else f8_launch_rows<1>(g, static_cast<const lp_f16*>(x), ldx, (int)K, s);
+        const int32_t rc = x_dtype == MH_F32    ? f8_launch_rows<1>(g, static_cast<const float*>(x), ldx, (int)K, s)
+                           : x_dtype == MH_BF16 ? f8_launch_rows<1>(g, static_cast<const lp_bf16*>(x), ldx, (int)K, s)
+                                                : f8_launch_rows<1>(g, static_cast<const lp_f16*>(x), ldx, (int)K, s);
+        if (rc) return rc;
         MH_CHECK_LAUNCH("mh_fp8_linear");
         return MH_OK;
     }
