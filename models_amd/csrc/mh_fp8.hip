@@ -657,7 +657,9 @@ F8Plan f8_plan(int64_t M, int64_t N, int64_t K) {
     const int kb = (int)mh_ceil_div(K, 128);
     p.slices = 1;
     p.kb_split = (kb + 3) / 4 * 4;
-    if (M <= ROWS_MOST) {
+    // The streaming kernel reads a once for every 64 rows of b at most; of four 16-row groups of a that is too much where b is neither long nor its
+    // rows short (64 x 512 x 8192: 31 us, 18 on the tiles; 48 rows, or 64 x 14341 x 4096: 23 against 28, 26 against 30).
+    if (M <= ROWS_MOST && (M <= 48 || N >= 8192 || kb < 16)) {
         p.rows = true;
         return p;
     }
