@@ -9,6 +9,7 @@
 // summed axis contiguous and padded with zeros to whole blocks, so the loop has no tail in k.
 #include "mh_lowp.h"
 
+#include <atomic>
 #include <type_traits>
 
 namespace {
@@ -689,14 +690,24 @@ int64_t f8_part_bytes(int64_t M, int64_t N, int64_t K) {
     return p.slices > 1 ? (int64_t)p.slices * M * N * 4 : 0;
 }
 
-template <typename K, typename... A>
-int32_t f8_launch(K kern, dim3 grid, dim3 block, int lds, hipStream_t s, A... args) {
-    if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
-        (void)hipGetLastError();
-        mh_set_error("mh_fp8_matmul: %d bytes of LDS refused", lds);
-        return MH_ERR_LAUNCH;
+// Launches KERN with more LDS than a launch may ask for unannounced: announced once on each device.
+template <auto KERN, typename... A>
+int32_t f8_launch(dim3 grid, dim3 block, int lds, hipStream_t s, A... args) {
+    static std::atomic<uint64_t> announced{0};
+    if (lds > 65536) {
+        int dev = 0;
+        (void)hipGetDevice(&dev);
+        const uint64_t bit = (uint64_t)1 << (dev & 63);
+        if (!(announced.load(std::memory_order_relaxed) & bit)) {
+            if (hipFuncSetAttribute(reinterpret_cast<const void*>(KERN), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
+                (void)hipGetLastError();
+                mh_set_error("mh_fp8_matmul: %d bytes of LDS refused", lds);
+                return MH_ERR_LAUNCH;
+            }
+            announced.fetch_or(bit, std::memory_order_relaxed);
+        }
     }
-    MH_LAUNCH(kern, grid, block, lds, s, args...);
+    MH_LAUNCH(KERN, grid, block, lds, s, args...);
     return MH_OK;
 }
 
@@ -707,15 +718,16 @@ int32_t f8_launch_tiles(F8Args g, int slices, bool wide, hipStream_t s) {
     g.per_xcd = (int)mh_ceil_div((int64_t)g.mt * g.nt, 8);
     const dim3 grid(8 * g.per_xcd, slices), block(WM * WN * 64);
     constexpr int lds = 2 * ((BM + BN) * 128 + (BM + BN) * 4);
-    const auto kern = wide ? fp8_gemm_kernel<BM, BN, WM, WN, true> : fp8_gemm_kernel<BM, BN, WM, WN, false>;
-    return f8_launch(kern, grid, block, lds, s, g);
+    return wide ? f8_launch<fp8_gemm_kernel<BM, BN, WM, WN, true>>(grid, block, lds, s, g)
+                : f8_launch<fp8_gemm_kernel<BM, BN, WM, WN, false>>(grid, block, lds, s, g);
 }
 
 template <int MT, int NB, typename X>
 int32_t f8_launch_rows_nb(const F8Args& g, const X* x, int64_t ldx, int K, int wk, hipStream_t s) {
     const dim3 grid((unsigned)mh_ceil_div(g.N, RW / wk * 16 * NB)), block(64 * RW);
-    const auto kern = g.kind != MH_BF16 ? fp8_rows_kernel<MT, NB, true, X> : fp8_rows_kernel<MT, NB, false, X>;
-    return f8_launch(kern, grid, block, RW * 2 * f8_rows_stage<NB>(), s, g, x, ldx, K, wk);
+    constexpr int lds = RW * 2 * f8_rows_stage<NB>();
+    return g.kind != MH_BF16 ? f8_launch<fp8_rows_kernel<MT, NB, true, X>>(grid, block, lds, s, g, x, ldx, K, wk)
+                             : f8_launch<fp8_rows_kernel<MT, NB, false, X>>(grid, block, lds, s, g, x, ldx, K, wk);
 }
 template <int MT, typename X>
 int32_t f8_launch_rows(const F8Args& g, const X* x, int64_t ldx, int K, hipStream_t s) {

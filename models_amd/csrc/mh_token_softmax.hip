@@ -302,9 +302,21 @@ __device__ __forceinline__ uint64_t key_threshold(int k, int most, C count) {
     return t;
 }
 
+// how many of n keys are larger: keys[n], if n is odd, is 0
+__device__ __forceinline__ int place_of(uint64_t key, const uint64_t* keys, int n) {
+    typedef uint64_t two __attribute__((ext_vector_type(2)));
+    int place = 0;
+#pragma unroll 4
+    for (int i = 0; i < n; i += 2) {
+        const two v = *reinterpret_cast<const two*>(keys + i);
+        place += (v[0] > key ? 1 : 0) + (v[1] > key ? 1 : 0);
+    }
+    return place;
+}
+
 template <int NT>
 struct TopLds {
-    uint64_t cand[CAND];
+    __attribute__((aligned(16))) uint64_t cand[CAND + 2];
     union {
         float most[buckets<NT>()];     // while the row is read
         uint16_t list[buckets<NT>()];  // the buckets to read again
@@ -413,11 +425,11 @@ __device__ __forceinline__ void top_entries(const T* x, int n, int first, int k,
         __syncthreads();
         have = s.n;
     }
+    if (threadIdx.x == 0) s.cand[have] = 0;  // the other of the last pair
+    __syncthreads();
     if (threadIdx.x < have) {
         const uint64_t key = s.cand[threadIdx.x];
-        int place = 0;
-#pragma unroll 8
-        for (int i = 0; i < have; ++i) place += s.cand[i] > key ? 1 : 0;
+        const int place = place_of(key, s.cand, have);
         if (place < k) emit(place, key);
     }
     for (int i = have + threadIdx.x; i < k; i += NT) emit(i, (uint64_t)0);
@@ -507,7 +519,7 @@ __device__ __forceinline__ Sum join_parts(const float4* part, int parts, float c
 
 template <typename T>
 __global__ __launch_bounds__(512) void token_logprobs_join_kernel(const LpArgs g) {
-    __shared__ uint64_t cand[512];
+    __shared__ __attribute__((aligned(16))) uint64_t cand[512 + 2];
     __shared__ Sum sums[8];
     __shared__ int red[16], have;
     const int64_t row = blockIdx.x;
@@ -537,11 +549,11 @@ __global__ __launch_bounds__(512) void token_logprobs_join_kernel(const LpArgs g
     for (int j = 0; j < JOIN_MOST / 512; ++j)
         if (key[j] >= th) cand[atomicAdd(&have, 1)] = key[j];
     __syncthreads();
+    if (threadIdx.x == 0) cand[have] = 0;
+    __syncthreads();
     if (threadIdx.x < have) {
         const uint64_t mine = cand[threadIdx.x];
-        int place = 0;
-#pragma unroll 8
-        for (int i = 0; i < have; ++i) place += cand[i] > mine ? 1 : 0;
+        const int place = place_of(mine, cand, have);
         if (place < g.k) lp_emit(g, row, t, place, mine);
     }
     for (int i = have + threadIdx.x; i < g.k; i += 512) lp_emit(g, row, t, i, (uint64_t)0);

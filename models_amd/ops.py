@@ -2141,13 +2141,16 @@ def _elsewhere(first: torch.Tensor, *others: Optional[torch.Tensor]) -> bool:
     for t in others:
         if t is not None and t.get_device() != at:
             raise ValueError(f"all tensors of a call must be on one device, got {first.device} and {t.device}")
-    return at != torch.cuda.current_device()
+    return at != torch._C._cuda_getDevice()
 
 
 def _float_2d(t: torch.Tensor, name: str) -> int:
     """The type code of a 2-D fp32 / bf16 / fp16 tensor whose rows are contiguous (any distance between rows)."""
-    _dev(t, name)
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        _dev(t, name)
     code = _FLOATS.get(t.dtype)
+    if code is not None and t.dim() == 2 and t.is_contiguous():
+        return code
     if code is None:
         raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
     if t.dim() != 2 or not (t.is_contiguous() or ((t.stride(1) == 1 or t.shape[1] <= 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]))):
@@ -2166,7 +2169,7 @@ def _at(t: Optional[torch.Tensor]) -> Optional[int]:
 
 def _here() -> int:
     """The current device's current stream (what ``_stream`` gives, without the objects around it: these calls can be a few microseconds)."""
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 class _Untimed:
@@ -2199,16 +2202,19 @@ class Fp8Matrix(NamedTuple):
 
 def _fp8_check(m: Fp8Matrix, name: str) -> Tuple[int, int]:
     v, s, K = m
-    _dev(v, name, torch.float8_e4m3fn)
-    _dev(s, name, torch.uint8)
+    if not (isinstance(v, torch.Tensor) and isinstance(s, torch.Tensor) and v.is_cuda and s.is_cuda
+            and v.dtype is torch.float8_e4m3fn and s.dtype is torch.uint8):
+        _dev(v, name, torch.float8_e4m3fn)
+        _dev(s, name, torch.uint8)
     kb = -(-K // _FP8_BLOCK)
-    if K < 1 or v.dim() != 2 or s.dim() != 2 or v.shape[1] != kb * _FP8_BLOCK or s.shape[0] != v.shape[0] or s.shape[1] != -(-kb // 4) * 4:
+    vs, ss = v.shape, s.shape
+    if K < 1 or len(vs) != 2 or vs[1] != kb * _FP8_BLOCK or ss != (vs[0], -(-kb // 4) * 4):
         raise ValueError(f"{name}: values {tuple(v.shape)} and scales {tuple(s.shape)} are not the 8-bit form of a matrix of {K} columns")
     if not (v.is_contiguous() and s.is_contiguous()):
         raise ValueError(f"{name}: values and scales must be contiguous")
     if s.get_device() != v.get_device():
         raise ValueError(f"{name}: values and scales must be on one device")
-    return v.shape[0], K
+    return vs[0], K
 
 
 def fp8_quantize(x: torch.Tensor, transpose: bool = False, column_sums: bool = False):
