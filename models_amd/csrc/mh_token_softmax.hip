@@ -306,7 +306,7 @@ __device__ __forceinline__ uint64_t key_threshold(int k, int most, C count) {
 __device__ __forceinline__ int place_of(uint64_t key, const uint64_t* keys, int n) {
     typedef uint64_t two __attribute__((ext_vector_type(2)));
     int place = 0;
-#pragma unroll 4
+#pragma unroll 8
     for (int i = 0; i < n; i += 2) {
         const two v = *reinterpret_cast<const two*>(keys + i);
         place += (v[0] > key ? 1 : 0) + (v[1] > key ? 1 : 0);
@@ -321,6 +321,7 @@ struct TopLds {
         float most[buckets<NT>()];     // while the row is read
         uint16_t list[buckets<NT>()];  // the buckets to read again
     };
+    uint32_t low;
     int n, nq, red[2 * (NT / 64)];
 };
 
@@ -337,17 +338,30 @@ __device__ __forceinline__ void top_entries(const T* x, int n, int first, int k,
     uint32_t mine[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) mine[i] = i * NT + (int)threadIdx.x < nb ? key_of(s.most[i * NT + threadIdx.x] + 0.f) : 0;
-    // the k-th largest of the threads' largest, to 16 bits: a little below the buckets' own, and one comparison a round
-    uint32_t largest = 0, low = 0;
+    // The k-th largest of the threads' largest, to 16 bits: a little below the buckets' own.  One wavefront looks for it, the others' in its registers:
+    // no barrier a round.
+    uint32_t* const top = reinterpret_cast<uint32_t*>(s.cand);
+    uint32_t largest = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) largest = mine[i] > largest ? mine[i] : largest;
-    if (nb >= k)
-        for (int b = 31; b >= 16; --b) {
-            const uint32_t next = low | 1u << b;
-            if (count_block<NT>(lanes(largest >= next), s.red, phase) >= k) low = next;
-        }
-    if (low <= KEY_NONE) low = KEY_NONE + 1;
+    top[threadIdx.x] = largest;
     __syncthreads();
+    if (threadIdx.x < 64) {
+        uint32_t of[NT / 64], t = 0;
+#pragma unroll
+        for (int w = 0; w < NT / 64; ++w) of[w] = top[w * 64 + threadIdx.x];
+        if (nb >= k)
+            for (int b = 31; b >= 16; --b) {
+                const uint32_t next = t | 1u << b;
+                int c = 0;
+#pragma unroll
+                for (int w = 0; w < NT / 64; ++w) c += lanes(of[w] >= next);
+                if (c >= k) t = next;
+            }
+        if (threadIdx.x == 0) s.low = t;
+    }
+    __syncthreads();
+    const uint32_t low = s.low <= KEY_NONE ? KEY_NONE + 1 : s.low;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
         if (mine[i] >= low) s.list[atomicAdd(&s.nq, 1)] = (uint16_t)(i * NT + threadIdx.x);
