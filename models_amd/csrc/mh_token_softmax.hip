@@ -15,9 +15,9 @@
 namespace {
 
 constexpr float LN2 = 0.693147180559945309f;
-// The pass works with l c up to a magnitude of 2^28 (see Run).  A thread's running maximum starts at -2^28 / c: entries below count as 0, and a row
-// whose entries all lie there (masks of the type's lowest value) comes out with a sum of zero; one with an entry beyond 2^29 / c is marked.  Both
-// are summed again against their true maximum.
+// The pass works with l c up to a magnitude of 2^28 (see Run).  A thread's running maximum starts at -2^28 / c: a row whose entries all lie below (masks
+// of the type's lowest value) comes out with a sum under 1, where the largest entry alone gives 1; one with an entry beyond 2^29 / c is marked.
+// Both are summed again against their true maximum.
 constexpr float FAR = 0x1p28f;
 constexpr float INF = __builtin_inff();
 constexpr int TOP_MOST = 256;        // most alternatives, and teacher entries, of a row
@@ -128,13 +128,15 @@ __device__ __forceinline__ int count_block(int of_wave, int* red, int& phase) {
 __device__ __forceinline__ int lanes(bool p) { return __popcll(__ballot(p)); }
 
 // The sums of a thread while it reads: t = l c - B in one fused operation, B the rounded product m c.  What B lacks of m c -- 16 at most below 2^29 --
-// is put right once, at the end, exactly: fma(m, c, -B) is what the rounding took.
+// is put right once, at the end, exactly: fma(m, c, -B) is what the rounding took.  The step from one B to the next takes the rounded products too:
+// fused with its subtraction, B - most c would miss what the later terms are measured from by as much as B lacks.
 struct Run {
     float m, B, s = 0.f, u = 0.f;
     __device__ __forceinline__ explicit Run(float c) : m(-FAR / c), B(m * c) {}
     template <bool ENT, int N>
     __device__ __forceinline__ void take(const float (&v)[N], float most, float c) {
         if (most > m) {
+#pragma clang fp contract(off)
             const float nb = most * c, d = fmaxf(B - nb, -200.f), f = ex2(d);
             if (ENT) u = f * fmaf(d, s, u);
             s *= f;
@@ -257,7 +259,7 @@ __device__ __forceinline__ Sum read_sums(const T* x, int n, float c, const uint3
     }
     const bool beyond = __syncthreads_or(!(r.B < 2.f * FAR));
     Sum t = sum_block<NT>(r.sum(c), c, red);
-    if (t.s == 0.f || beyond) {
+    if (t.s < 0.5f || beyond) {
         t = Sum{max_block<NT>(most, reinterpret_cast<float*>(red)), 0.f, 0.f};
         if (t.m == -INF) return t;
         Sum a = {t.m, 0.f, 0.f};
@@ -962,7 +964,7 @@ __global__ __launch_bounds__(NT) void distill_topk_train_kernel(const DsArgs g, 
     }
     const bool beyond = __syncthreads_or(!(run.B < 2.f * FAR));
     Sum t = sum_block<NT>(run.sum(g.c), g.c, red);
-    if (t.s == 0.f || beyond) {  // as in read_sums
+    if (t.s < 0.5f || beyond) {  // as in read_sums
         t = Sum{max_block<NT>(most, reinterpret_cast<float*>(red)), 0.f, 0.f};
         if (t.m != -INF) {
             Sum a = {t.m, 0.f, 0.f};
@@ -1041,8 +1043,9 @@ int32_t ts_check(const char* who, const void* x, int32_t dtype, int64_t ld, int6
     MH_REQUIRE(N == 0 || x, "%s: logits is NULL", who);
     return MH_OK;
 }
+// a launch has fewer than 2^32 threads
 int32_t ts_grid(const char* who, int64_t N, int parts) {
-    MH_REQUIRE(N * parts < (int64_t)1 << 31, "%s: %lld rows in %d parts are too many", who, (long long)N, parts);
+    MH_REQUIRE(N * parts < (int64_t)1 << 23, "%s: %lld rows in %d parts each are too many workgroups for one call", who, (long long)N, parts);
     return MH_OK;
 }
 int32_t ts_workspace(const char* who, const void* ws, int64_t bytes, int64_t need) {
@@ -1130,18 +1133,20 @@ void ds_train(const DsArgs& g, const float* dloss, void* d, int64_t ldd, hipStre
     else ds_train_launch<4, T>(g, dloss, out, ldd, s);
 }
 template <typename T>
-void grad_launch(GradArgs g, bool distill, hipStream_t s) {
+int32_t grad_launch(const char* who, GradArgs g, bool distill, hipStream_t s) {
     plan_parts(g.N, g.V, 1 << 20, mh_ceil_div(g.V * (int64_t)sizeof(T), distill ? GRAD_BYTES_DISTILL : GRAD_BYTES_LOGPROBS), g.parts, g.chunk);
+    if (int32_t rc = ts_grid(who, g.N, g.parts)) return rc;
     const dim3 grid((unsigned)(g.N * g.parts));
     if (distill) MH_LAUNCH((distill_topk_bwd_kernel<512, T>), grid, dim3(512), 0, s, g);
     else MH_LAUNCH((token_logprobs_bwd_kernel<512, T>), grid, dim3(512), 0, s, g);
-}
-int32_t grad_any(const char* who, const GradArgs& g, int32_t dtype, bool distill, hipStream_t s) {
-    if (dtype == MH_F32) grad_launch<float>(g, distill, s);
-    else if (dtype == MH_BF16) grad_launch<lp_bf16>(g, distill, s);
-    else grad_launch<lp_f16>(g, distill, s);
     MH_CHECK_LAUNCH(who);
     return MH_OK;
+}
+int32_t grad_any(const char* who, const GradArgs& g, int32_t dtype, bool distill, hipStream_t s) {
+    MH_REQUIRE(g.d != g.x || g.ldd == g.ld, "%s: a gradient in place of the logits needs their leading dimension", who);
+    if (dtype == MH_F32) return grad_launch<float>(who, g, distill, s);
+    if (dtype == MH_BF16) return grad_launch<lp_bf16>(who, g, distill, s);
+    return grad_launch<lp_f16>(who, g, distill, s);
 }
 
 }  // namespace
@@ -1238,6 +1243,8 @@ int32_t mh_distill_topk_train(const void* logits, int32_t dtype, int64_t ld, int
     if (N == 0) return MH_OK;
     MH_REQUIRE(teacher_ids && teacher_logp && loss && dlogits && ld_ids >= K && ld_logp >= K && ldd >= V,
                "mh_distill_topk_train: an argument is NULL, or rows are too short");
+    MH_REQUIRE(dlogits != logits || ldd == ld, "mh_distill_topk_train: a gradient in place of the logits needs their leading dimension");
+    if (int32_t rc = ts_grid("mh_distill_topk_train", N, 1)) return rc;
     const int64_t need = mh_distill_topk_train_workspace_bytes(N, V, K, dtype, tail);
     if (int32_t rc = ts_workspace("mh_distill_topk_train", workspace, workspace_bytes, need)) return rc;
     if (need) {

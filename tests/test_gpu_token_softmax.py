@@ -183,6 +183,9 @@ def awkward(dtype, V, rng):
     a = np.round(base); rows.append(a)                                                    # ties
     a = base.copy(); a[::4096] = 50 + np.arange(len(a[::4096])) % 3; rows.append(a)        # the largest at one stride
     a = np.where(np.arange(V) < V // 2, -1e8 if dtype != "f16" else -5e4, base); rows.append(a)  # a long masked prefix
+    if dtype == "f32":  # around the place where a thread's maximum starts
+        step = 16.0 * np.round(rng.normal(size=V))
+        rows += [-2.0 ** 28 / 1.4426950408889634 - 100 + step, -2.0 ** 28 / 1.4426950408889634 + step]
     if dtype != "f16":
         rows += [np.full(V, 1e10), np.full(V, -1e20), base * 1e12, base * 1e30, np.full(V, 3e38)]
     a = base.copy(); a[V // 3] = np.nan; rows.append(a)
@@ -446,6 +449,43 @@ def test_streams_and_graphs(device):
         assert same(step(xs[i]), want[i])
 
 
+def test_recorded_and_replayed(device):
+    """The library's own launch recording replays the calls on new inputs in the same buffers."""
+    import ctypes as C
+
+    from models_amd import _lib
+
+    lib = _lib.load()
+    rng = np.random.default_rng(2)
+    xs = [make(rng, 5, 3000, "f32", device) for _ in range(2)]
+    ids, (tid, tlp) = torch.tensor(rng.integers(0, 3000, 5), device=device), teacher(rng, 5, 3000, 7, device)
+    w8 = ops.fp8_quantize(torch.randn(40, 3000, device=device))
+    keep = []
+
+    def step(x):
+        r = ops.token_logprobs(x, ids, k=4)
+        s, d = ops.distill_topk_train(x, tid, tlp, None, 1.0, True)
+        keep.append((r, s, d))
+        return [r.logp, r.entropy, r.top_logp, r.top_ids, s.loss, d, ops.fp8_linear(x, w8)]
+
+    static = xs[0].clone()
+    h = C.c_void_p()
+    assert lib.mh_record_begin() == 0
+    out = step(static)
+    assert lib.mh_record_end(C.byref(h)) == 0
+    for i in (1, 0, 1):
+        static.copy_(xs[i])
+        torch.cuda.synchronize()
+        assert lib.mh_record_replay(h) == 0
+        torch.cuda.synchronize()
+        want = ops.token_logprobs(xs[i], ids, k=4)
+        s, d = ops.distill_topk_train(xs[i], tid, tlp, None, 1.0, True)
+        y = ops.fp8_linear(xs[i], w8)
+        for a, b in zip(out, [want.logp, want.entropy, want.top_logp, want.top_ids, s.loss, d, y]):
+            assert torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0))
+    lib.mh_record_free(h)
+
+
 def test_refusals(device):
     x = torch.zeros(4, 10, device=device)
     ids = torch.zeros(4, dtype=torch.int64, device=device)
@@ -471,6 +511,10 @@ def test_refusals(device):
                 lambda: ops.token_logprobs_backward(x, ids, r, dlogp=one.half())):
         with pytest.raises(TypeError):
             bad()
+    assert ops.token_logprobs(x, ids, temperature=np.float32(0.5)).logp.shape == (4,)
+    wide = torch.zeros(4, 12, device=device)
+    with pytest.raises(ValueError):
+        ops.token_logprobs_backward(wide[:2, :10], ids[:2], ops.token_logprobs(wide[:2, :10], ids[:2]), one[:2], out=wide.view(-1)[:20].view(2, 10))
     assert ops.token_logprobs(x[:0], ids[:0], k=2).top_ids.shape == (0, 2)
     assert ops.token_logprobs_backward(x[:0], ids[:0], ops.token_logprobs(x[:0], ids[:0]), dlogp=one[:0]).shape == (0, 10)
     assert ops.distill_topk_train(x[:0], tid[:0], tlp[:0])[1].shape == (0, 10)
