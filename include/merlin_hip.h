@@ -712,7 +712,8 @@ int32_t mh_sharded_lookup_bwd(mh_comm_t comm, int32_t F, int64_t B, int64_t capa
  * mh_fp8_matmul: out[M, N] = a b^T + bias, a [M, K] and b [N, K] in that form, bias [N] floats or NULL, out of type out_dtype with leading
  * dimension ldo.  An MH_F32 or MH_F16 output is summed in 32 bits throughout; an MH_BF16 one by the 8-bit matrix instruction, at twice the
  * rate, whose sums are off by at most 7 * 2^-13 of sum |a b| (under half a step of bf16; 1.5e-5 of the norm on random values).  mh_fp8_linear: x [M, K] quantised into the workspace, then the product with w [N, K].
- * K <= 2^24 - 128, leading dimensions of 8-bit values <= 2^24.  No atomics: results do not change from call to call.  Rows past M and columns past N of out are left as they were. */
+ * K <= 2^24 - 128, leading dimensions of 8-bit values <= 2^24, M, N < 2^27; in MH_F32 and MH_F16 outputs a value under 2^-126 may count as 0.
+ * No atomics: results do not change from call to call.  Rows past M and columns past N of out are left as they were. */
 int32_t mh_fp8_quantize(const void* x, int32_t dtype, int64_t ldx, int64_t R, int64_t K, int32_t transpose, void* q, int64_t ldq,
                         void* scales, int64_t lds, float* colsum, void* workspace, int64_t workspace_bytes, mh_stream_t stream);
 int64_t mh_fp8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K);
@@ -726,13 +727,13 @@ int32_t mh_fp8_linear(const void* x, int32_t x_dtype, int64_t ldx, const void* w
 
 /* ---- softmax over a catalogue's logits: log probabilities, entropy, alternatives; distillation ------------------------------------
  * logits [N, V] of type code dtype, leading dimension ld >= V, contiguous rows at any element's address; temperature in [1e-4, 1e4], z = logits /
- * temperature; V < 2^31 - 65536.  A logit of -inf is masked (p = 0).  A row with nothing left has log p = -inf, entropy 0, lse -inf and a
+ * temperature; V < 2^31 - 65536, N < 2^23.  A logit of -inf is masked (p = 0).  A row with nothing left has log p = -inf, entropy 0, lse -inf and a
  * gradient of zero.  A NaN or +inf among a row's logits makes its values NaN.  Sums in 32 bits; no atomics on results: they do not change from
  * call to call.
  * mh_token_logprobs: logp[n] = log softmax(z[n])[ids[n]] (0 where ids[n] is outside [0, V): padding; ids and logp may be NULL), entropy[n],
  * lse[n] = log sum exp z[n], and the k (<= 256, <= V) largest entries of each row, ties to the lowest index: top_ids [N, k] and their log
  * probabilities top_logp [N, k]; places past the row's unmasked entries hold -1 and -inf, NaN is never an alternative.  stats [N, 2]: for _bwd.
- * mh_token_logprobs_bwd: dlogits [N, V] (leading dimension ldd, type of logits, all V columns written; may be logits itself) =
+ * mh_token_logprobs_bwd: dlogits [N, V] (leading dimension ldd, type of logits, all V columns written; may be logits itself with ldd = ld) =
  * dlogp (onehot - p) - dentropy p (log p + entropy) + dlse p, over temperature.  dlogp / dentropy / dlse [N] or NULL (zero). */
 int64_t mh_token_logprobs_workspace_bytes(int64_t N, int64_t V, int32_t k);
 int32_t mh_token_logprobs(const void* logits, int32_t dtype, int64_t ld, int64_t N, int64_t V, const void* ids, int32_t ids_dtype, int32_t k,

@@ -805,11 +805,11 @@ int32_t f8_quantize(const T* x, int64_t ldx, int64_t R, int64_t K, bool transpos
                     hipStream_t s) {
     if (!transpose) {
         const int64_t quads = mh_ceil_div(mh_ceil_div(K, 128), 4), blocks = mh_ceil_div(R, 4) * quads;
-        MH_REQUIRE(blocks < (int64_t)1 << 31, "mh_fp8_quantize: matrix too large");
+        MH_REQUIRE(blocks < (int64_t)1 << 24, "mh_fp8_quantize: matrix too large for one launch (2^32 threads)");
         MH_LAUNCH(fp8_quantize_rows_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, x, ldx, R, (int)K, (int)quads, q, ldq, sc, lds);
     } else {
         const int64_t rb = mh_ceil_div(R, 128), blocks = rb * mh_ceil_div(K, 64);
-        MH_REQUIRE(blocks < (int64_t)1 << 31, "mh_fp8_quantize: matrix too large");
+        MH_REQUIRE(blocks < (int64_t)1 << 23, "mh_fp8_quantize: matrix too large for one launch (2^32 threads)");
         MH_LAUNCH(fp8_quantize_cols_kernel<T>, dim3((unsigned)blocks), dim3(512), 0, s, x, ldx, R, K, (int)rb, (int)(mh_ceil_div(rb, 4) * 4), q, ldq, sc, lds,
                   colsum);
     }
@@ -821,11 +821,11 @@ int64_t f8_q_bytes(int64_t rows, int64_t K) { return mh_ceil_div(rows * mh_ceil_
 int64_t f8_s_bytes(int64_t rows, int64_t K) { return mh_ceil_div(rows * mh_ceil_div(mh_ceil_div(K, 128), 4) * 4, 256) * 256; }
 
 int32_t f8_check_out(const char* who, int64_t M, int64_t N, int64_t K, int32_t kind, const void* out, int64_t ldo) {
-    MH_REQUIRE(M >= 0 && N >= 0 && K >= 1 && K <= MOST_K && M < (int64_t)1 << 31 && N < (int64_t)1 << 31, "%s: sizes M=%lld N=%lld K=%lld", who,
+    MH_REQUIRE(M >= 0 && N >= 0 && K >= 1 && K <= MOST_K && M < (int64_t)1 << 27 && N < (int64_t)1 << 27, "%s: sizes M=%lld N=%lld K=%lld", who,
                (long long)M, (long long)N, (long long)K);
     MH_REQUIRE(kind == MH_F32 || kind == MH_BF16 || kind == MH_F16, "%s: unknown output type %d", who, (int)kind);
     MH_REQUIRE(ldo >= N && (out || M * N == 0), "%s: output rows of %lld entries cannot hold %lld", who, (long long)ldo, (long long)N);
-    MH_REQUIRE(mh_ceil_div(M, 128) * mh_ceil_div(N, 128) < (int64_t)1 << 28 && M * mh_ceil_div(N, 4) < (int64_t)1 << 38, "%s: output too large", who);
+    MH_REQUIRE(mh_ceil_div(M, 128) * mh_ceil_div(N, 128) < (int64_t)1 << 23, "%s: output too large for one launch (2^32 threads)", who);
     return MH_OK;
 }
 

@@ -2381,14 +2381,15 @@ def _row_floats(t: Optional[torch.Tensor], shape, name: str) -> Optional[torch.T
 
 
 def _catalogue(logits: torch.Tensor, temperature: float):
-    """(type code, N, V) of catalogue logits, with the checks all of the following share."""
+    """(type code, N, V, temperature) of catalogue logits, with the checks all of the following share."""
     dt = _float_2d(logits, "logits")
     N, V = logits.shape
     if V < 1:
         raise ValueError(f"logits must have at least one column, got shape {tuple(logits.shape)}")
-    if not 1e-4 <= float(temperature) <= 1e4:
+    temperature = float(temperature)
+    if not 1e-4 <= temperature <= 1e4:
         raise ValueError(f"temperature must lie in [1e-4, 1e4], got {temperature}")
-    return dt, N, V
+    return dt, N, V, temperature
 
 
 def _dlogits(logits: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
@@ -2408,7 +2409,7 @@ def token_logprobs(logits: torch.Tensor, ids: Optional[torch.Tensor] = None, k: 
     (at most 256) of each row, from one pass over ``logits`` [N, V] (float32 / bfloat16 / float16; rows may be parts of wider ones, as the
     logits that ``inbatch_softmax`` or ``fp8_matmul`` returns).  Logits of -inf are masked; ids outside [0, V) are padding."""
     lib = _lib.load()
-    dt, N, V = _catalogue(logits, temperature)
+    dt, N, V, temperature = _catalogue(logits, temperature)
     ids, idt = _row_ids(ids, (N,), "ids")
     k = int(k)
     if not 0 <= k <= min(V, 256):
@@ -2436,7 +2437,7 @@ def token_logprobs_backward(logits: torch.Tensor, ids: Optional[torch.Tensor], r
     ids and temperature; each of the three is ``[N]`` float32 or None.  ``out`` may be ``logits`` itself.  Padded ids take no ``dlogp``;
     the top alternatives are to be read and have no gradient."""
     lib = _lib.load()
-    dt, N, V = _catalogue(logits, temperature)
+    dt, N, V, temperature = _catalogue(logits, temperature)
     ids, idt = _row_ids(ids, (N,), "ids")
     if dlogp is not None and ids is None:
         raise ValueError("dlogp needs ids")
@@ -2487,7 +2488,7 @@ def distill_topk(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logp: 
     ``tail=False``: the teacher's mass is the softmax of its K entries.  ``tail=True``: it is ``exp(teacher_logp)``, and what is left of 1 is
     held against the student's probability outside the entries.  Ids outside [0, V) are left out; a row without any has loss 0."""
     lib = _lib.load()
-    dt, N, V = _catalogue(logits, temperature)
+    dt, N, V, temperature = _catalogue(logits, temperature)
     if teacher_logp is None:
         raise ValueError("teacher_logp is needed")
     idt, K = _teacher(logits, teacher_ids, teacher_logp)
@@ -2512,7 +2513,7 @@ def distill_topk_backward(logits: torch.Tensor, teacher_ids: torch.Tensor, resul
     """d / d logits of ``sum(dloss * loss)`` (``dloss`` [N] float32; None: ones) for the ``result`` of ``distill_topk`` on the same logits, ids
     and temperature.  ``out`` may be ``logits`` itself."""
     lib = _lib.load()
-    dt, N, V = _catalogue(logits, temperature)
+    dt, N, V, temperature = _catalogue(logits, temperature)
     idt, K = _teacher(logits, teacher_ids)
     if result.stats is None or result.top_grad is None:
         raise ValueError("the result of distill_topk(..., need_grad=False) has no gradient")
@@ -2537,7 +2538,7 @@ def distill_topk_train(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_
     ``distill_topk_backward`` in one call, which is one launch and one read for rows of up to 32768 entries of 16 bits (16384 of 32).  The
     result holds the loss alone.  ``out`` may be ``logits`` itself."""
     lib = _lib.load()
-    dt, N, V = _catalogue(logits, temperature)
+    dt, N, V, temperature = _catalogue(logits, temperature)
     if teacher_logp is None:
         raise ValueError("teacher_logp is needed")
     idt, K = _teacher(logits, teacher_ids, teacher_logp)

@@ -20,7 +20,8 @@ def matmul(a=A, lda=256, sa=A, ldsa=4, b=A, ldb=256, sb=A, ldsb=4, M=4, N=8, K=2
 
 @pytest.mark.parametrize("kw", [dict(dtype=3), dict(dtype=-1), dict(ldx=255), dict(R=-1), dict(K=1 << 31), dict(x=None), dict(q=None), dict(s=None),
                                 dict(ldq=128), dict(ldq=264), dict(q=A + 8), dict(lds=2), dict(lds=6), dict(s=A + 2), dict(colsum=A),
-                                dict(transpose=1, R=300, ldq=256)])
+                                dict(transpose=1, R=300, ldq=256),
+                                dict(R=1 << 27), dict(R=1 << 27, K=1024, ldx=1024, transpose=1, ldq=1 << 27, lds=1 << 20)])
 def test_quantize_refuses(kw):
     assert quantize(**kw) == -1
     assert _lib.load().mh_last_error()
@@ -32,7 +33,8 @@ def test_quantize_needs_its_workspace_for_column_sums():
 
 
 @pytest.mark.parametrize("kw", [dict(a=None), dict(sb=None), dict(lda=240), dict(ldb=128), dict(ldsa=3), dict(dt=7), dict(ldo=7), dict(out=None), dict(K=0),
-                                dict(M=-1), dict(b=A + 4), dict(ldsb=0)])
+                                dict(M=-1), dict(b=A + 4), dict(ldsb=0), dict(M=1 << 27), dict(N=1 << 27, ldo=1 << 27), dict(M=1 << 26, N=1 << 20, ldo=1 << 20),
+                                dict(K=1 << 24, lda=1 << 24, ldb=1 << 24, ldsa=1 << 17, ldsb=1 << 17), dict(lda=(1 << 24) + 16)])
 def test_matmul_refuses(kw):
     assert matmul(**kw) == -1
 

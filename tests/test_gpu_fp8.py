@@ -195,6 +195,34 @@ def test_gradients_are_those_of_the_layer(device):
         assert abs(dw[i, j].item() - num) <= 0.13 * (np.abs(x[:, i]) * np.abs(dy[:, j])).sum() + 1e-5
 
 
+@pytest.mark.parametrize("M", [3, 40, 200])
+@pytest.mark.parametrize("out", ["f32", "bf16", "f16"])
+def test_nan_and_infinity_stay_in_their_row(device, M, out):
+    g = torch.Generator(device=device).manual_seed(M)
+    x, w = torch.randn(M, 300, generator=g, device=device), torch.randn(70, 300, generator=g, device=device)
+    w8 = ops.fp8_quantize(w)
+    want = ops.fp8_linear(x, w8, out_dtype=TYPES[out])
+    x[1, 7], x[M - 1, 299] = float("nan"), float("inf")
+    got = ops.fp8_linear(x, w8, out_dtype=TYPES[out])
+    assert torch.isnan(got[[1, M - 1]]).all()
+    rows = [r for r in range(M) if r not in (1, M - 1)]
+    assert torch.equal(got[rows], want[rows])
+
+
+def test_wide_range_of_scales(device):
+    """Blocks of very small and very large entries: what the product of the scales brings back into range is right."""
+    rng = np.random.default_rng(8)
+    for out in ("f32", "bf16"):
+        x, w = rng.normal(size=(20, 384)), rng.normal(size=(33, 384))
+        x[:, :128] *= 2.0 ** -60
+        w[:, :128] *= 2.0 ** 60
+        x[:, 256:] *= 2.0 ** 90
+        w[:, 256:] *= 2.0 ** -92
+        t = lambda a: torch.tensor(a, dtype=torch.float32, device=device)  # noqa: E731
+        y = ops.fp8_linear(t(x), ops.fp8_quantize(t(w)), out_dtype=TYPES[out])
+        check_product(y, quantized(f64(t(x)))[0], quantized(f64(t(w)))[0], None, out)
+
+
 def test_empty_and_refused(device):
     z = lambda *s, dtype=torch.float32: torch.zeros(*s, dtype=dtype, device=device)  # noqa: E731
     w8 = ops.fp8_quantize(z(4, 8), transpose=True)

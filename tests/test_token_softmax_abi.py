@@ -25,22 +25,22 @@ COMMON = [dict(x=None), dict(dt=3), dict(ld=999), dict(N=-1), dict(V=0), dict(V=
 
 
 @pytest.mark.parametrize("kw", COMMON + [dict(k=-1), dict(k=257), dict(k=1001), dict(ent=None), dict(lse=None), dict(logp=None), dict(tids=None), dict(tlogp=None),
-                                         dict(N=(1 << 31) - 1, V=20000, ld=20000, k=0, ids=None, ent=None)])
+                                         dict(N=1 << 23), dict(N=(1 << 31) - 1, V=20000, ld=20000)])
 def test_logprobs_refuses(kw):
     assert call("mh_token_logprobs", LP, LP, **kw) == -1
 
 
-@pytest.mark.parametrize("kw", COMMON + [dict(d=None), dict(ldd=999), dict(ent=None), dict(ids=None)])
+@pytest.mark.parametrize("kw", COMMON + [dict(d=None), dict(ldd=999), dict(ent=None), dict(ids=None), dict(N=1 << 23), dict(d=A, ldd=1001)])
 def test_logprobs_bwd_refuses(kw):
     assert call("mh_token_logprobs_bwd", LPB, LPB, **kw) == -1
 
 
-@pytest.mark.parametrize("kw", COMMON + [dict(K=0), dict(K=257), dict(ids=None), dict(tlp=None), dict(loss=None), dict(top=None), dict(ldi=4), dict(ldt=4)])
+@pytest.mark.parametrize("kw", COMMON + [dict(K=0), dict(K=257), dict(ids=None), dict(tlp=None), dict(loss=None), dict(top=None), dict(ldi=4), dict(ldt=4), dict(N=1 << 23)])
 def test_distill_refuses(kw):
     assert call("mh_distill_topk", DS, DS, **kw) == -1
 
 
-@pytest.mark.parametrize("kw", COMMON + [dict(K=0), dict(K=257), dict(ids=None), dict(top=None), dict(d=None), dict(ldd=10), dict(ldi=4)])
+@pytest.mark.parametrize("kw", COMMON + [dict(K=0), dict(K=257), dict(ids=None), dict(top=None), dict(d=None), dict(ldd=10), dict(ldi=4), dict(N=1 << 23), dict(ldd=1001)])
 def test_distill_bwd_refuses(kw):
     assert call("mh_distill_topk_bwd", DSB, DSB, **kw) == -1
 
@@ -73,7 +73,7 @@ def test_host_tensors_are_refused():
 DST = dict(x=A, dt=0, ld=1000, N=2, V=1000, ids=A, idt=1, ldi=5, tlp=A, ldt=5, K=5, T=1.0, tail=1, w=A, loss=A, d=A, ldd=1000, ws=A, nws=1 << 20, stream=0)
 
 
-@pytest.mark.parametrize("kw", COMMON[:-1] + [dict(K=0), dict(K=257), dict(ids=None), dict(tlp=None), dict(loss=None), dict(d=None), dict(ldi=4), dict(ldt=4), dict(ldd=999)])
+@pytest.mark.parametrize("kw", COMMON[:-1] + [dict(K=0), dict(K=257), dict(ids=None), dict(tlp=None), dict(loss=None), dict(d=None), dict(ldi=4), dict(ldt=4), dict(ldd=999), dict(N=1 << 23), dict(ldd=1001)])
 def test_distill_train_refuses(kw):
     assert call("mh_distill_topk_train", DST, DST, **kw) == -1
 
