@@ -711,8 +711,10 @@ int32_t mh_sharded_lookup_bwd(mh_comm_t comm, int32_t F, int64_t B, int64_t capa
  * only, [K] floats) receives the column sums of x in a fixed order, from a workspace of ceil(R / 128) * K floats.
  * mh_fp8_matmul: out[M, N] = a b^T + bias, a [M, K] and b [N, K] in that form, bias [N] floats or NULL, out of type out_dtype with leading
  * dimension ldo.  An MH_F32 or MH_F16 output is summed in 32 bits throughout; an MH_BF16 one by the 8-bit matrix instruction, at twice the
- * rate, whose sums are off by at most 7 * 2^-13 of sum |a b| (under half a step of bf16; 1.5e-5 of the norm on random values).  mh_fp8_linear: x [M, K] quantised into the workspace, then the product with w [N, K].
- * K <= 2^24 - 128, leading dimensions of 8-bit values <= 2^24, M, N < 2^27; in MH_F32 and MH_F16 outputs a value under 2^-126 may count as 0.
+ * rate, whose sums are off by at most 7 * 2^-13 of sum |a b| (under half a step of bf16; 1.5e-5 of the norm on random values).
+ * mh_fp8_linear: x [M, K] in the form of mh_fp8_quantize (into the workspace, or on the way for few rows), then the product with w [N, K].
+ * K <= 2^24 - 128, leading dimensions of 8-bit values and scales <= 2^24, M, N < 2^27; workspaces are 16-byte aligned.  In MH_F32 and MH_F16 outputs an
+ * operand's value under 2^-126 may count as 0 and one that rounds to 2^128 is infinite.
  * No atomics: results do not change from call to call.  Rows past M and columns past N of out are left as they were. */
 int32_t mh_fp8_quantize(const void* x, int32_t dtype, int64_t ldx, int64_t R, int64_t K, int32_t transpose, void* q, int64_t ldq,
                         void* scales, int64_t lds, float* colsum, void* workspace, int64_t workspace_bytes, mh_stream_t stream);

@@ -126,12 +126,22 @@ __global__ __launch_bounds__(512) void fp8_quantize_cols_kernel(const T* __restr
     if (cc < C) *reinterpret_cast<uint4*>(q + cc * ldq + rb * 128 + (threadIdx.x % 8) * 16) = *reinterpret_cast<const uint4*>(&tile[threadIdx.x / 8][(threadIdx.x % 8) * 16]);
 }
 
-// out[c] = sum_b part[b, c], in order
-__global__ __launch_bounds__(256) void fp8_colsum_kernel(const float* __restrict__ part, int blocks, int64_t C, float* __restrict__ out) {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c >= C) return;
+// out[c] = sum_b part[b, c]: sixteen wavefronts take every sixteenth b of 64 columns, then their sums in order
+__global__ __launch_bounds__(1024) void fp8_colsum_kernel(const float* __restrict__ part, int blocks, int64_t C, float* __restrict__ out) {
+    __shared__ float red[16][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
     float t = 0.f;
-    for (int b = 0; b < blocks; ++b) t += part[(int64_t)b * C + c];
+    if (c < C) {
+#pragma unroll 8
+        for (int b = w; b < blocks; b += 16) t += part[(int64_t)b * C + c];
+    }
+    red[w][lane] = t;
+    __syncthreads();
+    if (w || c >= C) return;
+    t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t += red[i][lane];
     out[c] = t;
 }
 
@@ -502,6 +512,8 @@ __global__ __launch_bounds__(64 * RW, 2) void fp8_rows_kernel(const F8Args g, co
     auto issue = [&](int kb) {
 #pragma unroll
         for (int j = 0; j < 2 * NB; ++j) f8_dma16(tb + (int64_t)kb * 128 + src[j], stage + (kb & 1) * STAGE + j * 1024);
+        asm volatile("" ::: "memory");  // before a's loads, for multiply() counts on it
+        __builtin_amdgcn_sched_barrier(0);
     };
     const uint8_t *pa[MT], *psa[MT];
     const X* px[MT];
@@ -752,8 +764,8 @@ int32_t f8_check_matrix(const char* who, const char* name, const void* q, int64_
     MH_REQUIRE(rows == 0 || (q && s), "%s: %s is NULL", who, name);
     MH_REQUIRE(ld >= kp && ld % 16 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0,
                "%s: rows of %s must be 16-byte aligned and hold %lld entries (whole blocks of 128)", who, name, (long long)kp);
-    MH_REQUIRE(lds >= mh_ceil_div(kp / 128, 4) * 4 && lds % 4 == 0 && (reinterpret_cast<uintptr_t>(s) & 3) == 0,
-               "%s: rows of the scales of %s must be 4-byte aligned and hold a multiple of four blocks", who, name);
+    MH_REQUIRE(lds >= mh_ceil_div(kp / 128, 4) * 4 && lds % 4 == 0 && lds <= 1 << 24 && (reinterpret_cast<uintptr_t>(s) & 3) == 0,
+               "%s: rows of the scales of %s must be 4-byte aligned, hold a multiple of four blocks and lie at most 2^24 apart", who, name);
     return MH_OK;
 }
 
@@ -783,8 +795,8 @@ int32_t f8_matmul(const char* who, const uint8_t* a, int64_t lda, const uint8_t*
     }
     F8Args t = g;
     if (p.slices > 1) {
-        if (ws_bytes < f8_part_bytes(M, N, K) || !ws) {
-            mh_set_error("%s: workspace too small (%lld bytes)", who, (long long)ws_bytes);
+        if (ws_bytes < f8_part_bytes(M, N, K) || !ws || (reinterpret_cast<uintptr_t>(ws) & 15)) {
+            mh_set_error("%s: workspace too small or not 16-byte aligned (%lld bytes)", who, (long long)ws_bytes);
             return MH_ERR_WORKSPACE;
         }
         g.slab = t.slab = M * N;
@@ -856,7 +868,7 @@ int32_t mh_fp8_quantize(const void* x, int32_t dtype, int64_t ldx, int64_t R, in
     else if (dtype == MH_BF16) rc = f8_quantize(static_cast<const lp_bf16*>(x), ldx, R, K, transpose != 0, qq, ldq, ss, lds, part, s);
     else rc = f8_quantize(static_cast<const lp_f16*>(x), ldx, R, K, transpose != 0, qq, ldq, ss, lds, part, s);
     if (rc == MH_OK && colsum) {
-        MH_LAUNCH(fp8_colsum_kernel, dim3((unsigned)mh_ceil_div(K, 256)), dim3(256), 0, s, (const float*)part, (int)rb, K, colsum);
+        MH_LAUNCH(fp8_colsum_kernel, dim3((unsigned)mh_ceil_div(K, 64)), dim3(1024), 0, s, (const float*)part, (int)rb, K, colsum);
         MH_CHECK_LAUNCH("mh_fp8_quantize");
     }
     return rc;
@@ -900,8 +912,8 @@ int32_t mh_fp8_linear(const void* x, int32_t x_dtype, int64_t ldx, const void* w
         MH_CHECK_LAUNCH("mh_fp8_linear");
         return MH_OK;
     }
-    if (!workspace || workspace_bytes < mh_fp8_linear_workspace_bytes(M, N, K)) {
-        mh_set_error("mh_fp8_linear: workspace too small (%lld bytes)", (long long)workspace_bytes);
+    if (!workspace || workspace_bytes < mh_fp8_linear_workspace_bytes(M, N, K) || (reinterpret_cast<uintptr_t>(workspace) & 15)) {
+        mh_set_error("mh_fp8_linear: workspace too small or not 16-byte aligned (%lld bytes)", (long long)workspace_bytes);
         return MH_ERR_WORKSPACE;
     }
     uint8_t* q = static_cast<uint8_t*>(workspace);

@@ -34,7 +34,8 @@ def test_quantize_needs_its_workspace_for_column_sums():
 
 @pytest.mark.parametrize("kw", [dict(a=None), dict(sb=None), dict(lda=240), dict(ldb=128), dict(ldsa=3), dict(dt=7), dict(ldo=7), dict(out=None), dict(K=0),
                                 dict(M=-1), dict(b=A + 4), dict(ldsb=0), dict(M=1 << 27), dict(N=1 << 27, ldo=1 << 27), dict(M=1 << 26, N=1 << 20, ldo=1 << 20),
-                                dict(K=1 << 24, lda=1 << 24, ldb=1 << 24, ldsa=1 << 17, ldsb=1 << 17), dict(lda=(1 << 24) + 16)])
+                                dict(K=1 << 24, lda=1 << 24, ldb=1 << 24, ldsa=1 << 17, ldsb=1 << 17), dict(lda=(1 << 24) + 16), dict(ldsa=(1 << 24) + 4),
+                                dict(ldsb=1 << 30)])
 def test_matmul_refuses(kw):
     assert matmul(**kw) == -1
 
@@ -43,6 +44,7 @@ def test_matmul_needs_its_workspace_where_the_sum_is_cut():
     need = _lib.load().mh_fp8_matmul_workspace_bytes(128, 128, 8192)
     assert need > 0
     assert matmul(M=128, N=128, K=8192, lda=8192, ldb=8192, ldsa=64, ldsb=64, ldo=128, ws=A, nws=need - 1) == -4
+    assert matmul(M=128, N=128, K=8192, lda=8192, ldb=8192, ldsa=64, ldsb=64, ldo=128, ws=A + 8, nws=need + 8) == -4
 
 
 def test_nothing_to_do_is_no_error():

@@ -209,6 +209,16 @@ def test_nan_and_infinity_stay_in_their_row(device, M, out):
     assert torch.equal(got[rows], want[rows])
 
 
+@pytest.mark.parametrize("R,C", [(1, 1), (127, 65), (128 * 17, 64), (128 * 40 + 5, 300)])
+def test_column_sums(device, R, C):
+    x = torch.randn(R, C, generator=torch.Generator(device=device).manual_seed(R), device=device)
+    m, sums = ops.fp8_quantize(x, transpose=True, column_sums=True)
+    assert torch.equal(m.values.view(torch.uint8), ops.fp8_quantize(x, transpose=True).values.view(torch.uint8))
+    # 24 additions within a block (16, then 8), one for each sixteenth block, then 16: each rounds by 2^-24 of sum |x| at most
+    tol = (24 + -(-R // 2048) + 16) * 2.0 ** -24 * x.double().abs().sum(0)
+    assert ((sums.double() - x.double().sum(0)).abs() <= tol).all()
+
+
 def test_wide_range_of_scales(device):
     """Blocks of very small and very large entries: what the product of the scales brings back into range is right."""
     rng = np.random.default_rng(8)
