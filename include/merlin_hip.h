@@ -709,6 +709,7 @@ int32_t mh_sharded_lookup_bwd(mh_comm_t comm, int32_t F, int64_t B, int64_t capa
  * block (at least -126; 0 for a block of zeros), values rounded to nearest, ties to even; an infinity or NaN becomes NaN and does not
  * enter the scale.  transpose != 0: the matrix stored is x^T -- K rows of R columns, blocks along the rows of x; colsum (optional, then
  * only, [K] floats) receives the column sums of x in a fixed order, from a workspace of ceil(R / 128) * K floats.
+ * mh_fp8_quantize_both: both forms from one read -- q / scales as with transpose = 0, qt / scales_t (and colsum) as with transpose = 1.
  * mh_fp8_matmul: out[M, N] = a b^T + bias, a [M, K] and b [N, K] in that form, bias [N] floats or NULL, out of type out_dtype with leading
  * dimension ldo.  An MH_F32 or MH_F16 output is summed in 32 bits throughout; an MH_BF16 one by the 8-bit matrix instruction, at twice the
  * rate, whose sums are off by at most 7 * 2^-13 of sum |a b| (under half a step of bf16; 1.5e-5 of the norm on random values).
@@ -718,6 +719,9 @@ int32_t mh_sharded_lookup_bwd(mh_comm_t comm, int32_t F, int64_t B, int64_t capa
  * No atomics: results do not change from call to call.  Rows past M and columns past N of out are left as they were. */
 int32_t mh_fp8_quantize(const void* x, int32_t dtype, int64_t ldx, int64_t R, int64_t K, int32_t transpose, void* q, int64_t ldq,
                         void* scales, int64_t lds, float* colsum, void* workspace, int64_t workspace_bytes, mh_stream_t stream);
+int32_t mh_fp8_quantize_both(const void* x, int32_t dtype, int64_t ldx, int64_t R, int64_t K, void* q, int64_t ldq, void* scales, int64_t lds,
+                             void* qt, int64_t ldqt, void* scales_t, int64_t ldst, float* colsum, void* workspace, int64_t workspace_bytes,
+                             mh_stream_t stream);
 int64_t mh_fp8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int32_t mh_fp8_matmul(const void* a, int64_t lda, const void* a_scales, int64_t ldas, const void* b, int64_t ldb, const void* b_scales,
                       int64_t ldbs, int64_t M, int64_t N, int64_t K, const float* bias, int32_t out_dtype, void* out, int64_t ldo,

@@ -115,6 +115,7 @@ SIGNATURES = {
     "mh_bce_mean_fwd_bwd": (_i32, [_p, _p, _i64, _f32, _p, _p, _p, _p]),
     "mh_mean": (_i32, [_p, _i64, _p, _p, _p]),
     "mh_fp8_quantize": (_i32, [_p, _i32, _i64, _i64, _i64, _i32, _p, _i64, _p, _i64, _p, _p, _i64, _p]),
+    "mh_fp8_quantize_both": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _p]),
     "mh_fp8_matmul_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "mh_fp8_matmul": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _i32, _p, _i64, _p, _i64, _p]),
     "mh_fp8_linear_workspace_bytes": (_i64, [_i64, _i64, _i64]),

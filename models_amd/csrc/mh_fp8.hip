@@ -20,28 +20,43 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 // ---- quantiser -----------------------------------------------------------------------------------------------------------------------
-// The scale's exponent from the block's largest magnitude: amax = 1.f 2^(E - 127) <= 448 2^e = 1.75 2^(8 + e) for e = E - 135, one more where
+// The scale's exponent from the bits of the block's largest magnitude: amax = 1.f 2^(E - 127) <= 448 2^e = 1.75 2^(8 + e) for e = E - 135, one more where
 // 1.f > 1.75.  -126 below keeps 2^e and 2^-e normal numbers.
-__device__ __forceinline__ int q_exponent(float amax) {
-    const uint32_t b = __float_as_uint(amax);
+__device__ __forceinline__ int q_exponent(uint32_t b) {
     if (b == 0) return 0;
     const int e = (int)(b >> 23) - 135 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
     return e < -126 ? -126 : e;
 }
 __device__ __forceinline__ float q_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
-// |v| where v is finite, else 0: an infinity or NaN becomes NaN in e4m3 and leaves its block's scale to the others
-__device__ __forceinline__ float q_mag(float v) {
-    const float a = fabsf(v);
-    return a <= 3.402823466e38f ? a : 0.f;
+// An infinity or NaN becomes NaN in e4m3 and leaves its block's scale to the others.  Magnitudes are compared as bits, an AND and half a three-way
+// maximum each, and whether a wavefront holds such a value is seen from the largest: only then are they looked at one by one (q_clean first, with
+// which the conversion needs no care for them, then q_bits<true>).
+constexpr uint32_t Q_INF = 0x7f800000u;
+template <bool ODD>
+__device__ __forceinline__ uint32_t q_bits(float v) {
+    const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+    return ODD && b >= Q_INF ? 0u : b;
 }
-__device__ __forceinline__ float q_in(float v) { return fabsf(v) <= 3.402823466e38f ? v : __uint_as_float(0x7fc00000u); }
+__device__ __forceinline__ uint32_t q_max(uint32_t a, uint32_t b) { return a > b ? a : b; }
+template <bool ODD, int N>
+__device__ __forceinline__ uint32_t q_most(const float (&v)[N]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = q_max(m, q_bits<ODD>(v[i]));
+    return m;
+}
+template <int N>
+__device__ __forceinline__ void q_clean(float (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = q_bits<false>(v[i]) >= Q_INF ? __uint_as_float(0x7fc00000u) : v[i];
+}
 __device__ __forceinline__ uint32_t q_pack4(float a, float b, float c, float d) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(q_in(a), q_in(b), 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q_in(c), q_in(d), w, true);
+    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
 }
 
 // Blocks along the rows of x.  A wavefront takes four blocks (512 entries, 8 a lane: 16 lanes share a block) of one row and writes one word of
-// scales; one pass, bound by its reads.
+// scales; one pass, bound by its reads and writes: 65536 x 3341 fp32 185 us, 5.9 TB/s; 65536 x 512 24 us, 7.0 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void fp8_quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t R, int K, int quads, uint8_t* __restrict__ q,
                                                                int64_t ldq, uint8_t* __restrict__ s, int64_t lds) {
@@ -58,11 +73,13 @@ __global__ __launch_bounds__(256) void fp8_quantize_rows_kernel(const T* __restr
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = k + i < K ? lp_float(p[i]) : 0.f;
     }
-    float a = 0.f;
+    uint32_t a = q_most<false>(v);
+    if (__any(a >= Q_INF)) {
+        q_clean(v);
+        a = q_most<true>(v);
+    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) a = fmaxf(a, q_mag(v[i]));
-#pragma unroll
-    for (int m = 8; m; m >>= 1) a = fmaxf(a, __shfl_xor(a, m));
+    for (int m = 8; m; m >>= 1) a = q_max(a, __shfl_xor(a, m));
     const int e = q_exponent(a);
     const float inv = q_pow2(-e);
     const int kp = (K + 127) / 128 * 128;
@@ -78,52 +95,119 @@ __global__ __launch_bounds__(256) void fp8_quantize_rows_kernel(const T* __restr
     if (lane == 0) *reinterpret_cast<uint32_t*>(s + row * lds + quad * 4) = sw;
 }
 
-// Blocks along the columns of x: q[c, r] = x[r, c].  A workgroup takes 128 rows x 64 columns; a wavefront reads 16 rows, whole lines, and the
-// tile turns round in LDS so that eight lanes write one 128-byte line of q.  colsum, if given, receives the tile's column sums ([blocks, C]).
-template <typename T>
-__global__ __launch_bounds__(512) void fp8_quantize_cols_kernel(const T* __restrict__ x, int64_t ldx, int64_t R, int64_t C, int rblocks, int sbytes,
-                                                               uint8_t* __restrict__ q, int64_t ldq, uint8_t* __restrict__ s, int64_t lds,
-                                                               float* __restrict__ colsum) {
-    __shared__ float red[8][64], red2[8][64];
-    __shared__ __attribute__((aligned(16))) uint8_t tile[64][144];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int rb = (int)(blockIdx.x % (uint32_t)rblocks);
-    const int64_t c0 = (int64_t)(blockIdx.x / (uint32_t)rblocks) * 64, c = c0 + lane;
-    const int64_t r0 = (int64_t)rb * 128 + w * 16;
-    float v[16], a = 0.f, t = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = (c < C && r0 + i < R) ? lp_float(x[(r0 + i) * ldx + c]) : 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        a = fmaxf(a, q_mag(v[i]));
-        t += v[i];
-    }
-    red[w][lane] = a;
-    red2[w][lane] = t;
-    __syncthreads();
-    t = 0.f;
+// Blocks along the columns of x: qt[c, r] = x[r, c], and with ROWS those along its rows from the same read.  A workgroup takes 128 x 128; a lane holds
+// eight rows of four columns.  The rows' maxima meet by halves -- 4, 2, 1 values, then two more steps -- which leaves row i's with lanes 4 i to
+// 4 i + 3 of its half wavefront; the columns' meet in LDS.  The tile turns round in LDS so that eight lanes write one 128-byte line of qt; sixteen
+// bytes chunk h of column c lie at h ^ ((c >> 2) & 7), or all 32 lanes of a write would meet in two banks.  colsum, if given, receives the tile's column
+// sums ([blocks, C]).  Bound by memory: 65536 x 512 fp32 26 us, 6.5 TB/s, and 33 us with ROWS (6.1 TB/s; the two forms apart 50); 65536 x 3341, whose rows
+// start at any word, 227 us, 4.8 TB/s.  Single columns in place of four neighbouring ones a lane took 26 us for 16384 x 1024, 16 now; the order of the
+// tiles made no difference.
+template <typename T, bool ROWS>
+__global__ __launch_bounds__(512) void fp8_quantize_tiles_kernel(const T* __restrict__ x, int64_t ldx, int64_t R, int64_t C, int cblocks, int rblocks,
+                                                                uint8_t* __restrict__ q, int64_t ldq, uint8_t* __restrict__ s, int64_t lds,
+                                                                uint8_t* __restrict__ qt, int64_t ldqt, uint8_t* __restrict__ st, int64_t ldst,
+                                                                float* __restrict__ colsum) {
+    __shared__ __attribute__((aligned(16))) uint32_t most[8][128];
+    __shared__ __attribute__((aligned(16))) float sums[8][128];
+    __shared__ __attribute__((aligned(16))) uint8_t tile[128][128];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, half = lane >> 5, c4 = (lane & 31) * 4;
+    const int cb = (int)(blockIdx.x % (uint32_t)cblocks), rb = (int)(blockIdx.x / (uint32_t)cblocks);
+    const int64_t c = (int64_t)cb * 128 + c4, r0 = (int64_t)rb * 128 + w * 16 + half * 8;
+    float v[8][4];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        a = fmaxf(a, red[i][lane]);
-        t += red2[i][lane];
+        const T* p = x + (r0 + i) * ldx + c;
+        if (r0 + i < R && c + 4 <= C) {
+            lp_load4(p, v[i]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[i][j] = r0 + i < R && c + j < C ? lp_float(p[j]) : 0.f;
+        }
     }
-    const int e = q_exponent(a);
-    const float inv = q_pow2(-e);
-    uint4 o;
-    o.x = q_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-    o.y = q_pack4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
-    o.z = q_pack4(v[8] * inv, v[9] * inv, v[10] * inv, v[11] * inv);
-    o.w = q_pack4(v[12] * inv, v[13] * inv, v[14] * inv, v[15] * inv);
-    *reinterpret_cast<uint4*>(&tile[lane][w * 16]) = o;
-    if (w == 0 && c < C) {
-        s[c * lds + rb] = (uint8_t)(e + 127);
-        if (rb == rblocks - 1)
-            for (int b = rblocks; b < sbytes; ++b) s[c * lds + b] = 127;
-        if (colsum) colsum[(int64_t)rb * C + c] = t;
+    if (colsum) {
+        f32x4 t = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t[j] += v[i][j];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t[j] += __shfl_xor(t[j], 32);
+        if (half == 0) *reinterpret_cast<f32x4*>(&sums[w][c4]) = t;
+    }
+    uint32_t a[4] = {0, 0, 0, 0}, m[8];
+    auto maxima = [&](auto odd) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            m[i] = q_most<decltype(odd)::value>(v[i]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) a[j] = q_max(i ? a[j] : 0, q_bits<decltype(odd)::value>(v[i][j]));
+        }
+    };
+    maxima(std::false_type{});
+    if (__any(q_max(q_max(a[0], a[1]), q_max(a[2], a[3])) >= Q_INF)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q_clean(v[i]);
+        maxima(std::true_type{});
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a[j] = q_max(a[j], __shfl_xor(a[j], 32));
+    if (half == 0) *reinterpret_cast<uint4*>(&most[w][c4]) = make_uint4(a[0], a[1], a[2], a[3]);
+    if (ROWS) {
+#pragma unroll
+        for (int n = 4; n; n >>= 1)
+#pragma unroll
+            for (int i = 0; i < n; ++i) {
+                const bool up = lane & (4 * n);
+                const uint32_t keep = up ? m[n + i] : m[i], give = up ? m[i] : m[n + i];
+                m[i] = q_max(keep, __shfl_xor(give, 4 * n));
+            }
+        m[0] = q_max(m[0], __shfl_xor(m[0], 2));
+        m[0] = q_max(m[0], __shfl_xor(m[0], 1));
+        const int e = q_exponent(m[0]), mine = (lane >> 2) & 7;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float inv = q_pow2(-__shfl(e, (lane & 32) + 4 * i));
+            if (r0 + i < R) *reinterpret_cast<uint32_t*>(q + (r0 + i) * ldq + c) = q_pack4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
+        }
+        if ((lane & 3) == 0 && r0 + mine < R) {
+            s[(r0 + mine) * lds + cb] = (uint8_t)(e + 127);
+            if (cb == cblocks - 1)
+                for (int b = cblocks; b & 3; ++b) s[(r0 + mine) * lds + b] = 127;
+        }
     }
     __syncthreads();
-    const int64_t cc = c0 + threadIdx.x / 8;
-    if (cc < C) *reinterpret_cast<uint4*>(q + cc * ldq + rb * 128 + (threadIdx.x % 8) * 16) = *reinterpret_cast<const uint4*>(&tile[threadIdx.x / 8][(threadIdx.x % 8) * 16]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint4 o = *reinterpret_cast<const uint4*>(&most[i][c4]);
+        a[0] = q_max(a[0], o.x), a[1] = q_max(a[1], o.y), a[2] = q_max(a[2], o.z), a[3] = q_max(a[3], o.w);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int e = q_exponent(a[j]);
+        const float inv = q_pow2(-e);
+        uint2 o;
+        o.x = q_pack4(v[0][j] * inv, v[1][j] * inv, v[2][j] * inv, v[3][j] * inv);
+        o.y = q_pack4(v[4][j] * inv, v[5][j] * inv, v[6][j] * inv, v[7][j] * inv);
+        *reinterpret_cast<uint2*>(&tile[c4 + j][((w ^ (lane & 7)) << 4) + half * 8]) = o;
+        if (w == 0 && half == 0 && c + j < C) {
+            st[(c + j) * ldst + rb] = (uint8_t)(e + 127);
+            if (rb == rblocks - 1)
+                for (int b = rblocks; b & 3; ++b) st[(c + j) * ldst + b] = 127;
+        }
+    }
+    if (colsum && threadIdx.x < 128 && (int64_t)cb * 128 + threadIdx.x < C) {
+        float u = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u += sums[i][threadIdx.x];
+        colsum[(int64_t)rb * C + cb * 128 + threadIdx.x] = u;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int col = i * 64 + threadIdx.x / 8, h = threadIdx.x & 7;
+        const int64_t cc = (int64_t)cb * 128 + col;
+        if (cc < C) *reinterpret_cast<uint4*>(qt + cc * ldqt + (int64_t)rb * 128 + h * 16) = *reinterpret_cast<const uint4*>(&tile[col][(h ^ ((col >> 2) & 7)) << 4]);
+    }
 }
 
 // out[c] = sum_b part[b, c]: sixteen wavefronts take every sixteenth b of 64 columns, then their sums in order
@@ -404,12 +488,14 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_gemm_kernel(const F8Args 
 }
 
 // 32 entries as 8-bit values and their scale's byte: the quantiser's own rule, the four lanes that share a block and a row agreeing on it
-__device__ __forceinline__ i32x8 f8_quantize32(const float (&v)[32], uint32_t& scale) {
-    float a = 0.f;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) a = fmaxf(a, q_mag(v[i]));
-    a = fmaxf(a, __shfl_xor(a, 16));
-    a = fmaxf(a, __shfl_xor(a, 32));
+__device__ __forceinline__ i32x8 f8_quantize32(float (&v)[32], uint32_t& scale) {
+    uint32_t a = q_most<false>(v);
+    if (__any(a >= Q_INF)) {
+        q_clean(v);
+        a = q_most<true>(v);
+    }
+    a = q_max(a, __shfl_xor(a, 16));
+    a = q_max(a, __shfl_xor(a, 32));
     const int e = q_exponent(a);
     const float inv = q_pow2(-e);
     scale = (uint32_t)(e + 127);
@@ -813,19 +899,43 @@ int32_t f8_matmul(const char* who, const uint8_t* a, int64_t lda, const uint8_t*
 }
 
 template <typename T>
-int32_t f8_quantize(const T* x, int64_t ldx, int64_t R, int64_t K, bool transpose, uint8_t* q, int64_t ldq, uint8_t* sc, int64_t lds, float* colsum,
-                    hipStream_t s) {
-    if (!transpose) {
-        const int64_t quads = mh_ceil_div(mh_ceil_div(K, 128), 4), blocks = mh_ceil_div(R, 4) * quads;
-        MH_REQUIRE(blocks < (int64_t)1 << 24, "mh_fp8_quantize: matrix too large for one launch (2^32 threads)");
-        MH_LAUNCH(fp8_quantize_rows_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, x, ldx, R, (int)K, (int)quads, q, ldq, sc, lds);
-    } else {
-        const int64_t rb = mh_ceil_div(R, 128), blocks = rb * mh_ceil_div(K, 64);
-        MH_REQUIRE(blocks < (int64_t)1 << 23, "mh_fp8_quantize: matrix too large for one launch (2^32 threads)");
-        MH_LAUNCH(fp8_quantize_cols_kernel<T>, dim3((unsigned)blocks), dim3(512), 0, s, x, ldx, R, K, (int)rb, (int)(mh_ceil_div(rb, 4) * 4), q, ldq, sc, lds,
-                  colsum);
-    }
+int32_t f8_quantize_rows(const T* x, int64_t ldx, int64_t R, int64_t K, uint8_t* q, int64_t ldq, uint8_t* sc, int64_t lds, hipStream_t s) {
+    const int64_t quads = mh_ceil_div(mh_ceil_div(K, 128), 4), blocks = mh_ceil_div(R, 4) * quads;
+    MH_REQUIRE(blocks < (int64_t)1 << 24, "mh_fp8_quantize: matrix too large for one launch (2^32 threads)");
+    MH_LAUNCH(fp8_quantize_rows_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, x, ldx, R, (int)K, (int)quads, q, ldq, sc, lds);
     MH_CHECK_LAUNCH("mh_fp8_quantize");
+    return MH_OK;
+}
+
+// q NULL: the columns' form alone
+template <typename T>
+int32_t f8_quantize_tiles(const char* who, const T* x, int64_t ldx, int64_t R, int64_t C, uint8_t* q, int64_t ldq, uint8_t* sc, int64_t lds, uint8_t* qt,
+                          int64_t ldqt, uint8_t* st, int64_t ldst, float* colsum, float* part, hipStream_t s) {
+    const int64_t rb = mh_ceil_div(R, 128), cb = mh_ceil_div(C, 128);
+    MH_REQUIRE(rb * cb < (int64_t)1 << 23, "%s: matrix too large for one launch (2^32 threads)", who);
+    if (!colsum) part = nullptr;
+    if (q) MH_LAUNCH((fp8_quantize_tiles_kernel<T, true>), dim3((unsigned)(rb * cb)), dim3(512), 0, s, x, ldx, R, C, (int)cb, (int)rb, q, ldq, sc, lds, qt, ldqt, st, ldst, part);
+    else MH_LAUNCH((fp8_quantize_tiles_kernel<T, false>), dim3((unsigned)(rb * cb)), dim3(512), 0, s, x, ldx, R, C, (int)cb, (int)rb, q, ldq, sc, lds, qt, ldqt, st, ldst, part);
+    MH_CHECK_LAUNCH(who);
+    if (colsum) {
+        MH_LAUNCH(fp8_colsum_kernel, dim3((unsigned)mh_ceil_div(C, 64)), dim3(1024), 0, s, (const float*)part, (int)rb, C, colsum);
+        MH_CHECK_LAUNCH(who);
+    }
+    return MH_OK;
+}
+
+int32_t f8_check_source(const char* who, const void* x, int32_t dtype, int64_t ldx, int64_t R, int64_t K) {
+    MH_REQUIRE(R >= 0 && K >= 0 && R < (int64_t)1 << 31 && K < (int64_t)1 << 31 && ldx >= K, "%s: sizes R=%lld K=%lld ldx=%lld", who, (long long)R,
+               (long long)K, (long long)ldx);
+    MH_REQUIRE(dtype == MH_F32 || dtype == MH_BF16 || dtype == MH_F16, "%s: unknown type %d", who, (int)dtype);
+    MH_REQUIRE(x || R == 0 || K == 0, "%s: x is NULL", who);
+    return MH_OK;
+}
+int32_t f8_check_sums(const char* who, const float* colsum, const void* ws, int64_t bytes, int64_t R, int64_t K) {
+    if (colsum && (!ws || bytes < mh_ceil_div(R, 128) * K * 4 || (reinterpret_cast<uintptr_t>(ws) & 3))) {
+        mh_set_error("%s: workspace too small or not aligned (%lld bytes)", who, (long long)bytes);
+        return MH_ERR_WORKSPACE;
+    }
     return MH_OK;
 }
 
@@ -847,31 +957,39 @@ extern "C" {
 
 int32_t mh_fp8_quantize(const void* x, int32_t dtype, int64_t ldx, int64_t R, int64_t K, int32_t transpose, void* q, int64_t ldq, void* scales,
                         int64_t lds, float* colsum, void* workspace, int64_t workspace_bytes, mh_stream_t stream) {
-    const int64_t rows = transpose ? K : R, len = transpose ? R : K;
-    MH_REQUIRE(R >= 0 && K >= 0 && R < (int64_t)1 << 31 && K < (int64_t)1 << 31 && ldx >= K, "mh_fp8_quantize: sizes R=%lld K=%lld ldx=%lld", (long long)R,
-               (long long)K, (long long)ldx);
-    MH_REQUIRE(dtype == MH_F32 || dtype == MH_BF16 || dtype == MH_F16, "mh_fp8_quantize: unknown type %d", (int)dtype);
+    const char* const who = "mh_fp8_quantize";
+    if (int32_t rc = f8_check_source(who, x, dtype, ldx, R, K)) return rc;
     MH_REQUIRE(!colsum || transpose, "mh_fp8_quantize: column sums come with transpose only");
-    if (rows == 0 || len == 0) return MH_OK;
-    MH_REQUIRE(x, "mh_fp8_quantize: x is NULL");
-    if (int32_t rc = f8_check_matrix("mh_fp8_quantize", "q", q, ldq, scales, lds, rows, len)) return rc;
-    const int64_t rb = mh_ceil_div(R, 128);
-    if (colsum && (!workspace || workspace_bytes < rb * K * 4)) {
-        mh_set_error("mh_fp8_quantize: workspace too small (%lld bytes)", (long long)workspace_bytes);
-        return MH_ERR_WORKSPACE;
-    }
+    if (R == 0 || K == 0) return MH_OK;
+    if (int32_t rc = f8_check_matrix(who, "q", q, ldq, scales, lds, transpose ? K : R, transpose ? R : K)) return rc;
+    if (int32_t rc = f8_check_sums(who, colsum, workspace, workspace_bytes, R, K)) return rc;
     hipStream_t s = mh_stream(stream);
     uint8_t *qq = static_cast<uint8_t*>(q), *ss = static_cast<uint8_t*>(scales);
-    float* part = colsum ? static_cast<float*>(workspace) : nullptr;
-    int32_t rc;
-    if (dtype == MH_F32) rc = f8_quantize(static_cast<const float*>(x), ldx, R, K, transpose != 0, qq, ldq, ss, lds, part, s);
-    else if (dtype == MH_BF16) rc = f8_quantize(static_cast<const lp_bf16*>(x), ldx, R, K, transpose != 0, qq, ldq, ss, lds, part, s);
-    else rc = f8_quantize(static_cast<const lp_f16*>(x), ldx, R, K, transpose != 0, qq, ldq, ss, lds, part, s);
-    if (rc == MH_OK && colsum) {
-        MH_LAUNCH(fp8_colsum_kernel, dim3((unsigned)mh_ceil_div(K, 64)), dim3(1024), 0, s, (const float*)part, (int)rb, K, colsum);
-        MH_CHECK_LAUNCH("mh_fp8_quantize");
-    }
-    return rc;
+    auto run = [&](auto* p) {
+        return transpose ? f8_quantize_tiles(who, p, ldx, R, K, nullptr, 0, nullptr, 0, qq, ldq, ss, lds, colsum, static_cast<float*>(workspace), s)
+                         : f8_quantize_rows(p, ldx, R, K, qq, ldq, ss, lds, s);
+    };
+    if (dtype == MH_F32) return run(static_cast<const float*>(x));
+    if (dtype == MH_BF16) return run(static_cast<const lp_bf16*>(x));
+    return run(static_cast<const lp_f16*>(x));
+}
+
+int32_t mh_fp8_quantize_both(const void* x, int32_t dtype, int64_t ldx, int64_t R, int64_t K, void* q, int64_t ldq, void* scales, int64_t lds, void* qt,
+                             int64_t ldqt, void* scales_t, int64_t ldst, float* colsum, void* workspace, int64_t workspace_bytes, mh_stream_t stream) {
+    const char* const who = "mh_fp8_quantize_both";
+    if (int32_t rc = f8_check_source(who, x, dtype, ldx, R, K)) return rc;
+    if (R == 0 || K == 0) return MH_OK;
+    if (int32_t rc = f8_check_matrix(who, "q", q, ldq, scales, lds, R, K)) return rc;
+    if (int32_t rc = f8_check_matrix(who, "qt", qt, ldqt, scales_t, ldst, K, R)) return rc;
+    if (int32_t rc = f8_check_sums(who, colsum, workspace, workspace_bytes, R, K)) return rc;
+    hipStream_t s = mh_stream(stream);
+    auto run = [&](auto* p) {
+        return f8_quantize_tiles(who, p, ldx, R, K, static_cast<uint8_t*>(q), ldq, static_cast<uint8_t*>(scales), lds, static_cast<uint8_t*>(qt), ldqt,
+                                 static_cast<uint8_t*>(scales_t), ldst, colsum, static_cast<float*>(workspace), s);
+    };
+    if (dtype == MH_F32) return run(static_cast<const float*>(x));
+    if (dtype == MH_BF16) return run(static_cast<const lp_bf16*>(x));
+    return run(static_cast<const lp_f16*>(x));
 }
 
 int64_t mh_fp8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K) { return M > 0 && N > 0 && K > 0 ? f8_part_bytes(M, N, K) : 0; }

@@ -82,6 +82,18 @@ __device__ __forceinline__ void lp_load8(const T* p, float (&v)[8]) {
     lp_unpack(lp_load16(p), v, p);
 }
 
+// four entries
+typedef uint32_t lp_u2_at2 __attribute__((ext_vector_type(2), aligned(2)));
+__device__ __forceinline__ void lp_load4(const float* p, float (&v)[4]) { lp_unpack(lp_load16(p), v, p); }
+template <typename T>
+__device__ __forceinline__ void lp_load4(const T* p, float (&v)[4]) {
+    const lp_u2_at2 w = *reinterpret_cast<const lp_u2_at2*>(p);
+    float u[8];
+    lp_unpack(make_uint4(w.x, w.y, 0, 0), u, p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = u[i];
+}
+
 // the sixteen bytes of lp_vec<T>::N rounded values
 __device__ __forceinline__ void lp_store16(float* p, const float (&v)[4]) {
     lp_u4_at4 w = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};

@@ -24,6 +24,7 @@ __all__ = [
     "dot_interaction",
     "Fp8Matrix",
     "fp8_quantize",
+    "fp8_quantize_both",
     "fp8_matmul",
     "fp8_linear",
     "fp8_linear_backward",
@@ -2217,6 +2218,12 @@ def _fp8_check(m: Fp8Matrix, name: str) -> Tuple[int, int]:
     return vs[0], K
 
 
+def _fp8_empty(rows: int, cols: int, device) -> Fp8Matrix:
+    kb = -(-cols // _FP8_BLOCK)
+    return Fp8Matrix(torch.empty((rows, kb * _FP8_BLOCK), dtype=torch.float8_e4m3fn, device=device),
+                     torch.empty((rows, -(-kb // 4) * 4), dtype=torch.uint8, device=device), cols)
+
+
 def fp8_quantize(x: torch.Tensor, transpose: bool = False, column_sums: bool = False):
     """``x`` [R, K] (float32 / bfloat16 / float16) as an ``Fp8Matrix``: e4m3 values with one power-of-two scale for each row and each block
     of 128 columns.  ``transpose=True``: the 8-bit form of ``x`` transposed (blocks of 128 along the rows of x), which is how the Keras kernel
@@ -2233,18 +2240,37 @@ def fp8_quantize(x: torch.Tensor, transpose: bool = False, column_sums: bool = F
     if _elsewhere(x):
         with torch.cuda.device(x.device):
             return fp8_quantize(x, transpose, column_sums)
-    kb = -(-cols // _FP8_BLOCK)
-    q = torch.empty((rows, kb * _FP8_BLOCK), dtype=torch.float8_e4m3fn, device=x.device)
-    s = torch.empty((rows, -(-kb // 4) * 4), dtype=torch.uint8, device=x.device)
+    m = q, s, _ = _fp8_empty(rows, cols, x.device)
     sums = torch.empty((K,), dtype=torch.float32, device=x.device) if column_sums else None
     if rows:
-        need = 4 * kb * K if column_sums else 0
+        need = 4 * -(-R // _FP8_BLOCK) * K if column_sums else 0
         ws = _scratch(need, x)
         with _if_timed("fp8_quantize", R * K * (x.element_size() + 1)):
             check(lib.mh_fp8_quantize(x.data_ptr(), dt, _ld(x), R, K, int(transpose), q.data_ptr(), q.shape[1], s.data_ptr(), s.shape[1],
                                       _at(sums), _at(ws), need, _here()), "mh_fp8_quantize")
-    m = Fp8Matrix(q, s, cols)
     return (m, sums) if column_sums else m
+
+
+def fp8_quantize_both(x: torch.Tensor, column_sums: bool = False):
+    """``(fp8_quantize(x), fp8_quantize(x, transpose=True))`` from one read of ``x`` -- what a gradient needs that enters two products -- and the
+    column sums of x third with ``column_sums=True``."""
+    lib = _lib.load()
+    dt = _float_2d(x, "x")
+    R, K = x.shape
+    if R < 1 or K < 1:
+        raise ValueError(f"fp8_quantize_both needs at least one entry along the blocks, got shape {tuple(x.shape)}")
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return fp8_quantize_both(x, column_sums)
+    m = q, s, _ = _fp8_empty(R, K, x.device)
+    mt = qt, st, _ = _fp8_empty(K, R, x.device)
+    sums = torch.empty((K,), dtype=torch.float32, device=x.device) if column_sums else None
+    need = 4 * -(-R // _FP8_BLOCK) * K if column_sums else 0
+    ws = _scratch(need, x)
+    with _if_timed("fp8_quantize_both", R * K * (x.element_size() + 2)):
+        check(lib.mh_fp8_quantize_both(x.data_ptr(), dt, _ld(x), R, K, q.data_ptr(), q.shape[1], s.data_ptr(), s.shape[1], qt.data_ptr(), qt.shape[1],
+                                       st.data_ptr(), st.shape[1], _at(sums), _at(ws), need, _here()), "mh_fp8_quantize_both")
+    return (m, mt, sums) if column_sums else (m, mt)
 
 
 def _fp8_out(M: int, N: int, out: Optional[torch.Tensor], out_dtype, device) -> torch.Tensor:
@@ -2333,15 +2359,23 @@ def fp8_linear_backward(x: torch.Tensor, w: Fp8Matrix, dy: torch.Tensor, need_dx
     if _elsewhere(x, dy, w.values if need_dx else None):
         with torch.cuda.device(x.device):
             return fp8_linear_backward(x, w, dy, need_dx, need_dw, need_db)
-    if need_dx:
-        dx = fp8_matmul(fp8_quantize(dy), w)
     if M == 0:
+        dx = torch.empty((0, K), dtype=torch.float32, device=x.device) if need_dx else None
         dw = torch.zeros((K, N), dtype=torch.float32, device=x.device) if need_dw else None
         db = torch.zeros((N,), dtype=torch.float32, device=x.device) if need_db else None
-    elif need_dw or need_db:
-        dyt = fp8_quantize(dy, transpose=True, column_sums=need_db)
-        if need_db:
-            dyt, db = dyt
+    else:
+        dyq = dyt = None
+        if need_dx and (need_dw or need_db):
+            dyq, dyt, *sums = fp8_quantize_both(dy, need_db)
+            db = sums[0] if need_db else None
+        elif need_dx:
+            dyq = fp8_quantize(dy)
+        elif need_db:
+            dyt, db = fp8_quantize(dy, transpose=True, column_sums=True)
+        elif need_dw:
+            dyt = fp8_quantize(dy, transpose=True)
+        if need_dx:
+            dx = fp8_matmul(dyq, w)
         if need_dw:
             dw = fp8_matmul(fp8_quantize(x, transpose=True), dyt)
     return (dx, dw, db) if need_db else (dx, dw)

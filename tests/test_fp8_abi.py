@@ -27,9 +27,21 @@ def test_quantize_refuses(kw):
     assert _lib.load().mh_last_error()
 
 
+def both(x=A, dtype=0, ldx=256, R=4, K=256, q=A, ldq=256, s=A, lds=4, qt=A, ldqt=128, st=A, ldst=4, colsum=None, ws=None, nws=0):
+    return _lib.load().mh_fp8_quantize_both(P(x), dtype, ldx, R, K, P(q), ldq, P(s), lds, P(qt), ldqt, P(st), ldst, P(colsum), P(ws), nws, P(0))
+
+
+@pytest.mark.parametrize("kw", [dict(dtype=3), dict(ldx=255), dict(R=-1), dict(x=None), dict(q=None), dict(s=None), dict(ldq=128), dict(q=A + 8), dict(lds=2),
+                                dict(qt=None), dict(st=None), dict(ldqt=112), dict(qt=A + 8), dict(ldst=2), dict(st=A + 2)])
+def test_quantize_both_refuses(kw):
+    assert both(**kw) == -1
+    assert _lib.load().mh_last_error()
+
+
 def test_quantize_needs_its_workspace_for_column_sums():
     assert quantize(transpose=1, R=128, ldq=128, colsum=A) == -4
     assert quantize(transpose=1, R=128, ldq=128, colsum=A, ws=A, nws=256 * 4 - 1) == -4
+    assert both(colsum=A) == -4 and both(colsum=A, ws=A, nws=256 * 4 - 1) == -4 and both(R=0) == 0 and both(K=0, ldx=0) == 0
 
 
 @pytest.mark.parametrize("kw", [dict(a=None), dict(sb=None), dict(lda=240), dict(ldb=128), dict(ldsa=3), dict(dt=7), dict(ldo=7), dict(out=None), dict(K=0),

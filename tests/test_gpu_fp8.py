@@ -76,6 +76,20 @@ def test_quantize(device, dtype, R, K, strided, transpose):
     assert (m.scales[:, e.shape[1]:] == 127).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("R,K,strided", [(1, 1, False), (3, 127, True), (128, 128, False), (129, 130, False), (300, 515, True), (1025, 64, False)])
+def test_quantize_both(device, dtype, R, K, strided):
+    x = matrix(np.random.default_rng(R + K), R, K, dtype, device, strided)
+    x[R // 2, K // 2], x[0, 0] = float("nan"), float("inf")
+    bits = lambda m: (m.values.view(torch.uint8), m.scales, m.cols)  # noqa: E731
+    m, mt = ops.fp8_quantize_both(x)
+    for got, want in ((m, ops.fp8_quantize(x)), (mt, ops.fp8_quantize(x, transpose=True))):
+        assert all(torch.equal(a, b) if isinstance(a, torch.Tensor) else a == b for a, b in zip(bits(got), bits(want)))
+    x[R // 2, K // 2], x[0, 0] = 1.0, 2.0
+    *_, sums = ops.fp8_quantize_both(x, column_sums=True)
+    assert torch.equal(sums, ops.fp8_quantize(x, transpose=True, column_sums=True)[1])
+
+
 def test_quantize_edges(device):
     """Zeros, subnormals, the largest values, scale borders (448 2^e and the next value), infinities and NaN, one block each."""
     rows = np.zeros((8, 256), np.float32)
@@ -214,7 +228,7 @@ def test_column_sums(device, R, C):
     x = torch.randn(R, C, generator=torch.Generator(device=device).manual_seed(R), device=device)
     m, sums = ops.fp8_quantize(x, transpose=True, column_sums=True)
     assert torch.equal(m.values.view(torch.uint8), ops.fp8_quantize(x, transpose=True).values.view(torch.uint8))
-    # 24 additions within a block (16, then 8), one for each sixteenth block, then 16: each rounds by 2^-24 of sum |x| at most
+    # 24 additions within a block at most, one for each sixteenth block, then 16: each rounds by 2^-24 of sum |x| at most
     tol = (24 + -(-R // 2048) + 16) * 2.0 ** -24 * x.double().abs().sum(0)
     assert ((sums.double() - x.double().sum(0)).abs() <= tol).all()
 
@@ -248,6 +262,8 @@ def test_empty_and_refused(device):
         ops.fp8_quantize(z(4, 8, dtype=torch.float64))
     with pytest.raises(ValueError):
         ops.fp8_quantize(z(4, 8), column_sums=True)
+    with pytest.raises(ValueError):
+        ops.fp8_quantize_both(z(0, 8))
     with pytest.raises(ValueError):
         ops.fp8_linear(z(3, 5), w8)
     with pytest.raises(ValueError):
