@@ -756,21 +756,25 @@ F8Plan f8_plan(int64_t M, int64_t N, int64_t K) {
     const int kb = (int)mh_ceil_div(K, 128);
     p.slices = 1;
     p.kb_split = (kb + 3) / 4 * 4;
-    // The streaming kernel reads a once for every 64 rows of b at most; of four 16-row groups of a that is too much where b is neither long nor its
-    // rows short (64 x 512 x 8192: 31 us, 18 on the tiles; 48 rows, or 64 x 14341 x 4096: 23 against 28, 26 against 30).
-    if (M <= ROWS_MOST && (M <= 48 || N >= 8192 || kb < 16)) {
+    // The streaming kernel's wavefronts work through the 16-row groups of a and their blocks of k one by one: too long where both are many, unless b
+    // is much to read as well.  Streaming / tiles, fp32 outputs (us in a graph): 48 x 2048, 32 blocks 11.9 / 13.5, 64 blocks 19.8 / 14.6; 48 x 14341, 32
+    // blocks 18.9 / 27.1, x 65536 57 / 101; 64 rows, x 2048, 16 blocks 9.9 / 14.0, 32 blocks 16.4 / 14.7; x 30000, 16 blocks 24.9 / 25.8, 32 blocks
+    // 42 / 37; x 200000, 32 blocks 327 / 354 (bf16 267 / 255).
+    const int64_t groups = mh_ceil_div(M, 16);
+    if (M <= ROWS_MOST && (groups == 1 || groups * kb <= 96 || (groups <= 3 && N > 8192))) {
         p.rows = true;
         return p;
     }
-    // Large tiles read less and small ones wait less at their ends: large where the sum is long and the chip has two rounds of them.  Large / small,
-    // fp32 and bf16 outputs: 8192 x 8192 x 8192 868 / 945, 486 / 583 us; 65536 x 512 x 3341 268 / 264, 165 / 179; 16384 x 1024 x 2048 81 / 74,
-    // 58 / 52; 65536 x 256 x 512 46 / 31, 48 / 25.
-    p.big = kb >= 16 && mh_ceil_div(M, 256) * mh_ceil_div(N, 256) >= 512;
+    // Large tiles read less, and where they fill the 256 compute units' rounds they are faster: large / small, fp32 outputs, 4096 x 4096 (one full round) x
+    // 128 18 / 20 us, x 4096 116 / 132; 4608 x 4096 (two rounds, 0.56 full) x 4096 180 / 151; 6144 x 4096 (0.75) x 512 42 / 40, x 4096 179 / 179 (bf16
+    // 100 / 108); 7168 x 4096 (0.875) x 128 29 / 31; 8192^3 821 / 935 (bf16 417 / 513).
+    const int64_t large = mh_ceil_div(M, 256) * mh_ceil_div(N, 256);
+    p.big = large >= 256 && large * 100 >= mh_ceil_div(large, 256) * 256 * (kb >= 16 ? 75 : 85);
     if (!p.big) {
         // Too few tiles for the chip: slices of the summed axis, each long enough to be worth its partial output (eight blocks: 1024^3 in one slice
-        // 14 us, two 17), and not more than the join reads well (128 x 415 x 65536: 64 slices 75 us, 32 50).  A tile for each of the 256 compute
-        // units is enough (2048^3 bf16: 17 us, 28 in two slices); below that two workgroups a unit are better than one (1024 x 2048 x 16384: 58,
-        // 64).
+        // 12 us, two 16), and not more than the join reads well (128 x 415 x 65536: 64 slices 76 us, 32 51).  A tile for each of the 256 compute
+        // units is enough (2048^3 bf16: 15 us, 26 in two slices); below that two workgroups a unit are better than one (1024 x 2048 x 16384: 76,
+        // 116 in one slice).
         const int64_t tiles = mh_ceil_div(M, 128) * mh_ceil_div(N, 128);
         int64_t s = tiles >= 256 ? 1 : 512 / tiles;
         if (s > kb / 8) s = kb / 8;
@@ -829,11 +833,17 @@ int32_t f8_launch_rows_nb(const F8Args& g, const X* x, int64_t ldx, int K, int w
 }
 template <int MT, typename X>
 int32_t f8_launch_rows(const F8Args& g, const X* x, int64_t ldx, int K, hipStream_t s) {
-    const int wk = g.kblocks >= 8 ? 8 : g.kblocks >= 4 ? 4 : g.kblocks >= 2 ? 2 : 1;
-    // more rows of b a wavefront: a is read, or quantised, fewer times, as long as the workgroups still fill the chip
+    // Long b: rather rows of its own for a wavefront than a short share of k, as long as there are workgroups for most of the chip and no share is longer
+    // than 16 blocks (24 x 1024 -> 65536: 25 us with eight sharing, 17 with two; 48 x 2048 -> 20000: 20 in 313 workgroups, 17 in 157; 16 x 8192 -> 65536:
+    // 115 with eight, 107 with four, 142 with one).
+    int wk = g.kblocks >= 8 ? 8 : g.kblocks >= 4 ? 4 : g.kblocks >= 2 ? 2 : 1;
+    while (wk > 1 && g.kblocks * 2 <= 16 * wk && mh_ceil_div(g.N, RW / (wk / 2) * 64) >= 150) wk /= 2;
+    // As few rows of b a wavefront as still give one workgroup a compute unit: fewer leave compute units idle, and a second workgroup on some takes as long
+    // as one on all (48 x 4096 -> 11000 in 344 workgroups of two groups of 16 a wavefront: 29 us, in 172 of four 19; 8192 rows in 256 of two 15.6, in
+    // 128 of four 18.0; 2048 rows in 128 of one 13.0, in 64 of two 13.9).
     auto groups = [&](int nb) { return mh_ceil_div(g.N, RW / wk * 16 * nb); };
-    if (groups(4) >= 192) return f8_launch_rows_nb<MT, 4>(g, x, ldx, K, wk, s);
-    if (groups(2) >= 192) return f8_launch_rows_nb<MT, 2>(g, x, ldx, K, wk, s);
+    if (groups(2) > 256) return f8_launch_rows_nb<MT, 4>(g, x, ldx, K, wk, s);
+    if (groups(1) > 256) return f8_launch_rows_nb<MT, 2>(g, x, ldx, K, wk, s);
     return f8_launch_rows_nb<MT, 1>(g, x, ldx, K, wk, s);
 }
 int32_t f8_launch_rows_any(const F8Args& g, hipStream_t s) {

@@ -141,9 +141,10 @@ def test_linear_and_matmul(device, M, N, K, out):
 
 
 @pytest.mark.parametrize("out", ["f32", "bf16"])
-@pytest.mark.parametrize("M,N,K", [(4100, 4200, 260), (5000, 3400, 1030)])
+@pytest.mark.parametrize("M,N,K", [(4100, 4200, 260), (5000, 3400, 1030), (4000, 4090, 130), (33001, 500, 1030), (64, 40001, 2300), (48, 38501, 2050),
+                                   (24, 65701, 520), (40, 20001, 1030), (16, 39001, 1030), (7, 80001, 130), (16, 11000, 1100)])
 def test_large_tiles(device, M, N, K, out):
-    """Sizes that fill the chip with the large tile, ragged in every axis, against the product of the same 8-bit values in float64 on the device."""
+    """Sizes that fill the chip with the large tile, or with few rows and a long b, ragged in every axis, against the product of the same 8-bit values in float64 on the device."""
     g = torch.Generator(device=device).manual_seed(M)
     x, w = (torch.randn(n, K, generator=g, device=device) for n in (M, N))
     x8, w8 = ops.fp8_quantize(x), ops.fp8_quantize(w)
