@@ -310,7 +310,8 @@ __device__ __forceinline__ void f8_wave_fence() {
 // the result and hides that; the finer types take the bf16 instruction, which adds in fp32, at half the rate.
 // Each wavefront holds (BM / WM) x (BN / WN) of the output as 32 x 32 accumulators, rows of b as the instruction's rows: a lane then owns four
 // neighbouring columns of C.  Tiles of one block of k (128 bytes a row) come by direct-to-LDS loads, two stages, one barrier a block; 16-byte
-// chunk c of row r lies at c ^ ((r >> 1) & 7), which spreads the 16 rows of a read phase over all 64 banks.
+// chunk c of row r lies at c ^ ((r >> 1) & 7), which spreads the 16 rows of a read phase over all 64 banks.  Bound by the matrix pipe: 8192^3 414 us, 2650
+// TFLOP/s, and WIDE 808 us, 1360 TFLOP/s; 65536 x 512 x 3341 WIDE 192 us, 1170 TFLOP/s.
 template <int BM, int BN, int WM, int WN, bool WIDE>
 __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_gemm_kernel(const F8Args g) {
     constexpr int NT = WM * WN * 64, TM = BM / WM / 32, TN = BN / WN / 32;
@@ -565,6 +566,8 @@ struct F8Lane<f8_stored> {
 // wavefront's own, the next block's while one is multiplied, and no barrier is needed.  Partial sums meet in LDS in a fixed order and leave as
 // whole stretches of output rows.  X: the type of a where it is quantised on the way (at most 16 rows: the work is done again for every 16 NB
 // rows of b), or f8_stored.
+// 16 x 4096 -> 65536 45 us, 6.0 TB/s; 48 x 4096 -> 14341 20 us, 2.9 TB/s (225 workgroups, one round: what is left is its beginning and end); 1 x 1024 ->
+// 4096 4.6 us, nearly all of it a launch.
 constexpr int RW = 8;  // wavefronts
 template <int NB>
 constexpr int f8_rows_stage() {
