@@ -339,7 +339,10 @@ __device__ __forceinline__ void top_entries(const T* x, int n, int first, int k,
     __syncthreads();
     uint32_t mine[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) mine[i] = i * NT + (int)threadIdx.x < nb ? key_of(s.most[i * NT + threadIdx.x] + 0.f) : 0;
+    for (int i = 0; i < PER; ++i) {  // a stretch with nothing but -inf and NaN has no key: its largest entry is -inf or, NaN throughout, a NaN
+        const float q = i * NT + (int)threadIdx.x < nb ? s.most[i * NT + threadIdx.x] : -INF;
+        mine[i] = q > -INF ? key_of(q + 0.f) : 0;
+    }
     // The k-th largest of the threads' largest, to 16 bits: a little below the buckets' own.  One wavefront looks for it, the others' in its registers:
     // no barrier a round.
     uint32_t* const top = reinterpret_cast<uint32_t*>(s.cand);
