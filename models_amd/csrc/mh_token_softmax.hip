@@ -327,6 +327,45 @@ struct TopLds {
     int n, nq, red[2 * (NT / 64)];
 };
 
+// Behind `have` keys, the first k - have entries of key `low` in order of their places; how many keys there are then.  The workgroup goes along the row
+// together and stops where it has them.
+template <int NT, typename T>
+__device__ __forceinline__ int first_ties(const T* x, int n, int first, uint32_t low, int have, int k, TopLds<NT>& s) {
+    constexpr int VE = lp_vec<T>::N;
+    const int nv = n / VE, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    int phase = 0;
+    for (int at = 0; have < k && at <= nv; at += NT) {
+        const int v = at + (int)threadIdx.x;
+        float a[VE];
+        if (v < nv) {
+            lp_unpack(lp_load16(x + (int64_t)v * VE), a, x);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VE; ++i) a[i] = v == nv && nv * VE + i < n ? lp_float(x[nv * VE + i]) : -INF;
+        }
+        uint32_t tie = 0;
+#pragma unroll
+        for (int i = 0; i < VE; ++i) tie |= (a[i] > -INF && key_of(a[i] + 0.f) == low ? 1u : 0u) << i;
+        int before = __popc(tie);  // ties of this thread and the lanes before it
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int u = __shfl_up(before, o);
+            before += lane >= o ? u : 0;
+        }
+        int* const r = s.red + (phase ^= 1) * (NT / 64);
+        if (lane == 63) r[w] = before;
+        __syncthreads();
+        int place = have + before - __popc(tie);
+#pragma unroll
+        for (int i = 0; i < NT / 64; ++i) {
+            place += i < w ? r[i] : 0;
+            have += r[i];
+        }
+        for (; tie && place < k; tie &= tie - 1, ++place) s.cand[place] = (uint64_t)low << 32 | (uint32_t)~(first + v * VE + __ffs(tie) - 1);
+    }
+    return have < k ? have : k;
+}
+
 // The k largest keys of the n entries at x, in order, to emit(place, key).  The k-th largest among largest entries of parts of the row bounds the row's
 // k-th largest from below, so only about k buckets are read again, as whole lines.  (With one bucket a thread, its vectors NT apart, 100 of 512 buckets
 // touched nearly every line of the row: 64 x 1000000, k = 100 took 84 us, 43 without alternatives.)
@@ -343,30 +382,33 @@ __device__ __forceinline__ void top_entries(const T* x, int n, int first, int k,
         const float q = i * NT + (int)threadIdx.x < nb ? s.most[i * NT + threadIdx.x] : -INF;
         mine[i] = q > -INF ? key_of(q + 0.f) : 0;
     }
-    // The k-th largest of the threads' largest, to 16 bits: a little below the buckets' own.  One wavefront looks for it, the others' in its registers:
-    // no barrier a round.
-    uint32_t* const top = reinterpret_cast<uint32_t*>(s.cand);
     uint32_t largest = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) largest = mine[i] > largest ? mine[i] : largest;
-    top[threadIdx.x] = largest;
-    __syncthreads();
-    if (threadIdx.x < 64) {
-        uint32_t of[NT / 64], t = 0;
+    // The k-th largest of the threads' largest, from the high bits down to bit `end`: a little below the buckets' own.  One wavefront looks for it, the
+    // others' in its registers: no barrier a bit.
+    auto bound = [&](int end) {
+        uint32_t* const top = reinterpret_cast<uint32_t*>(s.cand);
+        top[threadIdx.x] = largest;
+        __syncthreads();
+        if (threadIdx.x < 64) {
+            uint32_t of[NT / 64], t = 0;
 #pragma unroll
-        for (int w = 0; w < NT / 64; ++w) of[w] = top[w * 64 + threadIdx.x];
-        if (nb >= k)
-            for (int b = 31; b >= 16; --b) {
-                const uint32_t next = t | 1u << b;
-                int c = 0;
+            for (int w = 0; w < NT / 64; ++w) of[w] = top[w * 64 + threadIdx.x];
+            if (nb >= k)
+                for (int b = 31; b >= end; --b) {
+                    const uint32_t next = t | 1u << b;
+                    int c = 0;
 #pragma unroll
-                for (int w = 0; w < NT / 64; ++w) c += lanes(of[w] >= next);
-                if (c >= k) t = next;
-            }
-        if (threadIdx.x == 0) s.low = t;
-    }
-    __syncthreads();
-    const uint32_t low = s.low <= KEY_NONE ? KEY_NONE + 1 : s.low;
+                    for (int w = 0; w < NT / 64; ++w) c += lanes(of[w] >= next);
+                    if (c >= k) t = next;
+                }
+            if (threadIdx.x == 0) s.low = t;
+        }
+        __syncthreads();
+        return s.low <= KEY_NONE ? KEY_NONE + 1 : s.low;
+    };
+    uint32_t low = bound(16);
 #pragma unroll
     for (int i = 0; i < PER; ++i)
         if (mine[i] >= low) s.list[atomicAdd(&s.nq, 1)] = (uint16_t)(i * NT + threadIdx.x);
@@ -400,7 +442,24 @@ __device__ __forceinline__ void top_entries(const T* x, int n, int first, int k,
     }
     __syncthreads();
     int have = s.n;
-    if (have > CAND) {  // ties, or large entries that fell to the same few stretches: look for the threshold in the row itself
+    if (have > CAND) {
+        // The bound to its last bit (logits of 300 +- 1 are 2 apart in 16 bits), what lies above it, and the first of its ties: a row, or a part of one, of
+        // one value, as masks of a finite value leave them, has more than LDS holds (4096 x 131072 bf16 with ten entries left, 20 alternatives: 557 us; a
+        // search of the row for the threshold bit by bit took 8100).
+        __syncthreads();
+        low = bound(0);
+        if (threadIdx.x == 0) s.n = 0;
+        __syncthreads();
+        each_entry<NT>(x, n, [&](const float(&l)[VE], int at) {
+#pragma unroll
+            for (int i = 0; i < VE; ++i)
+                if (l[i] > -INF && key_of(l[i] + 0.f) > low) put(key_at(l[i], first + at + i));
+        });
+        __syncthreads();
+        have = s.n;
+        if (have < k) have = first_ties<NT>(x, n, first, low, have, k, s);
+    }
+    if (have > CAND) {  // more large entries than that fell to the same few threads: look for the threshold in the row itself
         const uint64_t t = key_threshold(k, CAND, [&](uint64_t next) {
             int c = 0;
             each_entry<NT>(x, n, [&](const float(&l)[VE], int at) {
@@ -500,9 +559,10 @@ __device__ __forceinline__ void lp_emit(const LpArgs& g, int64_t row, const Sum&
 }
 
 // One read of the logits: 8192 x 32769 fp32 (rows at any word) 193 - 216 us, 5.0 - 5.6 TB/s; 64 x 1000000 fp32 with 100 alternatives 50 us, 5.1 TB/s;
-// 1 x 131072 bf16 with 20 alternatives 9.8 us in parts, the join behind it 7.3: both latency.
+// 1 x 131072 bf16 with 20 alternatives 9.8 us in parts, the join behind it 7.3: both latency.  Eight wavefronts a SIMD are asked for where the compiler would
+// leave room for seven: 4096 x 16384 fp32, 20 alternatives, 51 us and 57.
 template <int NT, typename T, bool TOP>
-__global__ __launch_bounds__(NT) void token_logprobs_kernel(const LpArgs g) {
+__global__ __launch_bounds__(NT, TOP && NT == 512 ? 8 : 1) void token_logprobs_kernel(const LpArgs g) {
     __shared__ Sum red[NT / 64];
     __shared__ TopLds<TOP ? NT : 64> lds;
     const int64_t row = blockIdx.x / (uint32_t)g.parts;
