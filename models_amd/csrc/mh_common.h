@@ -58,8 +58,9 @@ void mh_record_op(std::function<void()>&& op);
     } while (0)
 
 // Tuning / ablation knobs of the labs (tools/exp, profiles/*_notes.md) exist only in a library built with -DMH_LAB
-// (MH_LAB=1 python -c "from models_amd import build; build.build(force=True)").  The shipped library reads the switches documented in
-// README.md ("Environment switches", enforced by tests/test_abi.py) and nothing else: MH_LAB_ENV is a constant nullptr there.
+// (MH_LAB=1 python -c "from models_amd import build; build.build()", and MH_LAB=1 where it is loaded: without it that library counts as
+// stale).  The shipped library reads the switches documented in README.md ("Environment switches", enforced by tests/test_abi.py) and
+// nothing else: MH_LAB_ENV is a constant nullptr there.
 #ifdef MH_LAB
 #define MH_LAB_ENV(name) getenv(name)
 #else
