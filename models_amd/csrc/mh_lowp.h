@@ -2,6 +2,16 @@
 #pragma once
 #include "mh_common.h"
 
+// Host: whether nx rows of wx bytes at x, lx bytes apart, and nd rows of wd bytes at d, ld apart, share a byte.  Rows that are equally far apart may lie
+// between each other (columns of one wider buffer); others count as sharing where their ranges do.
+static inline bool lp_shared(const void* x, int64_t lx, int64_t wx, int64_t nx, const void* d, int64_t ld, int64_t wd, int64_t nd) {
+    if (nx <= 0 || nd <= 0 || wx <= 0 || wd <= 0) return false;
+    const int64_t by = (int64_t)(reinterpret_cast<uintptr_t>(d) - reinterpret_cast<uintptr_t>(x));
+    if (lx != ld || (nx == 1 && nd == 1)) return by < (nx - 1) * lx + wx && -by < (nd - 1) * ld + wd;
+    const int64_t q = by >= 0 ? by / lx : -((-by + lx - 1) / lx), r = by - q * lx;  // row j of d begins r bytes into row j + q of x
+    return (r < wx && q < nx && -q < nd) || (r + wd > lx && q + 1 < nx && -(q + 1) < nd);
+}
+
 struct lp_bf16 {
     uint16_t u;
 };

@@ -983,7 +983,7 @@ __device__ __forceinline__ T* at_offset(T* p, uint32_t bytes) {
 }
 
 template <int NT, int R, int E, typename T, bool TAIL>
-__global__ __launch_bounds__(NT) void distill_topk_train_kernel(const DsArgs g, const float* __restrict__ dloss, T* __restrict__ dall, int64_t ldd) {
+__global__ __launch_bounds__(NT) void distill_topk_train_kernel(const DsArgs g, const float* dloss, T* dall, int64_t ldd) {  // dall may be g.x
     constexpr int VE = lp_vec<T>::N;
     extern __shared__ uint32_t bits[];
     __shared__ Sum red[NT / 64];
@@ -1111,6 +1111,13 @@ int32_t ts_check(const char* who, const void* x, int32_t dtype, int64_t ld, int6
     MH_REQUIRE(N == 0 || x, "%s: logits is NULL", who);
     return MH_OK;
 }
+// a gradient lies in place of the logits or apart from them
+int32_t ts_gradient(const char* who, const void* x, int32_t dtype, int64_t ld, const void* d, int64_t ldd, int64_t N, int64_t V) {
+    const int64_t es = dtype == MH_F32 ? 4 : 2;
+    MH_REQUIRE(d != x || ldd == ld, "%s: a gradient in place of the logits needs their leading dimension", who);
+    MH_REQUIRE(d == x || !lp_shared(x, ld * es, V * es, N, d, ldd * es, V * es, N), "%s: the gradient overlaps the logits and does not lie in their place", who);
+    return MH_OK;
+}
 // a launch has fewer than 2^32 threads
 int32_t ts_grid(const char* who, int64_t N, int parts) {
     MH_REQUIRE(N * parts < (int64_t)1 << 23, "%s: %lld rows in %d parts each are too many workgroups for one call", who, (long long)N, parts);
@@ -1211,7 +1218,7 @@ int32_t grad_launch(const char* who, GradArgs g, bool distill, hipStream_t s) {
     return MH_OK;
 }
 int32_t grad_any(const char* who, const GradArgs& g, int32_t dtype, bool distill, hipStream_t s) {
-    MH_REQUIRE(g.d != g.x || g.ldd == g.ld, "%s: a gradient in place of the logits needs their leading dimension", who);
+    if (int32_t rc = ts_gradient(who, g.x, dtype, g.ld, g.d, g.ldd, g.N, g.V)) return rc;
     if (dtype == MH_F32) return grad_launch<float>(who, g, distill, s);
     if (dtype == MH_BF16) return grad_launch<lp_bf16>(who, g, distill, s);
     return grad_launch<lp_f16>(who, g, distill, s);
@@ -1311,7 +1318,7 @@ int32_t mh_distill_topk_train(const void* logits, int32_t dtype, int64_t ld, int
     if (N == 0) return MH_OK;
     MH_REQUIRE(teacher_ids && teacher_logp && loss && dlogits && ld_ids >= K && ld_logp >= K && ldd >= V,
                "mh_distill_topk_train: an argument is NULL, or rows are too short");
-    MH_REQUIRE(dlogits != logits || ldd == ld, "mh_distill_topk_train: a gradient in place of the logits needs their leading dimension");
+    if (int32_t rc = ts_gradient("mh_distill_topk_train", logits, dtype, ld, dlogits, ldd, N, V)) return rc;
     if (int32_t rc = ts_grid("mh_distill_topk_train", N, 1)) return rc;
     const int64_t need = mh_distill_topk_train_workspace_bytes(N, V, K, dtype, tail);
     if (int32_t rc = ts_workspace("mh_distill_topk_train", workspace, workspace_bytes, need)) return rc;

@@ -2164,6 +2164,20 @@ def _ld(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
 
 
+def _shared(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the rows of two 2-D tensors share memory.  Rows that are equally far apart may lie between each other (columns of one wider
+    buffer); others count as sharing where their ranges do."""
+    la, lb = _ld(a) * a.element_size(), _ld(b) * b.element_size()
+    wa, wb = a.shape[1] * a.element_size(), b.shape[1] * b.element_size()
+    (na, nb), by = (a.shape[0], b.shape[0]), b.data_ptr() - a.data_ptr()
+    if not (na and nb and wa and wb):
+        return False
+    if la != lb or (na == 1 and nb == 1):
+        return by < (na - 1) * la + wa and -by < (nb - 1) * lb + wb
+    q, r = divmod(by, la)  # row j of b begins r bytes into row j + q of a
+    return (r < wa and q < na and -q < nb) or (r + wb > la and q + 1 < na and -(q + 1) < nb)
+
+
 def _at(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
@@ -2427,7 +2441,7 @@ def _catalogue(logits: torch.Tensor, temperature: float):
 
 
 def _dlogits(logits: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
-    """The gradient's buffer: ``out`` (``logits`` itself is allowed), or a new contiguous one."""
+    """The gradient's buffer: ``out`` (``logits`` itself, or apart from them), or a new contiguous one."""
     if out is None:
         return torch.empty_like(logits, memory_format=torch.contiguous_format)
     _float_2d(out, "out")
@@ -2435,6 +2449,8 @@ def _dlogits(logits: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
         raise ValueError(f"out must be {list(logits.shape)} of {logits.dtype}, got {list(out.shape)} of {out.dtype}")
     if out.data_ptr() == logits.data_ptr() and _ld(out) != _ld(logits):
         raise ValueError("out may be the logits themselves, but not other rows that start where they start")
+    if out.data_ptr() != logits.data_ptr() and _shared(logits, out):
+        raise ValueError("out may be the logits themselves or apart from them, but not overlap them elsewhere")
     return out
 
 
