@@ -711,8 +711,9 @@ int32_t mh_sharded_lookup_bwd(mh_comm_t comm, int32_t F, int64_t B, int64_t capa
  * only, [K] floats) receives the column sums of x in a fixed order, from a workspace of ceil(R / 128) * K floats.
  * mh_fp8_quantize_both: both forms from one read -- q / scales as with transpose = 0, qt / scales_t (and colsum) as with transpose = 1.
  * mh_fp8_matmul: out[M, N] = a b^T + bias, a [M, K] and b [N, K] in that form, bias [N] floats or NULL, out of type out_dtype with leading
- * dimension ldo.  An MH_F32 or MH_F16 output is summed in 32 bits throughout; an MH_BF16 one by the 8-bit matrix instruction, at twice the
- * rate, whose sums are off by at most 7 * 2^-13 of sum |a b| (under half a step of bf16; 1.5e-5 of the norm on random values).
+ * dimension ldo.  An MH_F32 or MH_F16 output, or one of up to 16 rows, is summed in 32 bits throughout; an MH_BF16 one of more rows by the 8-bit
+ * matrix instruction, at twice the rate, whose sums are off by up to 7 * 2^-13 of sum |a b| (1.5e-5 of the norm on random values): many steps of
+ * bf16 where the terms cancel.  An MH_F32 output rounded to bf16 has its rounding alone.
  * mh_fp8_linear: x [M, K] in the form of mh_fp8_quantize (into the workspace, or on the way for few rows), then the product with w [N, K].
  * K <= 2^24 - 128, leading dimensions of 8-bit values and scales <= 2^24, M, N < 2^27; workspaces are 16-byte aligned.  In MH_F32 and MH_F16 outputs an
  * operand's value under 2^-126 may count as 0 and one that rounds to 2^128 is infinite.

@@ -306,8 +306,9 @@ __device__ __forceinline__ void f8_wave_fence() {
 
 // Tiled product.  WIDE: operands widened to bf16 on the way from LDS, for outputs of fp32 and fp16.  The 8-bit matrix instruction takes its
 // products in groups of eight and cuts each at 2^-13 of the group's largest (measured with single products on both shapes; the groups' sums
-// are then added in fp32): at most 7 2^-13 = 2^-10.2 of sum |a b|, 1.5e-5 of the norm on random values.  Half a step of a bf16 output is 2^-8 of
-// the result and hides that; the finer types take the bf16 instruction, which adds in fp32, at half the rate.
+// are then added in fp32): at most 7 2^-13 = 2^-10.2 of sum |a b|, 1.5e-5 of the norm on random values.  A bf16 output takes it all the same, for twice
+// the rate: where the terms do not cancel its rounding, 2^-8 of the result, is larger, but where they do the sum can be off by many of its steps (quantising
+// the operands is off by up to 2^-4 of each term already).  The finer types take the bf16 instruction, which adds in fp32, at half the rate.
 // Each wavefront holds (BM / WM) x (BN / WN) of the output as 32 x 32 accumulators, rows of b as the instruction's rows: a lane then owns four
 // neighbouring columns of C.  Tiles of one block of k (128 bytes a row) come by direct-to-LDS loads, two stages, one barrier a block; 16-byte
 // chunk c of row r lies at c ^ ((r >> 1) & 7), which spreads the 16 rows of a read phase over all 64 banks.  Bound by the matrix pipe: 8192^3 414 us, 2650
@@ -831,8 +832,13 @@ template <int MT, int NB, typename X>
 int32_t f8_launch_rows_nb(const F8Args& g, const X* x, int64_t ldx, int K, int wk, hipStream_t s) {
     const dim3 grid((unsigned)mh_ceil_div(g.N, RW / wk * 16 * NB)), block(64 * RW);
     constexpr int lds = RW * 2 * f8_rows_stage<NB>();
-    return g.kind != MH_BF16 ? f8_launch<fp8_rows_kernel<MT, NB, true, X>>(grid, block, lds, s, g, x, ldx, K, wk)
-                             : f8_launch<fp8_rows_kernel<MT, NB, false, X>>(grid, block, lds, s, g, x, ldx, K, wk);
+    // Up to 16 rows the sums are in 32 bits for bf16 outputs as well, which costs next to nothing: reading b is the bound (8-bit instruction / widened, us: 8 x
+    // 4096 -> 65536 42.8 / 43.0, 16 x 4096 -> 65536 43.2 / 43.2, 16 x 8192 -> 65536 105 / 106, 1 x 4096 -> 16384 13.1 / 13.9).  More rows: 48 x 4096 -> 14341
+    // 19.3 / 21.0, 64 x 128 -> 1000000 87 / 96, 64 x 1024 -> 30000 12.9 / 15.3.
+    if constexpr (MT > 1) {
+        if (g.kind == MH_BF16) return f8_launch<fp8_rows_kernel<MT, NB, false, X>>(grid, block, lds, s, g, x, ldx, K, wk);
+    }
+    return f8_launch<fp8_rows_kernel<MT, NB, true, X>>(grid, block, lds, s, g, x, ldx, K, wk);
 }
 template <int MT, typename X>
 int32_t f8_launch_rows(const F8Args& g, const X* x, int64_t ldx, int K, hipStream_t s) {

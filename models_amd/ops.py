@@ -2308,8 +2308,9 @@ def _fp8_bias(bias: Optional[torch.Tensor], N: int) -> None:
 def fp8_matmul(a: Fp8Matrix, b: Fp8Matrix, bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``a @ b.T + bias`` of two 8-bit matrices ``[M, K]`` and ``[N, K]`` -> ``[M, N]``.  A float32 or
-    float16 output is summed in 32 bits throughout; a bfloat16 one by the scaled 8-bit matrix instruction, at twice the rate: its sums are
-    off by at most 2^-10.2 of sum |a b|, where half a step of bfloat16 is 2^-8 of the result."""
+    float16 output, or one of up to 16 rows, is summed in 32 bits throughout; a bfloat16 one of more rows by the scaled 8-bit matrix
+    instruction, at twice the rate: its sums are off by up to 2^-10.2 of sum |a b|, which is many steps of bfloat16 where the terms cancel.
+    A float32 output rounded afterwards (``.to(torch.bfloat16)``) has its rounding alone."""
     lib = _lib.load()
     M, K = _fp8_check(a, "a")
     N, Kb = _fp8_check(b, "b")
@@ -2333,7 +2334,8 @@ def fp8_matmul(a: Fp8Matrix, b: Fp8Matrix, bias: Optional[torch.Tensor] = None, 
 def fp8_linear(x: torch.Tensor, w: Fp8Matrix, bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """A Dense layer with 8-bit operands: ``x`` [M, K] quantised by blocks of 128 and multiplied with ``w``, the layer's kernel as
-    ``fp8_quantize(kernel, transpose=True)`` (``[N, K]``), made once.  ``linear`` is the layer in 32 bits."""
+    ``fp8_quantize(kernel, transpose=True)`` (``[N, K]``), made once.  Sums as ``fp8_matmul`` has them.  ``linear`` is the layer in 32
+    bits."""
     lib = _lib.load()
     dt = _float_2d(x, "x")
     N, K = _fp8_check(w, "w")
