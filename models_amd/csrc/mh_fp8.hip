@@ -528,10 +528,6 @@ struct F8Lane {
             }
         }
     }
-    __device__ __forceinline__ void arrived() {
-#pragma unroll
-        for (int i = 0; i < N; ++i) asm volatile("" : "+v"(w[i].x), "+v"(w[i].y), "+v"(w[i].z), "+v"(w[i].w));
-    }
     __device__ __forceinline__ i32x8 values(uint32_t& scale) const {
         float v[32];
         const X* type = nullptr;
@@ -554,7 +550,6 @@ struct F8Lane<f8_stored> {
         hi = *reinterpret_cast<const i32x4*>(p + 16);
         s = *ps;
     }
-    __device__ __forceinline__ void arrived() { asm volatile("" : "+v"(lo), "+v"(hi), "+v"(s)); }
     __device__ __forceinline__ i32x8 values(uint32_t& scale) const {
         scale = s;
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -602,7 +597,7 @@ __global__ __launch_bounds__(64 * RW, 2) void fp8_rows_kernel(const F8Args g, co
     auto issue = [&](int kb) {
 #pragma unroll
         for (int j = 0; j < 2 * NB; ++j) f8_dma16(tb + (int64_t)kb * 128 + src[j], stage + (kb & 1) * STAGE + j * 1024);
-        asm volatile("" ::: "memory");  // before a's loads, for multiply() counts on it
+        asm volatile("" ::: "memory");  // all of b's lines first, then a: mixed by the compiler, 48 x 4096 -> 14341 took 19.9 us instead of 19.2
         __builtin_amdgcn_sched_barrier(0);
     };
     const uint8_t *pa[MT], *psa[MT];
@@ -633,15 +628,14 @@ __global__ __launch_bounds__(64 * RW, 2) void fp8_rows_kernel(const F8Args g, co
             else v.a[i].load(px[i] + (int64_t)kb * 128, K - kb * 128 - h * 32);
         }
     };
-    // Block kb: b's lines were asked for before a's, and loads arrive in order: where a is there, b is.
+    // Loads arrive in order: with no more left on the way than the next block's lines of b, which were asked for after this block's, those are there.
     auto multiply = [&](int kb, Block& v) {
         if (kb == kb0 || (kb & 3) == 0) {
 #pragma unroll
             for (int j = 0; j < NB; ++j) sb[j] = *reinterpret_cast<const uint32_t*>(tbs + (kb & ~3) + ssrc[j]);
         }
-#pragma unroll
-        for (int i = 0; i < MT; ++i) v.a[i].arrived();
-        asm volatile("" ::: "memory");
+        if (kb + 1 < kb1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NB) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         const uint8_t* st = stage + (kb & 1) * STAGE;
         const int sw = (l15 >> 1) & 7, sh = (kb & 3) * 8;
         i32x8 va[MT];
