@@ -925,7 +925,7 @@ template <typename T>
 int32_t f8_quantize_tiles(const char* who, const T* x, int64_t ldx, int64_t R, int64_t C, uint8_t* q, int64_t ldq, uint8_t* sc, int64_t lds, uint8_t* qt,
                           int64_t ldqt, uint8_t* st, int64_t ldst, float* colsum, float* part, hipStream_t s) {
     const int64_t rb = mh_ceil_div(R, 128), cb = mh_ceil_div(C, 128);
-    MH_REQUIRE(rb * cb < (int64_t)1 << 23, "%s: matrix too large for one launch (2^32 threads)", who);
+    MH_REQUIRE(rb * cb < (int64_t)1 << 23 && (!colsum || mh_ceil_div(C, 64) < (int64_t)1 << 22), "%s: matrix too large for one launch (2^32 threads)", who);
     if (!colsum) part = nullptr;
     if (q) MH_LAUNCH((fp8_quantize_tiles_kernel<T, true>), dim3((unsigned)(rb * cb)), dim3(512), 0, s, x, ldx, R, C, (int)cb, (int)rb, q, ldq, sc, lds, qt, ldqt, st, ldst, part);
     else MH_LAUNCH((fp8_quantize_tiles_kernel<T, false>), dim3((unsigned)(rb * cb)), dim3(512), 0, s, x, ldx, R, C, (int)cb, (int)rb, q, ldq, sc, lds, qt, ldqt, st, ldst, part);
