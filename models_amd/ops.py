@@ -2496,7 +2496,7 @@ def token_logprobs_backward(logits: torch.Tensor, ids: Optional[torch.Tensor], r
     for t, n in ((dlogp, "dlogp"), (dentropy, "dentropy"), (dlse, "dlse"), (result.entropy, "result.entropy")):
         _row_floats(t, (N,), n)
     _row_floats(result.stats, (N, 2), "result.stats")
-    if _elsewhere(logits, ids, result.stats, dlogp, dentropy, dlse, out):
+    if _elsewhere(logits, ids, result.stats, result.entropy, dlogp, dentropy, dlse, out):
         with torch.cuda.device(logits.device):
             return token_logprobs_backward(logits, ids, result, dlogp, dentropy, dlse, temperature, out)
     out = _dlogits(logits, out)
