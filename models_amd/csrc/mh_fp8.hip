@@ -1033,6 +1033,9 @@ int32_t mh_fp8_linear(const void* x, int32_t x_dtype, int64_t ldx, const void* w
     if (M <= FUSED_MOST) {
         MH_REQUIRE(x && ldx >= K, "mh_fp8_linear: x is NULL or its rows are shorter than %lld", (long long)K);
         MH_REQUIRE(x_dtype == MH_F32 || x_dtype == MH_BF16 || x_dtype == MH_F16, "mh_fp8_linear: unknown type %d", (int)x_dtype);
+        const int64_t xs = x_dtype == MH_F32 ? 4 : 2, os = out_dtype == MH_F32 ? 4 : 2;
+        MH_REQUIRE(!lp_shared(x, ldx * xs, K * xs, M, out, ldo * os, N * os, M), "mh_fp8_linear: out overlaps x, which up to %d rows read while out is written",
+                   FUSED_MOST);
         const F8Args g = f8_args(nullptr, 0, nullptr, 0, static_cast<const uint8_t*>(w), ldw, static_cast<const uint8_t*>(w_scales), ldws, M, N, K, bias, out_dtype,
                                  out, ldo);
         hipStream_t s = mh_stream(stream);

@@ -2133,6 +2133,7 @@ def route_local_rows(recv_keys: torch.Tensor, base: torch.Tensor, shard_rows: Op
 # --------------------------------------------------------------------------------------------
 _FLOATS = {torch.float32: _lib.MH_F32, torch.bfloat16: _lib.MH_BF16, torch.float16: _lib.MH_F16}
 _FP8_BLOCK = 128
+_FP8_FUSED_ROWS = 16  # mh_fp8_linear quantises as many rows of x on the way
 
 
 def _elsewhere(first: torch.Tensor, *others: Optional[torch.Tensor]) -> bool:
@@ -2287,7 +2288,7 @@ def fp8_quantize_both(x: torch.Tensor, column_sums: bool = False):
     return (m, mt, sums) if column_sums else (m, mt)
 
 
-def _fp8_out(M: int, N: int, out: Optional[torch.Tensor], out_dtype, device) -> torch.Tensor:
+def _fp8_out(M: int, N: int, out: Optional[torch.Tensor], out_dtype, device, bias: Optional[torch.Tensor], *operands: Fp8Matrix) -> torch.Tensor:
     if out_dtype not in _FLOATS:
         raise TypeError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
     if out is None:
@@ -2295,6 +2296,8 @@ def _fp8_out(M: int, N: int, out: Optional[torch.Tensor], out_dtype, device) -> 
     _float_2d(out, "out")
     if tuple(out.shape) != (M, N) or out.dtype != out_dtype:
         raise ValueError(f"out must be [{M}, {N}] of {out_dtype}, got {tuple(out.shape)} of {out.dtype}")
+    if (bias is not None and _shared(out, bias.view(1, -1))) or any(_shared(out, t) for m in operands for t in (m.values, m.scales)):
+        raise ValueError("out must not share memory with the 8-bit operands or the bias")
     return out
 
 
@@ -2320,7 +2323,7 @@ def fp8_matmul(a: Fp8Matrix, b: Fp8Matrix, bias: Optional[torch.Tensor] = None, 
     if _elsewhere(a.values, b.values, bias, out):
         with torch.cuda.device(a.values.device):
             return fp8_matmul(a, b, bias, out_dtype, out)
-    out = _fp8_out(M, N, out, out_dtype, a.values.device)
+    out = _fp8_out(M, N, out, out_dtype, a.values.device, bias, a, b)
     if M and N:
         need = lib.mh_fp8_matmul_workspace_bytes(M, N, K)
         ws = _scratch(need, out)
@@ -2334,8 +2337,8 @@ def fp8_matmul(a: Fp8Matrix, b: Fp8Matrix, bias: Optional[torch.Tensor] = None, 
 def fp8_linear(x: torch.Tensor, w: Fp8Matrix, bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """A Dense layer with 8-bit operands: ``x`` [M, K] quantised by blocks of 128 and multiplied with ``w``, the layer's kernel as
-    ``fp8_quantize(kernel, transpose=True)`` (``[N, K]``), made once.  Sums as ``fp8_matmul`` has them.  ``linear`` is the layer in 32
-    bits."""
+    ``fp8_quantize(kernel, transpose=True)`` (``[N, K]``), made once.  Sums as ``fp8_matmul`` has them.  ``out`` may
+    overlap ``x``, but not ``w`` or the bias.  ``linear`` is the layer in 32 bits."""
     lib = _lib.load()
     dt = _float_2d(x, "x")
     N, K = _fp8_check(w, "w")
@@ -2346,8 +2349,10 @@ def fp8_linear(x: torch.Tensor, w: Fp8Matrix, bias: Optional[torch.Tensor] = Non
     if _elsewhere(x, w.values, bias, out):
         with torch.cuda.device(x.device):
             return fp8_linear(x, w, bias, out_dtype, out)
-    out = _fp8_out(M, N, out, out_dtype, x.device)
+    given, out = out, _fp8_out(M, N, out, out_dtype, x.device, bias, w)
     if M and N:
+        if given is not None and M <= _FP8_FUSED_ROWS and _shared(x, out):  # quantised on the way, x would be read while out is written
+            return fp8_matmul(fp8_quantize(x), w, bias, out_dtype, out)
         need = lib.mh_fp8_linear_workspace_bytes(M, N, K)
         ws = _scratch(need, x)
         with _if_timed("fp8_linear", M * K * x.element_size() + N * K + M * N * out.element_size(), 2 * M * N * K):
