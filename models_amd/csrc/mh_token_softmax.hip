@@ -442,7 +442,7 @@ __device__ __forceinline__ void top_entries(const T* x, int n, int first, int k,
     }
     __syncthreads();
     int have = s.n;
-    if (have > CAND) {
+    if (__builtin_expect(have > CAND, 0)) {
         // The bound to its last bit (logits of 300 +- 1 are 2 apart in 16 bits), what lies above it, and the first of its ties: a row, or a part of one, of
         // one value, as masks of a finite value leave them, has more than LDS holds (4096 x 131072 bf16 with ten entries left, 20 alternatives: 557 us; a
         // search of the row for the threshold bit by bit took 8100).
@@ -459,7 +459,7 @@ __device__ __forceinline__ void top_entries(const T* x, int n, int first, int k,
         have = s.n;
         if (have < k) have = first_ties<NT>(x, n, first, low, have, k, s);
     }
-    if (have > CAND) {  // more large entries than that fell to the same few threads: look for the threshold in the row itself
+    if (__builtin_expect(have > CAND, 0)) {  // more large entries than that fell to the same few threads: look for the threshold in the row itself
         const uint64_t t = key_threshold(k, CAND, [&](uint64_t next) {
             int c = 0;
             each_entry<NT>(x, n, [&](const float(&l)[VE], int at) {
