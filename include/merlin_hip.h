@@ -741,9 +741,9 @@ int32_t mh_fp8_linear(const void* x, int32_t x_dtype, int64_t ldx, const void* w
  * mh_token_logprobs: logp[n] = log softmax(z[n])[ids[n]] (0 where ids[n] is outside [0, V): padding; ids and logp may be NULL), entropy[n],
  * lse[n] = log sum exp z[n], and the k (<= 256, <= V) largest entries of each row, ties to the lowest index: top_ids [N, k] and their log
  * probabilities top_logp [N, k]; places past the row's unmasked entries hold -1 and -inf, NaN is never an alternative.  stats [N, 2]: for _bwd.
- * mh_token_logprobs_bwd: dlogits [N, V] (leading dimension ldd, type of logits, all V columns written; may be logits itself with ldd = ld, and shares no
- * memory with them otherwise) =
- * dlogp (onehot - p) - dentropy p (log p + entropy) + dlse p, over temperature.  dlogp / dentropy / dlse [N] or NULL (zero). */
+ * mh_token_logprobs_bwd: dlogits [N, V] (leading dimension ldd, type of logits, all V columns written; may be logits itself with ldd = ld, and
+ * shares no memory with them otherwise) = dlogp (onehot - p) - dentropy p (log p + entropy) + dlse p, over temperature.  dlogp / dentropy / dlse
+ * [N] or NULL (zero). */
 int64_t mh_token_logprobs_workspace_bytes(int64_t N, int64_t V, int32_t k);
 int32_t mh_token_logprobs(const void* logits, int32_t dtype, int64_t ld, int64_t N, int64_t V, const void* ids, int32_t ids_dtype, int32_t k,
                           float temperature, float* logp, float* entropy, float* lse, float* top_logp, int32_t* top_ids, float* stats,
@@ -752,11 +752,13 @@ int32_t mh_token_logprobs_bwd(const void* logits, int32_t dtype, int64_t ld, int
                               float temperature, const float* stats, const float* entropy, const float* dlogp, const float* dentropy,
                               const float* dlse, void* dlogits, int64_t ldd, mh_stream_t stream);
 /* CategoricalCrossEntropy against a teacher's few entries (tf/losses/listwise.py:38-52 with soft targets), as a Kullback-Leibler divergence.
- * teacher_ids / teacher_logp [N, K], K <= 256, leading dimensions ld_ids / ld_logp: ids outside [0, V) are left out; an id given twice counts with both masses.  tail == 0: q =
- * softmax of the row's entries of teacher_logp (any constant may be added to a row); tail != 0: q = exp(teacher_logp), and what is left of 1
- * is held against the student's probability outside the entries.  loss[n] = sum q (log q - log p) (+ r (log r - log p_rest)); a row without
- * entries has loss 0 and no gradient; one whose student row is masked throughout has loss +inf and no gradient.  stats [N, 3] and top_grad
- * [N, K] (both or neither NULL) are for _bwd: dlogits = dloss[n] (1 where dloss is NULL) * d loss / d logits, may be logits itself, as above. */
+ * teacher_ids / teacher_logp [N, K], K <= 256, leading dimensions ld_ids / ld_logp: ids outside [0, V) are left out; an id given twice counts
+ * with both masses.  tail == 0: q = softmax of the row's entries of teacher_logp (any constant may be added to a row); tail != 0: q =
+ * exp(teacher_logp), and what is left of 1, r, is held against the student's probability outside the entries (and dropped where the student
+ * has no unmasked column there).  loss[n] = sum q (log q - log p) (+ r (log r - log p_rest)); a row without entries has loss 0 and no
+ * gradient; one whose student row is masked throughout has loss +inf (0 if its entries have no mass) and no gradient.  stats [N, 3] and
+ * top_grad [N, K] (both or neither NULL) are for _bwd: dlogits = dloss[n] (1 where dloss is NULL) * d loss / d logits, may be logits itself,
+ * as above. */
 int64_t mh_distill_topk_workspace_bytes(int64_t N, int64_t V, int32_t tail);
 int32_t mh_distill_topk(const void* logits, int32_t dtype, int64_t ld, int64_t N, int64_t V, const void* teacher_ids, int32_t ids_dtype,
                         int64_t ld_ids, const float* teacher_logp, int64_t ld_logp, int32_t K, float temperature, int32_t tail, float* loss,

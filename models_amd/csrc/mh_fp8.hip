@@ -56,7 +56,8 @@ __device__ __forceinline__ uint32_t q_pack4(float a, float b, float c, float d) 
 }
 
 // Blocks along the rows of x.  A wavefront takes four blocks (512 entries, 8 a lane: 16 lanes share a block) of one row and writes one word of
-// scales; one pass, bound by its reads and writes: 65536 x 3341 fp32 185 us, 5.9 TB/s; 65536 x 512 24 us, 7.0 TB/s.
+// scales; one pass, bound by its reads and writes: 65536 x 3341 fp32 201 us, 5.5 TB/s; 65536 x 512 25 us, 6.8 TB/s
+// (medians of a trace, as all kernel times in this file that are not set against another).
 template <typename T>
 __global__ __launch_bounds__(256) void fp8_quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t R, int K, int quads, uint8_t* __restrict__ q,
                                                                int64_t ldq, uint8_t* __restrict__ s, int64_t lds) {
@@ -99,8 +100,8 @@ __global__ __launch_bounds__(256) void fp8_quantize_rows_kernel(const T* __restr
 // eight rows of four columns.  The rows' maxima meet by halves -- 4, 2, 1 values, then two more steps -- which leaves row i's with lanes 4 i to
 // 4 i + 3 of its half wavefront; the columns' meet in LDS.  The tile turns round in LDS so that eight lanes write one 128-byte line of qt; sixteen
 // bytes chunk h of column c lie at h ^ ((c >> 2) & 7), or all 32 lanes of a write would meet in two banks.  colsum, if given, receives the tile's column
-// sums ([blocks, C]).  Bound by memory: 65536 x 512 fp32 26 us, 6.5 TB/s, and 33 us with ROWS (6.1 TB/s; the two forms apart 50); 65536 x 3341, whose rows
-// start at any word, 227 us, 4.8 TB/s.  Single columns in place of four neighbouring ones a lane took 26 us for 16384 x 1024, 16 now; the order of the
+// sums ([blocks, C]).  Bound by memory: 65536 x 512 fp32 26 us, 6.4 TB/s, and 34 us with ROWS (6.0 TB/s; the two forms apart 50); 65536 x 3341, whose rows
+// start at any word, 233 us, 4.7 TB/s.  Single columns in place of four neighbouring ones a lane took 26 us for 16384 x 1024, 16 now; the order of the
 // tiles made no difference.
 template <typename T, bool ROWS>
 __global__ __launch_bounds__(512) void fp8_quantize_tiles_kernel(const T* __restrict__ x, int64_t ldx, int64_t R, int64_t C, int cblocks, int rblocks,
@@ -311,8 +312,8 @@ __device__ __forceinline__ void f8_wave_fence() {
 // the operands is off by up to 2^-4 of each term already).  The finer types take the bf16 instruction, which adds in fp32, at half the rate.
 // Each wavefront holds (BM / WM) x (BN / WN) of the output as 32 x 32 accumulators, rows of b as the instruction's rows: a lane then owns four
 // neighbouring columns of C.  Tiles of one block of k (128 bytes a row) come by direct-to-LDS loads, two stages, one barrier a block; 16-byte
-// chunk c of row r lies at c ^ ((r >> 1) & 7), which spreads the 16 rows of a read phase over all 64 banks.  Bound by the matrix pipe: 8192^3 414 us, 2650
-// TFLOP/s, and WIDE 808 us, 1360 TFLOP/s; 65536 x 512 x 3341 WIDE 192 us, 1170 TFLOP/s.
+// chunk c of row r lies at c ^ ((r >> 1) & 7), which spreads the 16 rows of a read phase over all 64 banks.  Bound by the matrix pipe: 8192^3 463 us (440 at
+// best), 2380 TFLOP/s, and WIDE 809 us, 1360 TFLOP/s; 65536 x 512 x 3341 WIDE 226 us right behind the quantiser (185 at best), 990 TFLOP/s.
 template <int BM, int BN, int WM, int WN, bool WIDE>
 __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_gemm_kernel(const F8Args g) {
     constexpr int NT = WM * WN * 64, TM = BM / WM / 32, TN = BN / WN / 32;
@@ -562,8 +563,9 @@ struct F8Lane<f8_stored> {
 // wavefront's own, the next block's while one is multiplied, and no barrier is needed.  Partial sums meet in LDS in a fixed order and leave as
 // whole stretches of output rows.  X: the type of a where it is quantised on the way (at most 16 rows: the work is done again for every 16 NB
 // rows of b), or f8_stored.
-// 16 x 4096 -> 65536 45 us, 6.0 TB/s; 48 x 4096 -> 14341 20 us, 2.9 TB/s (225 workgroups, one round: what is left is its beginning and end); 1 x 1024 ->
-// 4096 4.6 us, nearly all of it a launch.
+// 16 x 4096 -> 65536 45 us, 6.1 TB/s; 48 x 4096 -> 14341 20 us, 3.0 TB/s (225 workgroups, one round, and the word of b's scales is asked for behind the next
+// block's lines, so that its use waits for those too: the two stages overlap between wavefronts, not within one); 1 x 1024 -> 4096 4.8 us, nearly all of it
+// a launch.
 constexpr int RW = 8;  // wavefronts
 template <int NB>
 constexpr int f8_rows_stage() {

@@ -444,7 +444,7 @@ __device__ __forceinline__ void top_entries(const T* x, int n, int first, int k,
     int have = s.n;
     if (__builtin_expect(have > CAND, 0)) {
         // The bound to its last bit (logits of 300 +- 1 are 2 apart in 16 bits), what lies above it, and the first of its ties: a row, or a part of one, of
-        // one value, as masks of a finite value leave them, has more than LDS holds (4096 x 131072 bf16 with ten entries left, 20 alternatives: 557 us; a
+        // one value, as masks of a finite value leave them, has more than LDS holds (4096 x 131072 bf16 with eleven entries left, 20 alternatives: 585 us; a
         // search of the row for the threshold bit by bit took 8100).
         __syncthreads();
         low = bound(0);
@@ -558,9 +558,9 @@ __device__ __forceinline__ void lp_emit(const LpArgs& g, int64_t row, const Sum&
     g.top_logp[row * g.k + place] = key ? lp_value(key_value((uint32_t)(key >> 32)), t, g.inv_t) : -INF;
 }
 
-// One read of the logits: 8192 x 32769 fp32 (rows at any word) 193 - 216 us, 5.0 - 5.6 TB/s; 64 x 1000000 fp32 with 100 alternatives 50 us, 5.1 TB/s;
-// 1 x 131072 bf16 with 20 alternatives 9.8 us in parts, the join behind it 7.3: both latency.  Eight wavefronts a SIMD are asked for where the compiler would
-// leave room for seven: 4096 x 16384 fp32, 20 alternatives, 51 us and 57.
+// One read of the logits: 8192 x 32769 fp32 (rows at any word) 216 us, 5.0 TB/s; 64 x 1000000 fp32 with 100 alternatives 51 us, 5.0 TB/s;
+// 1 x 131072 bf16 with 20 alternatives 9.6 us in parts, the join behind it 7.4: both latency.  Eight wavefronts a SIMD are asked for where the compiler would
+// leave room for seven: 4096 x 16384 fp32, 20 alternatives, 52 us and 58.
 template <int NT, typename T, bool TOP>
 __global__ __launch_bounds__(NT, TOP && NT == 512 ? 8 : 1) void token_logprobs_kernel(const LpArgs g) {
     __shared__ Sum red[NT / 64];
@@ -695,7 +695,7 @@ __device__ __forceinline__ void zero_row(T* d, int n) {
     if (threadIdx.x < n - nv * VE) lp_store(d + nv * VE + threadIdx.x, 0.f);
 }
 
-// 8192 x 32769 fp32 346 us, 6.2 TB/s read and written; 4096 x 131003 bf16 with the entropy's term 342 us, 6.3 TB/s.
+// 8192 x 32769 fp32 351 us, 6.1 TB/s read and written; 4096 x 131003 bf16 with the entropy's term 347 us, 6.2 TB/s.
 template <int NT, typename T>
 __global__ __launch_bounds__(NT) void token_logprobs_bwd_kernel(const GradArgs g) {
     const int64_t row = blockIdx.x / (uint32_t)g.parts;
@@ -931,8 +931,8 @@ __device__ __forceinline__ void ds_bits(const DsArgs& g, int64_t row, int c0, in
 }
 
 // The sums of a row, or a part of one, with a tail without the teacher's entries.  E != 0: a row a workgroup, which has one wavefront more for the
-// teacher's entries, done while the others read.  2048 x 50021 f16, 64 entries: 35 - 37 us, 5.5 - 5.9 TB/s; 4096 x 131072 bf16, 128 entries and a tail: 199 -
-// 230 us, 4.7 - 5.4 TB/s.
+// teacher's entries, done while the others read.  2048 x 50021 f16, 64 entries: 36 us, 5.6 TB/s; 4096 x 131072 bf16, 128 entries and a tail: 233 us
+// (200 at best), 4.6 TB/s.
 template <int NT, int E, typename T, bool TAIL>
 __global__ __launch_bounds__(NT + (E ? 64 : 0), E == 1 || E == 2 ? 8 : 1) void distill_topk_sums_kernel(const DsArgs g) {
     extern __shared__ uint32_t bits[];
@@ -953,7 +953,7 @@ __global__ __launch_bounds__(NT + (E ? 64 : 0), E == 1 || E == 2 ? 8 : 1) void d
     }
 }
 
-// 4096 x 131072 bf16, 128 entries: 323 us, 6.6 TB/s read and written.
+// 4096 x 131072 bf16, 128 entries: 327 us, 6.6 TB/s read and written.
 template <int NT, typename T>
 __global__ __launch_bounds__(NT) void distill_topk_bwd_kernel(const GradArgs g) {
     const int64_t row = blockIdx.x / (uint32_t)g.parts;

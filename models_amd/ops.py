@@ -2543,7 +2543,8 @@ def distill_topk(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logp: 
     """Kullback-Leibler divergence of ``softmax(logits / temperature)`` from a teacher of whom each row's top entries are known:
     ``teacher_ids`` [N, K] and ``teacher_logp`` [N, K], as ``token_logprobs(teacher_logits, k=K, temperature=temperature)`` gives them.
     ``tail=False``: the teacher's mass is the softmax of its K entries.  ``tail=True``: it is ``exp(teacher_logp)``, and what is left of 1 is
-    held against the student's probability outside the entries.  Ids outside [0, V) are left out; a row without any has loss 0."""
+    held against the student's probability outside the entries (and dropped where the student has no unmasked column there).  Ids outside
+    [0, V) are left out; a row without any has loss 0."""
     lib = _lib.load()
     dt, N, V, temperature = _catalogue(logits, temperature)
     if teacher_logp is None:
