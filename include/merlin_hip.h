@@ -716,7 +716,7 @@ int32_t mh_sharded_lookup_bwd(mh_comm_t comm, int32_t F, int64_t B, int64_t capa
  * bf16 where the terms cancel.  An MH_F32 output rounded to bf16 has its rounding alone.
  * mh_fp8_linear: x [M, K] in the form of mh_fp8_quantize (into the workspace, or on the way for few rows), then the product with w [N, K].
  * out shares no memory with the operands and the bias; it may overlap the x of mh_fp8_linear where that has more than 16 rows.
- * K <= 2^24 - 128, leading dimensions of 8-bit values and scales <= 2^24, M, N < 2^27; workspaces are 16-byte aligned.  In MH_F32 and MH_F16 outputs an
+ * K <= 2^24 - 128, leading dimensions of 8-bit values and scales <= 2^24, M, N < 2^27; workspaces are 16-byte aligned.  Where sums are in 32 bits an
  * operand's value under 2^-126 may count as 0 and one that rounds to 2^128 is infinite.
  * No atomics: results do not change from call to call.  Rows past M and columns past N of out are left as they were. */
 int32_t mh_fp8_quantize(const void* x, int32_t dtype, int64_t ldx, int64_t R, int64_t K, int32_t transpose, void* q, int64_t ldq,
